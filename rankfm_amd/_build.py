@@ -20,7 +20,10 @@ ARCH = "gfx950"
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-ffp-contract=off",
          "-Wall", "-Wno-unused-function",
          # LDS / memory atomics of a few lanes on one address are cheaper left to the hardware than turned into a scalar loop
-         "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
+         "-mllvm", "-amdgpu-atomic-optimizer-strategy=None",
+         # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have returned wrong results on the target machines.
+         # (hipcc's host pass does not know the feature and says so: harmless)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
