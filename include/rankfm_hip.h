@@ -282,6 +282,95 @@ int rfm_recommend_host(const rfm_model_view *host_model, int64_t n_rec_users, co
 #define RFM_SIMILAR_USERS 1
 int rfm_similar_host(const rfm_model_view *host_model, int32_t kind, int32_t index, int32_t n, float *out, int device);
 
+/* ---- Rows of catalogue scores (no reference counterpart: the reference hands out ranked items only and knows one rule,
+ * filter_previous).  `scores` of the entry points below: n_rows rows of n_items, `stride` elements apart, of element type RFM_F32 / RFM_F16 /
+ * RFM_BF16; arithmetic is fp32.  Everything is enqueued on `hip_stream` without synchronising, and may be captured. ---- */
+#define RFM_F32 0
+#define RFM_F16 1
+#define RFM_BF16 2
+
+/* score rows of the model: float32 [n, n_items], row-major; users float32 [n] indexes, rows of unknown users (NaN) come out NaN.
+ * Scores are compute_ui_utility's (rankfm/_rankfm.pyx:48-89) up to summation order. */
+size_t rfm_scores_workspace_bytes(const rfm_model_view *model, int64_t n_users);
+int rfm_scores_device(const rfm_model_view *dev_model, int64_t n_users, const float *dev_users, float *dev_scores, void *workspace,
+                      size_t workspace_bytes, void *hip_stream);
+
+/* the factored form of the same scores: score(u, i) = bias[i] + < user_rows[u], item_rows[i] >, rows of `rfm_effective_factors()` floats:
+ * [ v_u + x_uf.v_uf | v_u ] and [ v_i | x_if.v_if ] (the second halves only with item features), padded with zeros to a multiple of 32.
+ * dev_users NULL: no user rows are made.  dev_item_rows / dev_bias NULL: no item rows are made. */
+int32_t rfm_effective_factors(const rfm_model_view *model);
+int rfm_effective_factors_device(const rfm_model_view *dev_model, int64_t n_users, const float *dev_users, float *dev_user_rows,
+                                 float *dev_item_rows, float *dev_bias, void *hip_stream);
+
+/* What is done to the score s of item i in row r, c being the number of times i stands in the row's history; in this order, every operation
+ * rounded once in fp32, the result once to the element type:
+ *   c > 0:                     s = s > 0 ? s / repetition : s * repetition;  s = s - frequency * c;  s = s - presence
+ *   item_bias:                 s = s + item_bias[i]
+ *   row r's biases name i:     s = s + the value of the LAST entry that does
+ *   i is not allowed in row r: s = -inf, whatever it was
+ * Every array is optional (NULL).  Items outside [0, n_items) in a list are skipped.  A row that names a history or a mask behind the last
+ * one comes out NaN (and has no top scores); a negative one means none. */
+typedef struct rfm_score_rules {
+    const int64_t *history_offsets;   /* [n_history + 1] into history_items: lists in any order, with repeats */
+    const int32_t *history_items;     /* [n_history_items] */
+    const int32_t *history_rows;      /* [n_rows] the list of each row; NULL: row r has list r */
+    int64_t n_history, n_history_items;
+    const float *repetition;          /* [n_rows] > 0, or NULL: repetition_all (1 = off) */
+    const float *frequency;           /* [n_rows], or NULL: frequency_all (0 = off) */
+    const float *presence;            /* [n_rows], or NULL: presence_all (0 = off) */
+    float repetition_all, frequency_all, presence_all;
+    int32_t reserved;                 /* 0 */
+    const float *item_bias;           /* [n_items] */
+    const int64_t *bias_offsets;      /* [n_rows + 1] into bias_items / bias_values: the row's own biases */
+    const int32_t *bias_items;        /* [n_bias_items] */
+    const float *bias_values;         /* [n_bias_items] */
+    int64_t n_bias_items;
+    const uint32_t *allowed;          /* [n_allowed, ceil(n_items / 32)]: bit b of word w allows item 32 w + b */
+    const int32_t *allowed_rows;      /* [n_rows] the mask of each row; NULL: row r has mask r, or all rows the one there is */
+    int64_t n_allowed;
+} rfm_score_rules;
+
+/* out = rules(scores); `out` may be `scores` itself (same stride), and must not overlap it otherwise */
+int rfm_adjust_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_t n_rows, int32_t n_items, const void *dev_scores, int64_t stride,
+                             void *dev_out, int64_t out_stride, void *hip_stream);
+
+/* the n best items of every row under `rules` (NULL: none) by descending score, the lower index first among equals, and their scores:
+ * int32 / float32 [n_rows, n].  NaN and -inf never rank; rows with fewer than n ranking items end in (-1, -inf). */
+size_t rfm_top_scores_workspace_bytes(int64_t n_rows, int32_t n_items, int32_t n);
+int rfm_top_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_t n_rows, int32_t n_items, const void *dev_scores, int64_t stride,
+                          int32_t n, int32_t *dev_items, float *dev_values, void *workspace, size_t workspace_bytes, void *hip_stream);
+
+/* ---- Learning from another model's answers (no reference counterpart).  Student: z[r, i] = < users[r], items[i] > + bias[i].
+ * Teacher: n_teacher items and scores per row (such as rfm_top_scores_device makes).  With q = softmax(z / temperature) over the allowed
+ * items and p = softmax(teacher score / temperature) over the row's usable entries (item in [0, n_items) and allowed, score not -inf; an
+ * item that stands there twice counts twice):
+ *   loss[r]  = temperature^2 * sum_j p_j (log p_j - log q[item_j])             a row without a usable entry: 0
+ *   gradients of sum_r row_weight[r] * loss[r]:  with dz = temperature * row_weight * (q - p) (a row without a usable entry: 0)
+ *   d_users = dz . items    d_items = dz^T . users    d_bias = column sums of dz
+ * All of it float32 in and out; no array of the size n_rows x n_items of scores is kept (a block of rows is, above 128 factors).
+ * d_users = d_items = d_bias = NULL: the loss alone.  A row that names a mask behind the last one has loss NaN. ---- */
+typedef struct rfm_distill_args {
+    int64_t n_rows;
+    int32_t n_items, n_factors, n_teacher;
+    float temperature;                /* > 0 */
+    const float *users;               /* [n_rows, n_factors], rows user_stride apart */
+    const float *items;               /* [n_items, n_factors], rows item_stride apart */
+    int64_t user_stride, item_stride;
+    const float *bias;                /* [n_items] or NULL */
+    const int32_t *teacher_items;     /* [n_rows, n_teacher] */
+    const float *teacher_scores;      /* [n_rows, n_teacher] */
+    const uint32_t *allowed;          /* [n_allowed, ceil(n_items / 32)] or NULL, as in rfm_score_rules */
+    const int32_t *allowed_rows;      /* [n_rows] or NULL */
+    int64_t n_allowed;
+    const float *row_weight;          /* [n_rows] or NULL: 1 */
+    float *loss;                      /* [n_rows] */
+    float *d_users;                   /* [n_rows, n_factors] */
+    float *d_items;                   /* [n_items, n_factors] */
+    float *d_bias;                    /* [n_items], or NULL */
+} rfm_distill_args;
+size_t rfm_distill_workspace_bytes(const rfm_distill_args *args);
+int rfm_distill_device(const rfm_distill_args *dev, void *workspace, size_t workspace_bytes, void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,3 +10,15 @@ from ._rankfm import DEFAULT_ENGINE, REFERENCE_ENGINE, EngineOptions, UserItemsC
 from .rankfm import RankFM   # noqa: F401
 
 __version__ = "0.1.0"
+
+# what works on torch tensors is imported when it is first asked for: the rest of the package does without PyTorch
+_ON_TENSORS = {"ScoreRules": "scores", "TopScores": "scores", "adjust_scores": "scores", "pack_allowed": "scores", "top_scores": "scores",
+               "DistillGradients": "distill", "distill_gradients": "distill", "distill_loss": "distill"}
+
+
+def __getattr__(name):
+    if name not in _ON_TENSORS:
+        raise AttributeError("module %r has no attribute %r" % (__name__, name))
+    from importlib import import_module
+    value = globals()[name] = getattr(import_module("." + _ON_TENSORS[name], __name__), name)
+    return value

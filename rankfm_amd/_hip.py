@@ -17,6 +17,7 @@ ERR_NONFINITE = 100
 SCHEDULE_CONSTANT, SCHEDULE_INVSCALING = 0, 1
 MODE_HOGWILD, MODE_SERIAL = 0, 1
 RNG_MT19937, RNG_COUNTER = 0, 1
+F32, F16, BF16 = 0, 1, 2       # element types of score rows
 REFERENCE_MT_SEED = 1492       # rankfm/_rankfm.pyx:182
 
 
@@ -113,12 +114,38 @@ class ModelView(C.Structure):
     ]
 
 
+class ScoreRulesStruct(C.Structure):
+    """rfm_score_rules"""
+    _fields_ = [
+        ("history_offsets", C.c_void_p), ("history_items", C.c_void_p), ("history_rows", C.c_void_p),
+        ("n_history", C.c_int64), ("n_history_items", C.c_int64),
+        ("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p),
+        ("repetition_all", C.c_float), ("frequency_all", C.c_float), ("presence_all", C.c_float), ("reserved", C.c_int32),
+        ("item_bias", C.c_void_p),
+        ("bias_offsets", C.c_void_p), ("bias_items", C.c_void_p), ("bias_values", C.c_void_p), ("n_bias_items", C.c_int64),
+        ("allowed", C.c_void_p), ("allowed_rows", C.c_void_p), ("n_allowed", C.c_int64),
+    ]
+
+
+class DistillArgs(C.Structure):
+    """rfm_distill_args"""
+    _fields_ = [
+        ("n_rows", C.c_int64), ("n_items", C.c_int32), ("n_factors", C.c_int32), ("n_teacher", C.c_int32), ("temperature", C.c_float),
+        ("users", C.c_void_p), ("items", C.c_void_p), ("user_stride", C.c_int64), ("item_stride", C.c_int64), ("bias", C.c_void_p),
+        ("teacher_items", C.c_void_p), ("teacher_scores", C.c_void_p),
+        ("allowed", C.c_void_p), ("allowed_rows", C.c_void_p), ("n_allowed", C.c_int64), ("row_weight", C.c_void_p),
+        ("loss", C.c_void_p), ("d_users", C.c_void_p), ("d_items", C.c_void_p), ("d_bias", C.c_void_p),
+    ]
+
+
 # every symbol include/rankfm_hip.h declares (tests check the library exports all of them)
 EXPORTS = (
     "rfm_abi_version", "rfm_status_string", "rfm_last_error", "rfm_device_count", "rfm_fit_supported",
     "rfm_fit_workspace_bytes", "rfm_fit_device", "rfm_fit_host", "rfm_fit_export_weights", "rfm_predict_device", "rfm_predict_host",
     "rfm_recommend_device", "rfm_recommend_workspace_bytes", "rfm_recommend_host", "rfm_similar_host", "rfm_hbm_probe",
     "rfm_delta_begin", "rfm_delta_finish", "rfm_release_cache",
+    "rfm_scores_workspace_bytes", "rfm_scores_device", "rfm_effective_factors", "rfm_effective_factors_device",
+    "rfm_adjust_scores_device", "rfm_top_scores_workspace_bytes", "rfm_top_scores_device", "rfm_distill_workspace_bytes", "rfm_distill_device",
 )
 
 _lib = None
@@ -184,6 +211,26 @@ def lib():
     L.rfm_release_cache.restype = None
     L.rfm_similar_host.restype = C.c_int
     L.rfm_similar_host.argtypes = [C.POINTER(ModelView), C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int]
+    L.rfm_scores_workspace_bytes.restype = C.c_size_t
+    L.rfm_scores_workspace_bytes.argtypes = [C.POINTER(ModelView), C.c_int64]
+    L.rfm_scores_device.restype = C.c_int
+    L.rfm_scores_device.argtypes = [C.POINTER(ModelView), C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.rfm_effective_factors.restype = C.c_int32
+    L.rfm_effective_factors.argtypes = [C.POINTER(ModelView)]
+    L.rfm_effective_factors_device.restype = C.c_int
+    L.rfm_effective_factors_device.argtypes = [C.POINTER(ModelView), C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    L.rfm_adjust_scores_device.restype = C.c_int
+    L.rfm_adjust_scores_device.argtypes = [C.POINTER(ScoreRulesStruct), C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                           C.c_int64, C.c_void_p]
+    L.rfm_top_scores_workspace_bytes.restype = C.c_size_t
+    L.rfm_top_scores_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
+    L.rfm_top_scores_device.restype = C.c_int
+    L.rfm_top_scores_device.argtypes = [C.POINTER(ScoreRulesStruct), C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.rfm_distill_workspace_bytes.restype = C.c_size_t
+    L.rfm_distill_workspace_bytes.argtypes = [C.POINTER(DistillArgs)]
+    L.rfm_distill_device.restype = C.c_int
+    L.rfm_distill_device.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_size_t, C.c_void_p]
     if L.rfm_abi_version() != ABI_VERSION:
         raise EngineUnavailable("librankfm_hip.so ABI %d != binding ABI %d: rebuild" % (L.rfm_abi_version(), ABI_VERSION))
     _lib = L

@@ -178,6 +178,13 @@ __global__ void __launch_bounds__(256) scores_mfma_kernel(const float *__restric
     }
 }
 
+// rows of unknown users (rankfm/_rankfm.pyx:435-437): NaN
+__global__ void __launch_bounds__(256) unknown_rows_kernel(const float *__restrict__ users, int n_items, float *__restrict__ scores) {
+    const long long slot = blockIdx.x;
+    if (!isnan(users[slot])) return;
+    for (int i = threadIdx.x; i < n_items; i += blockDim.x) scores[(size_t)slot * n_items + i] = __uint_as_float(0x7fc00000u);
+}
+
 // one block per user slot: optionally knock out the user's observed items, then n_rec rounds of block-wide argmax.
 // Ranking is descending by utility; equal scores may come out in any order (np.argsort in the reference is
 // unstable too, rankfm/_rankfm.pyx:444).
@@ -1015,6 +1022,50 @@ int rfm_recommend_host(const rfm_model_view *hm, int64_t n_users, const float *u
     if (rc != RFM_OK) (void)hipDeviceSynchronize();      // (nothing of a failed call may still be running on the arena)
     arena_done(arena);
     return rc;
+}
+
+// score rows handed out as they are (rfm_top_scores_device / rfm_adjust_scores_device work on them): the chunked path's product, no ranking.
+// workspace: veff [I, Kp] | bias [I] | ueff [chunk, Kp]
+constexpr long long kScoreChunk = 65536;
+size_t rfm_scores_workspace_bytes(const rfm_model_view *m, int64_t n_users) {
+    if (check_model(m) != RFM_OK || n_users < 0) return 0;
+    const size_t chunk = (size_t)(n_users < kScoreChunk ? (n_users > 0 ? n_users : 1) : kScoreChunk), kp = (size_t)padded_k(m), I = (size_t)m->n_items;
+    return sizeof(float) * (I * kp + I + chunk * kp) + 1024;
+}
+
+int rfm_scores_device(const rfm_model_view *m, int64_t n_users, const float *users, float *scores, void *workspace, size_t workspace_bytes, void *hip_stream) {
+    int rc = check_model(m);
+    if (rc != RFM_OK) return rc;
+    if (n_users < 0 || (n_users > 0 && (!users || !scores))) return RFM_ERR_BAD_ARG;
+    if (n_users == 0) return RFM_OK;
+    if (!workspace || workspace_bytes < rfm_scores_workspace_bytes(m, n_users)) return RFM_ERR_WORKSPACE;
+    hipStream_t stream = (hipStream_t)hip_stream;
+    const int kp = padded_k(m);
+    const size_t I = (size_t)m->n_items;
+    auto up256 = [](size_t x) { return (x + 63) & ~(size_t)63; };
+    float *veff = (float *)workspace, *bias = veff + up256(I * kp), *ueff = bias + up256(I);
+    build_veff_kernel<<<dim3(512), dim3(256), 0, stream>>>(*m, kp, veff, bias);
+    for (long long u0 = 0; u0 < n_users; u0 += kScoreChunk) {
+        const long long nu = (n_users - u0) < kScoreChunk ? (n_users - u0) : kScoreChunk;
+        float *rows = scores + (size_t)u0 * I;
+        build_ueff_kernel<<<dim3(256), dim3(256), 0, stream>>>(*m, users, u0, (int)nu, kp, ueff);
+        scores_mfma_kernel<<<dim3((unsigned)((I + 63) / 64), (unsigned)((nu + 63) / 64)), dim3(256), 0, stream>>>(ueff, veff, bias, (int)nu, m->n_items, kp, rows);
+        unknown_rows_kernel<<<dim3((unsigned)nu), dim3(256), 0, stream>>>(users + u0, m->n_items, rows);
+    }
+    return hipGetLastError() == hipSuccess ? RFM_OK : RFM_ERR_HIP;
+}
+
+int32_t rfm_effective_factors(const rfm_model_view *m) { return check_model(m) == RFM_OK ? padded_k(m) : 0; }
+
+int rfm_effective_factors_device(const rfm_model_view *m, int64_t n_users, const float *users, float *user_rows, float *item_rows, float *bias, void *hip_stream) {
+    int rc = check_model(m);
+    if (rc != RFM_OK) return rc;
+    if (n_users < 0 || n_users > 0x7fffffff || (users && n_users > 0 && !user_rows) || (!item_rows != !bias)) return RFM_ERR_BAD_ARG;
+    hipStream_t stream = (hipStream_t)hip_stream;
+    const int kp = padded_k(m);
+    if (item_rows) build_veff_kernel<<<dim3(512), dim3(256), 0, stream>>>(*m, kp, item_rows, bias);
+    if (users && n_users > 0) build_ueff_kernel<<<dim3(256), dim3(256), 0, stream>>>(*m, users, 0, (int)n_users, kp, user_rows);
+    return hipGetLastError() == hipSuccess ? RFM_OK : RFM_ERR_HIP;
 }
 
 // (called by rfm_release_cache, rfm_api.hip)

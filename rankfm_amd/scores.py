@@ -1,0 +1,219 @@
+"""Rows of catalogue scores on the device: rules applied to them (`adjust_scores`) and their best entries (`top_scores`).
+
+The reference hands out ranked items only and knows one rule, `filter_previous` (rankfm/_rankfm.pyx:450-451).  Here the caller says what
+else holds: penalties for what a user has already had, biases, and masks of what may be shown at all.  Tensors are torch tensors on one
+MI355X; work is enqueued on that device's current stream and nothing synchronises, so the calls may be captured into a graph.
+"""
+import ctypes as C
+from dataclasses import dataclass
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import _hip
+
+_DTYPES = {torch.float32: _hip.F32, torch.float16: _hip.F16, torch.bfloat16: _hip.BF16}
+
+
+@dataclass
+class ScoreRules:
+    """what holds for the rows of a call; every field is optional, tensors live on the scores' device
+
+    In this order, c being how often item i stands in the row's history and each operation rounded once in float32:
+
+        c > 0:                   s = s / repetition if s > 0 else s * repetition;  s -= frequency * c;  s -= presence
+        item_bias:               s += item_bias[i]
+        row_bias names i:        s += the value of the last entry that does
+        i is not allowed:        s = -inf, whatever it was
+
+    history        (offsets int64 [H + 1], items int32): lists in any order, with repeats
+    history_rows   int32 [rows], the list of each row (negative: none); without it row r has list r
+    repetition, frequency, presence    a number for all rows or float32 [rows]; they need `history`
+    item_bias      float32 [items]
+    row_bias       (offsets int64 [rows + 1], items int32, values float32): the rows' own biases
+    allowed        int32 [masks, ceil(items / 32)]: bit b of word w allows item 32 w + b (`pack_allowed` makes it)
+    allowed_rows   int32 [rows], the mask of each row (negative: none); without it row r has mask r, or every row the only one
+
+    Items outside the catalogue in a list are skipped.  A row that names a history or a mask behind the last one comes out NaN.
+    """
+    history: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+    history_rows: Optional[torch.Tensor] = None
+    repetition: Union[float, torch.Tensor] = 1.0
+    frequency: Union[float, torch.Tensor] = 0.0
+    presence: Union[float, torch.Tensor] = 0.0
+    item_bias: Optional[torch.Tensor] = None
+    row_bias: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
+    allowed: Optional[torch.Tensor] = None
+    allowed_rows: Optional[torch.Tensor] = None
+
+    def penalises(self):
+        """whether the rules look at a history at all"""
+        return any(isinstance(v, torch.Tensor) or v != off for v, off in ((self.repetition, 1.0), (self.frequency, 0.0), (self.presence, 0.0)))
+
+
+class TopScores(NamedTuple):
+    """int32 / float32 [rows, n]: items by descending score and the scores; -1 and -inf behind the last ranking item"""
+    items: torch.Tensor
+    scores: torch.Tensor
+
+
+def pack_allowed(mask):
+    """bool [masks, items] -> int32 [masks, ceil(items / 32)], bit b of word w for item 32 w + b"""
+    if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool or mask.dim() != 2:
+        raise ValueError("[mask] must be a bool tensor [masks, items]")
+    words = (mask.shape[1] + 31) // 32
+    full = torch.zeros((mask.shape[0], words * 32), dtype=torch.bool, device=mask.device)
+    full[:, :mask.shape[1]] = mask
+    value = (full.view(mask.shape[0], words, 32).long() << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(value >= 2 ** 31, value - 2 ** 32, value).int()
+
+
+def check_tensor(t, name, dtype, shape, device):
+    """a contiguous tensor of this type and shape (None: any size) on this device, or ValueError"""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError("[%s] must be a torch tensor" % name)
+    if t.dtype != dtype:
+        raise ValueError("[%s] must be %s, got %s" % (name, str(dtype).replace("torch.", ""), str(t.dtype).replace("torch.", "")))
+    if t.dim() != len(shape) or any(w is not None and g != w for g, w in zip(t.shape, shape)):
+        raise ValueError("[%s] must have shape %s, got %s" % (name, list(shape), list(t.shape)))
+    if t.device != device:
+        raise ValueError("[%s] is on %s, the call on %s" % (name, t.device, device))
+    if not t.is_contiguous():
+        raise ValueError("[%s] must be contiguous" % name)
+    return t.data_ptr()
+
+
+def check_device(t, name):
+    if t.device.type != "cuda":
+        if not torch.cuda.is_available():
+            raise _hip.EngineUnavailable("no MI355X visible to PyTorch-ROCm: rankfm_amd has no CPU fallback")
+        raise ValueError("[%s] must be on the GPU" % name)
+    return t.device
+
+
+def _check_scores(scores):
+    if not isinstance(scores, torch.Tensor) or scores.dtype not in _DTYPES or scores.dim() != 2:
+        raise ValueError("[scores] must be a float32, float16 or bfloat16 tensor [rows, items]")
+    if scores.shape[1] < 1:
+        raise ValueError("[scores] must have at least one item")
+    if scores.shape[1] > 1 and scores.stride(1) != 1 or scores.shape[0] > 1 and scores.stride(0) < scores.shape[1]:
+        raise ValueError("[scores] must have rows of consecutive items that do not overlap")
+    return check_device(scores, "scores")
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _number_or_rows(u, name, value, rows, device):
+    if isinstance(value, torch.Tensor):
+        setattr(u, name, check_tensor(value, name, torch.float32, (rows,), device))
+    else:
+        value = float(value)
+        if not (value > 0.0 if name == "repetition" else value == value) or value in (float("inf"), float("-inf")):
+            raise ValueError("[%s] must be a finite number%s" % (name, " above 0" if name == "repetition" else ""))
+        setattr(u, name + "_all", value)
+
+
+def allowed_fields(u, allowed, allowed_rows, rows, items, device):
+    """the mask fields of rfm_score_rules / rfm_distill_args"""
+    if allowed is None:
+        if allowed_rows is not None:
+            raise ValueError("[allowed_rows] needs [allowed]")
+        return
+    u.allowed = check_tensor(allowed, "allowed", torch.int32, (None, (items + 31) // 32), device)
+    u.n_allowed = allowed.shape[0]
+    if u.n_allowed < 1:
+        raise ValueError("[allowed] must hold at least one mask")
+    if allowed_rows is not None:
+        u.allowed_rows = check_tensor(allowed_rows, "allowed_rows", torch.int32, (rows,), device)
+    elif u.n_allowed not in (1, rows):
+        raise ValueError("[allowed] must hold one mask, or one per row, or be given [allowed_rows]")
+
+
+def _rules_struct(rules, rows, items, device):
+    if not isinstance(rules, ScoreRules):
+        raise ValueError("[rules] must be a rankfm_amd.ScoreRules")
+    u = _hip.ScoreRulesStruct(repetition_all=1.0)
+    if rules.history is not None:
+        offsets, listed = rules.history
+        u.history_offsets = check_tensor(offsets, "history offsets", torch.int64, (None,), device)
+        u.history_items = check_tensor(listed, "history items", torch.int32, (None,), device)
+        u.n_history, u.n_history_items = offsets.shape[0] - 1, listed.shape[0]
+        if u.n_history < 0:
+            raise ValueError("[history offsets] must have at least one entry")
+        if rules.history_rows is not None:
+            u.history_rows = check_tensor(rules.history_rows, "history_rows", torch.int32, (rows,), device)
+        elif u.n_history != rows:
+            raise ValueError("[history] must hold one list per row, or be given [history_rows]")
+        for name in ("repetition", "frequency", "presence"):
+            _number_or_rows(u, name, getattr(rules, name), rows, device)
+    elif rules.history_rows is not None or rules.penalises():
+        raise ValueError("[repetition], [frequency], [presence] and [history_rows] need [history]")
+    if rules.item_bias is not None:
+        u.item_bias = check_tensor(rules.item_bias, "item_bias", torch.float32, (items,), device)
+    if rules.row_bias is not None:
+        offsets, listed, values = rules.row_bias
+        u.bias_offsets = check_tensor(offsets, "row_bias offsets", torch.int64, (rows + 1,), device)
+        u.bias_items = check_tensor(listed, "row_bias items", torch.int32, (None,), device)
+        u.bias_values = check_tensor(values, "row_bias values", torch.float32, tuple(listed.shape), device)
+        u.n_bias_items = listed.shape[0]
+    allowed_fields(u, rules.allowed, rules.allowed_rows, rows, items, device)
+    return u
+
+
+def _byte_range(t):
+    return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()
+
+
+def adjust_scores(scores, rules, out=None):
+    """the score rows under the rules, rounded once to the scores' type
+
+    scores   float32, float16 or bfloat16 [rows, items], rows of consecutive items (the rows themselves may be strided)
+    out      None (a new tensor), `scores` itself (in place), or a tensor of the same type and shape that does not overlap it
+    """
+    device = _check_scores(scores)
+    rows, items = scores.shape
+    if out is None:
+        out = torch.empty((rows, items), dtype=scores.dtype, device=device)
+    elif out is not scores:
+        if not isinstance(out, torch.Tensor) or out.dtype != scores.dtype or out.shape != scores.shape or out.device != device:
+            raise ValueError("[out] must be a tensor of the scores' type, shape and device")
+        if items > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < items:
+            raise ValueError("[out] must have rows of consecutive items that do not overlap")
+        if rows and (out.data_ptr(), out.stride()) != (scores.data_ptr(), scores.stride()):
+            (a, b), (c, d) = _byte_range(scores), _byte_range(out)
+            if a < d and c < b:
+                raise ValueError("[out] must be [scores] itself or not overlap it")
+    u = _rules_struct(rules, rows, items, device)
+    if rows == 0:
+        return out
+    with torch.cuda.device(device):
+        rc = _hip.lib().rfm_adjust_scores_device(C.byref(u), _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), out.data_ptr(),
+                                                 _row_stride(out), torch.cuda.current_stream(device).cuda_stream)
+    _hip.raise_for_status(rc)
+    return out
+
+
+def top_scores(scores, n, rules=None):
+    """the `n` best items of every row and their scores under the rules: `TopScores(items, scores)`
+
+    By descending score, the lower index first among equals; NaN and -inf never rank.  The adjusted rows are not written anywhere.
+    """
+    device = _check_scores(scores)
+    rows, items = scores.shape
+    n = int(n)
+    if n < 1 or n > items:
+        raise ValueError("[n] must be between 1 and the number of items")
+    u = None if rules is None else _rules_struct(rules, rows, items, device)
+    best = torch.empty((rows, n), dtype=torch.int32, device=device)
+    value = torch.empty((rows, n), dtype=torch.float32, device=device)
+    if rows == 0:
+        return TopScores(best, value)
+    lib = _hip.lib()
+    with torch.cuda.device(device):
+        ws = torch.empty(lib.rfm_top_scores_workspace_bytes(rows, items, n), dtype=torch.uint8, device=device)
+        rc = lib.rfm_top_scores_device(C.byref(u) if u is not None else None, _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), n,
+                                       best.data_ptr(), value.data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(device).cuda_stream)
+    _hip.raise_for_status(rc)
+    return TopScores(best, value)
