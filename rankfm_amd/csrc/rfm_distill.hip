@@ -5,7 +5,10 @@
 //   loss[r] = tau^2 sum_j p_j (log p_j - z[r, t_j] / tau + lse_r),   lse_r = log sum_i exp(z[r, i] / tau)
 //   dz = tau * weight[r] * (q - p);   d_users = dz . items;   d_items = dz^T . users;   d_bias = column sums of dz
 //
-// The matrix path: the scores of a block of rows are written out, turned into dz in place and multiplied; every sum has a fixed order.
+// Two paths.  Up to 128 factors and 256 teacher entries the scores never leave the registers: one pass over the items per block of rows keeps a
+// running maximum and sum (and, for the gradients, the weighted sum of item rows), a second one over the rows per block of items gives the
+// items' gradient (rfm_distill_fused.hpp).  Beyond, the matrix path: the scores of a block of rows are written out, turned into dz in place
+// and multiplied.  Every sum has a fixed order on both.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -15,6 +18,8 @@
 
 namespace rfm {
 namespace distill {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMaxTeacher = 1024;                // entries of a teacher's list (their ids sit in LDS)
 
@@ -39,10 +44,11 @@ __device__ __forceinline__ const uint32_t *row_mask(const rfm_distill_args &a, l
 
 // One wavefront per row: the teacher's distribution over the usable entries, and its part of the loss.
 //   part[r] = sum_j p_j (log p_j - z[r, t_j] / tau)     mass[r] = 1, 0 without a usable entry, NaN where the row's mask does not exist
-// For the gradients the list is left merged: an item's first entry holds the sum of its entries' p, the others are off (-1, 0), so that no
-// two entries of a row meet in one element of dz.
+// For the gradients the list is left with the usable entries' p (-1, 0 elsewhere).  MERGE: merged too -- an item's first entry holds the sum of
+// its entries' p, the others are off, so that no two entries of a row meet in one element of dz.  acc [rows, kp]: sum_j p_j items[t_j].
+template <bool MERGE, int ACC>
 __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ merged_item,
-                                                      float *__restrict__ merged_p) {
+                                                      float *__restrict__ merged_p, float *__restrict__ acc_out) {
     extern __shared__ int s_dyn[];               // per wavefront: ids [n], p [n]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = a.n_teacher;
     const long long r = (long long)blockIdx.x * 4 + wave;
@@ -79,14 +85,27 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
     // the student's scores of the entries: one dot product per entry, 16 lanes each
     const float *u = a.users + (size_t)r * a.user_stride;
     const int sub = lane & 15, grp = lane >> 4;
-    float acc = 0.0f;
+    float acc = 0.0f, wsum[ACC > 0 ? ACC : 1] = {0.0f};
     for (int j0 = 0; j0 < n; j0 += 4) {
         const int j = j0 + grp;
         const int i = j < n ? id[j] : -1;
         float d = 0.0f;
         if (i >= 0) {
             const float *v = a.items + (size_t)i * a.item_stride;
-            for (int f = sub; f < a.n_factors; f += 16) d = fmaf(u[f], v[f], d);
+            if constexpr (ACC > 0) {
+                const float e = pr[j];
+#pragma unroll
+                for (int q = 0; q < ACC; ++q) {
+                    const int f = sub + 16 * q;
+                    if (f < a.n_factors) {
+                        const float x = v[f];
+                        d = fmaf(u[f], x, d);
+                        wsum[q] = fmaf(e, x, wsum[q]);
+                    }
+                }
+            } else {
+                for (int f = sub; f < a.n_factors; f += 16) d = fmaf(u[f], v[f], d);
+            }
         }
 #pragma unroll
         for (int m = 8; m > 0; m >>= 1) d += __shfl_xor(d, m);
@@ -100,11 +119,20 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
         part[r] = some ? acc : 0.0f;
         mass[r] = bad ? __uint_as_float(0x7fc00000u) : some ? 1.0f : 0.0f;
     }
+    if constexpr (ACC > 0) {
+#pragma unroll
+        for (int q = 0; q < ACC; ++q) {
+            float x = wsum[q];
+            x += __shfl_xor(x, 16);
+            x += __shfl_xor(x, 32);
+            if (grp == 0) acc_out[(size_t)r * (16 * ACC) + sub + 16 * q] = some ? x * inv : 0.0f;
+        }
+    }
     if (!merged_item) return;
     for (int j = lane; j < n; j += 64) {
         int i = id[j];
         float p = i >= 0 ? pr[j] * inv : 0.0f;
-        if (i >= 0) {
+        if (MERGE && i >= 0) {
             bool first = true;
             for (int k = 0; k < j; ++k) first &= id[k] != i;
             if (first) {
@@ -117,13 +145,13 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
     }
 }
 
-// C[m, n] (+)= sum_k A[m, k] B[k, n] (+ bias[n]), any strides; slices of k (blockIdx.y) go to slices of C.  64 x 64 tile per workgroup, four
+// C[m, n] (+)= sum_k A[m, k] B[k, n] (+ bias[n]), any strides; slices of k (blockIdx.y) go to slices of C.  live: rows k of B whose entry is 0
+// or NaN count as zeros, whatever they hold (rows without a usable teacher entry may be padding).  64 x 64 tile per workgroup, four
 // wavefronts of one 32 x 32 accumulator each (v_mfma_f32_32x32x2_f32, exact fp32), k in LDS stages of 32.
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kKT = 32, kLd = kKT + 1;
 __global__ void __launch_bounds__(256) gemm_kernel(const float *__restrict__ A, long long am, long long ak, const float *__restrict__ B, long long bk, long long bn,
                                                    const float *__restrict__ bias, float *__restrict__ C, long long cm, long long slice_stride, long long M, int N, int K,
-                                                   int k_slice, int n_tiles, int accumulate) {
+                                                   int k_slice, int n_tiles, int accumulate, const float *__restrict__ live) {
     __shared__ float sA[64 * kLd], sB[64 * kLd];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave >> 1, wc = wave & 1;
     const long long m0 = (long long)(blockIdx.x / n_tiles) * 64;
@@ -138,7 +166,7 @@ __global__ void __launch_bounds__(256) gemm_kernel(const float *__restrict__ A, 
             const int ra = ak == 1 ? e >> 5 : e & 63, ca = ak == 1 ? e & 31 : e >> 6;      // (consecutive threads along the contiguous side)
             const int rb = bk == 1 ? e >> 5 : e & 63, cb = bk == 1 ? e & 31 : e >> 6;
             sA[ra * kLd + ca] = m0 + ra < M && k0 + ca < ke ? A[(m0 + ra) * am + (long long)(k0 + ca) * ak] : 0.0f;
-            sB[rb * kLd + cb] = n0 + rb < N && k0 + cb < ke ? B[(long long)(k0 + cb) * bk + (long long)(n0 + rb) * bn] : 0.0f;
+            sB[rb * kLd + cb] = n0 + rb < N && k0 + cb < ke && (!live || live[k0 + cb] > 0.0f) ? B[(long long)(k0 + cb) * bk + (long long)(n0 + rb) * bn] : 0.0f;
         }
         __syncthreads();
         const float *pa = sA + (wr * 32 + (lane & 31)) * kLd + (lane >> 5), *pb = sB + (wc * 32 + (lane & 31)) * kLd + (lane >> 5);
@@ -217,25 +245,39 @@ __global__ void __launch_bounds__(256) sum_slices_kernel(const float *__restrict
     }
 }
 
+}  // namespace distill
+}  // namespace rfm
+
+#include "rfm_distill_fused.hpp"
+
+namespace rfm {
+namespace distill {
+
 static int check(const rfm_distill_args *a) {
     if (!a || a->n_rows < 0 || a->n_items < 1 || a->n_factors < 1 || a->n_teacher < 1) return RFM_ERR_BAD_ARG;
     if (!(a->temperature > 0.0f && a->temperature < INFINITY)) return RFM_ERR_BAD_ARG;
     if (a->user_stride < a->n_factors || a->item_stride < a->n_factors) return RFM_ERR_BAD_ARG;
     if (a->allowed && (a->n_allowed < 1 || (!a->allowed_rows && a->n_allowed != 1 && a->n_allowed < a->n_rows))) return RFM_ERR_BAD_ARG;
     if (!a->d_users != !a->d_items || (a->d_bias && !a->d_items)) return RFM_ERR_BAD_ARG;
-    if (a->n_factors > 1024 || a->n_teacher > kMaxTeacher || a->n_items > 0x7fffff00 || a->n_rows > 0x7fffff00) return RFM_ERR_UNSUPPORTED;
+    if (a->n_factors > 1024 || a->n_teacher > kMaxTeacher || a->n_items > (1 << 25) || a->n_rows > (1 << 24)) return RFM_ERR_UNSUPPORTED;      // (launches stay below 2^32 threads)
     return RFM_OK;
 }
 
 static size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
-struct Layout {
+// The fused path holds a wavefront's factors and sums in registers (up to 128 factors) and sorts a tile's teacher entries in LDS (up to 256 per
+// row).  What is larger takes the matrix path.
+static bool fused(const rfm_distill_args *a) {
+    return a->n_factors <= 128 && a->n_teacher <= kFusedTeacher;
+}
+
+struct MatrixLayout {
     long long block;                             // rows whose scores are kept at once
     int slices;                                  // of the items, for the users' gradient
     size_t part, mass, merged_item, merged_p, z, d_part, bytes;
 };
-static Layout layout(const rfm_distill_args *a) {
-    Layout w;
+static MatrixLayout matrix_layout(const rfm_distill_args *a) {
+    MatrixLayout w;
     const size_t R = (size_t)a->n_rows, I = (size_t)a->n_items, n = (size_t)a->n_teacher;
     w.block = std::max<long long>(64, std::min<long long>(4096, ((long long)1 << 28) / a->n_items));
     w.block = std::min<long long>(w.block, std::max<long long>(1, a->n_rows));
@@ -251,6 +293,126 @@ static Layout layout(const rfm_distill_args *a) {
     return w;
 }
 
+static int run_matrix(const rfm_distill_args *a, char *base, hipStream_t stream) {
+    const MatrixLayout w = matrix_layout(a);
+    const bool grad = a->d_users != nullptr;
+    float *part = (float *)(base + w.part), *mass = (float *)(base + w.mass), *z = (float *)(base + w.z), *d_part = (float *)(base + w.d_part);
+    int32_t *mi = grad ? (int32_t *)(base + w.merged_item) : nullptr;
+    float *mp = grad ? (float *)(base + w.merged_p) : nullptr;
+    const int I = a->n_items, K = a->n_factors;
+    teacher_kernel<true, 0><<<dim3((unsigned)((a->n_rows + 3) / 4)), dim3(256), (size_t)a->n_teacher * 2 * 4 * 4, stream>>>(*a, part, mass, mi, mp, nullptr);
+    const int it = (I + 63) / 64, kt = (K + 63) / 64;
+    const int slice = ((I + w.slices - 1) / w.slices + 31) / 32 * 32;
+    const int slices = (I + slice - 1) / slice;
+    for (long long r0 = 0; r0 < a->n_rows; r0 += w.block) {
+        const long long nr = std::min<long long>(w.block, a->n_rows - r0);
+        const float *u = a->users + (size_t)r0 * a->user_stride;
+        const unsigned rt = (unsigned)((nr + 63) / 64);
+        const int more = r0 > 0;
+        gemm_kernel<<<dim3(rt * (unsigned)it), dim3(256), 0, stream>>>(u, a->user_stride, 1, a->items, 1, a->item_stride, a->bias, z, I, 0, nr, I, K, K, it, 0, nullptr);
+        softmax_rows_kernel<<<dim3((unsigned)nr), dim3(256), 0, stream>>>(*a, r0, z, part, mass, mi, mp);
+        if (!grad) continue;
+        gemm_kernel<<<dim3(rt * (unsigned)kt, (unsigned)slices), dim3(256), 0, stream>>>(z, I, 1, a->items, a->item_stride, 1, nullptr, d_part, K, nr * K, nr, K, I, slice, kt, 0, nullptr);
+        sum_slices_kernel<<<dim3(1024), dim3(256), 0, stream>>>(d_part, nr * K, slices, a->d_users + (size_t)r0 * K);
+        gemm_kernel<<<dim3((unsigned)it * (unsigned)kt), dim3(256), 0, stream>>>(z, 1, I, u, a->user_stride, 1, nullptr, a->d_items, K, 0, I, K, (int)nr, 1 << 20, kt, more, mass + r0);
+        if (a->d_bias) column_sum_kernel<<<dim3((unsigned)((I + 255) / 256)), dim3(256), 0, stream>>>(z, nr, I, a->d_bias, more);
+    }
+    return RFM_OK;
+}
+
+// How often the streamed tiles are split: workgroups run `slots` at a time, a workgroup costs its tiles and about four more to start and end,
+// a split costs its partial sums.  The cheapest count wins; the sums of a count are always joined in the same order.
+constexpr int kCus = 256;
+static int pick_splits(int blocks, int tiles, int slots) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 256 && s <= std::max(1, tiles / 2); ++s) {
+        const int chunk = (tiles + s - 1) / s, used = (tiles + chunk - 1) / chunk;
+        if (used != s) continue;
+        const double rounds = (double)(((long long)blocks * s + slots - 1) / slots);
+        const double cost = rounds * (chunk + 4) + 0.25 * s;
+        if (cost < least) { least = cost; best = s; }
+    }
+    return best;
+}
+
+struct FusedLayout {
+    int kp, waves, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, splits_i;
+    size_t part, mass, ids, ps, acc, user_frag, user_frag_t, item_frag, item_frag_t, bias2, mask_row, part_m, part_l, part_o, row_data, entry, entry_at, part_items, part_bias, bytes;
+};
+static FusedLayout fused_layout(const rfm_distill_args *a) {
+    FusedLayout w;
+    const bool grad = a->d_users != nullptr;
+    w.kp = (a->n_factors + 31) / 32 * 32;
+    w.waves = w.kp <= 64 ? 4 : 8;
+    const size_t R = (size_t)a->n_rows, n = (size_t)a->n_teacher, kp = (size_t)w.kp;
+    w.user_tiles = (int)((a->n_rows + 31) / 32);
+    w.item_tiles = (a->n_items + 31) / 32;
+    w.user_blocks = (w.user_tiles + w.waves - 1) / w.waves;
+    w.item_blocks = (w.item_tiles + w.waves - 1) / w.waves;
+    const int slots = kCus * (w.waves == 4 ? 2 : 1);
+    w.splits_f = pick_splits(w.user_blocks, w.item_tiles, slots);
+    w.splits_i = grad ? pick_splits(w.item_blocks, w.user_tiles, slots) : 1;
+    const size_t ur = (size_t)w.user_tiles * 32, ir = (size_t)w.item_tiles * 32;
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += up(bytes ? bytes : 1); return at; };
+    w.part = take(4 * R); w.mass = take(4 * R);
+    w.ids = take(grad ? 4 * R * n : 0); w.ps = take(grad ? 4 * R * n : 0); w.acc = take(grad ? 4 * R * kp : 0);
+    w.user_frag = take(6 * ur * kp); w.item_frag = take(6 * ir * kp);
+    w.user_frag_t = take(grad ? 6 * ur * kp : 0); w.item_frag_t = take(grad ? 6 * ir * kp : 0);
+    w.bias2 = take(4 * (ir + 64)); w.mask_row = take(a->allowed ? 4 * ur : 0);
+    w.part_m = take(4 * w.splits_f * ur); w.part_l = take(4 * w.splits_f * ur); w.part_o = take(grad ? 4 * w.splits_f * ur * kp : 0);
+    w.row_data = take(grad ? (size_t)w.user_tiles * kRowData * 4 : 0);
+    w.entry = take(grad ? ur * n * 8 : 0); w.entry_at = take(grad ? 4 * (size_t)w.user_tiles * (w.item_blocks + 1) : 0);
+    w.part_items = take(grad ? 4 * w.splits_i * ir * kp : 0); w.part_bias = take(grad ? 4 * w.splits_i * ir : 0);
+    w.bytes = off;
+    return w;
+}
+
+template <int KP, int WAVES>
+static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base, hipStream_t stream) {
+    const bool grad = a->d_users != nullptr;
+    auto at = [&](size_t off) { return base + off; };
+    float *part = (float *)at(w.part), *mass = (float *)at(w.mass), *acc = (float *)at(w.acc), *ps = (float *)at(w.ps);
+    int32_t *ids = (int32_t *)at(w.ids);
+    const size_t lds = (size_t)a->n_teacher * 2 * 4 * 4;
+    const dim3 rows4((unsigned)((a->n_rows + 3) / 4));
+    if (grad) teacher_kernel<false, KP / 16><<<rows4, dim3(256), lds, stream>>>(*a, part, mass, ids, ps, acc);
+    else teacher_kernel<false, 0><<<rows4, dim3(256), lds, stream>>>(*a, part, mass, nullptr, nullptr, nullptr);
+    FusedArgs f = {};
+    f.a = *a;
+    f.user_tiles = w.user_tiles; f.item_tiles = w.item_tiles; f.item_blocks = w.item_blocks;
+    f.user_frag = at(w.user_frag); f.user_frag_t = at(w.user_frag_t); f.item_frag = at(w.item_frag); f.item_frag_t = at(w.item_frag_t);
+    f.bias2 = (const float *)at(w.bias2); f.mask_row = (const int32_t *)at(w.mask_row);
+    f.part_m = (float *)at(w.part_m); f.part_l = (float *)at(w.part_l); f.part_o = (float *)at(w.part_o);
+    f.row_data = (const float *)at(w.row_data);
+    f.entry = (const uint2 *)at(w.entry); f.entry_at = (const int32_t *)at(w.entry_at);
+    f.part_items = (float *)at(w.part_items); f.part_bias = (float *)at(w.part_bias);
+    const float c = 1.4426950408889634f / a->temperature;
+    frags_kernel<KP><<<dim3((unsigned)(w.user_tiles + w.item_tiles)), dim3(256), 0, stream>>>(*a, w.user_tiles, w.item_tiles, c, mass, (char *)f.user_frag, grad ? (char *)f.user_frag_t : nullptr,
+                                                                                              (char *)f.item_frag, grad ? (char *)f.item_frag_t : nullptr, (float *)f.bias2, (int32_t *)f.mask_row);
+    f.splits = w.splits_f;
+    f.chunk = (w.item_tiles + w.splits_f - 1) / w.splits_f;
+    const dim3 grid_f((unsigned)(w.user_blocks * w.splits_f)), threads(WAVES * 64);
+    if (grad && a->allowed) forward_kernel<KP, true, true, WAVES><<<grid_f, threads, 0, stream>>>(f);
+    else if (grad) forward_kernel<KP, true, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
+    else if (a->allowed) forward_kernel<KP, false, true, WAVES><<<grid_f, threads, 0, stream>>>(f);
+    else forward_kernel<KP, false, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
+    join_rows_kernel<KP><<<dim3((unsigned)(w.user_tiles * 8)), dim3(256), 0, stream>>>(f, part, mass, acc, (float *)f.row_data);
+    if (!grad) return RFM_OK;
+    int p2 = 64;
+    while (p2 < 32 * a->n_teacher) p2 <<= 1;
+    sort_entries_kernel<<<dim3((unsigned)w.user_tiles), dim3(256), (size_t)p2 * 8, stream>>>(a->n_rows, a->n_teacher, WAVES * 32, w.item_blocks, p2, ids, ps, (uint2 *)f.entry, (int32_t *)f.entry_at);
+    f.splits = w.splits_i;
+    f.chunk = (w.user_tiles + w.splits_i - 1) / w.splits_i;
+    const dim3 grid_i((unsigned)(w.item_blocks * w.splits_i));
+    if (a->allowed) items_kernel<KP, true, WAVES><<<grid_i, threads, 0, stream>>>(f);
+    else items_kernel<KP, false, WAVES><<<grid_i, threads, 0, stream>>>(f);
+    const long long n = (long long)a->n_items * a->n_factors;
+    join_items_kernel<KP><<<dim3((unsigned)std::min<long long>(8192, (n + 255) / 256)), dim3(256), 0, stream>>>(f);
+    return RFM_OK;
+}
+
 }  // namespace distill
 }  // namespace rfm
 
@@ -258,43 +420,31 @@ using namespace rfm;
 
 extern "C" {
 
-size_t rfm_distill_workspace_bytes(const rfm_distill_args *a) { return distill::check(a) == RFM_OK ? distill::layout(a).bytes : 0; }
+size_t rfm_distill_workspace_bytes(const rfm_distill_args *a) {
+    if (distill::check(a) != RFM_OK) return 0;
+    return distill::fused(a) ? distill::fused_layout(a).bytes : distill::matrix_layout(a).bytes;
+}
 
 int rfm_distill_device(const rfm_distill_args *a, void *workspace, size_t workspace_bytes, void *hip_stream) {
-    const int rc = distill::check(a);
+    int rc = distill::check(a);
     if (rc != RFM_OK) return rc;
     hipStream_t stream = (hipStream_t)hip_stream;
-    const bool grad = a->d_users != nullptr;
     if (!a->items || (a->n_rows > 0 && (!a->users || !a->teacher_items || !a->teacher_scores || !a->loss))) return RFM_ERR_BAD_ARG;
-    const distill::Layout w = distill::layout(a);
-    if (!workspace || workspace_bytes < w.bytes) return RFM_ERR_WORKSPACE;
-    char *base = (char *)workspace;
-    float *part = (float *)(base + w.part), *mass = (float *)(base + w.mass), *z = (float *)(base + w.z), *d_part = (float *)(base + w.d_part);
-    int32_t *mi = grad ? (int32_t *)(base + w.merged_item) : nullptr;
-    float *mp = grad ? (float *)(base + w.merged_p) : nullptr;
-    const int I = a->n_items, K = a->n_factors;
-    if (a->n_rows > 0)
-        distill::teacher_kernel<<<dim3((unsigned)((a->n_rows + 3) / 4)), dim3(256), (size_t)a->n_teacher * 2 * 4 * 4, stream>>>(*a, part, mass, mi, mp);
-    const int it = (I + 63) / 64, kt = (K + 63) / 64;
-    const int slice = ((I + w.slices - 1) / w.slices + 31) / 32 * 32;
-    const int slices = (I + slice - 1) / slice;
-    for (long long r0 = 0; r0 < std::max<int64_t>(a->n_rows, grad ? 1 : 0); r0 += w.block) {      // (no rows at all: the items' gradients are still set, to zero)
-        const long long nr = std::min<long long>(w.block, a->n_rows - r0);
-        const float *u = a->users + (size_t)r0 * a->user_stride;
-        if (nr > 0) {
-            const unsigned rt = (unsigned)((nr + 63) / 64);
-            distill::gemm_kernel<<<dim3(rt * (unsigned)it), dim3(256), 0, stream>>>(u, a->user_stride, 1, a->items, 1, a->item_stride, a->bias, z, I, 0, nr, I, K, K, it, 0);
-            distill::softmax_rows_kernel<<<dim3((unsigned)nr), dim3(256), 0, stream>>>(*a, r0, z, part, mass, mi, mp);
-            if (!grad) continue;
-            distill::gemm_kernel<<<dim3(rt * (unsigned)kt, (unsigned)slices), dim3(256), 0, stream>>>(z, I, 1, a->items, a->item_stride, 1, nullptr, d_part, K, (long long)nr * K, nr, K,
-                                                                                                       I, slice, kt, 0);
-            distill::sum_slices_kernel<<<dim3(1024), dim3(256), 0, stream>>>(d_part, nr * K, slices, a->d_users + (size_t)r0 * K);
-        }
-        const int more = r0 > 0;
-        distill::gemm_kernel<<<dim3((unsigned)it * (unsigned)kt), dim3(256), 0, stream>>>(z, 1, I, u, a->user_stride, 1, nullptr, a->d_items, K, 0, I, K, (int)std::max<long long>(nr, 0), 1 << 20, kt,
-                                                                                           more);
-        if (a->d_bias) distill::column_sum_kernel<<<dim3((unsigned)((I + 255) / 256)), dim3(256), 0, stream>>>(z, std::max<long long>(nr, 0), I, a->d_bias, more);
+    if (!workspace || workspace_bytes < rfm_distill_workspace_bytes(a)) return RFM_ERR_WORKSPACE;
+    if (a->n_rows == 0) {                        // nothing to learn from: the items' gradients are zero
+        if (a->d_items) distill::zero_kernel<<<dim3(1024), dim3(256), 0, stream>>>(a->d_items, (long long)a->n_items * a->n_factors);
+        if (a->d_bias) distill::zero_kernel<<<dim3(1024), dim3(256), 0, stream>>>(a->d_bias, a->n_items);
+    } else if (!distill::fused(a)) {
+        rc = distill::run_matrix(a, (char *)workspace, stream);
+    } else {
+        const distill::FusedLayout w = distill::fused_layout(a);
+        char *base = (char *)workspace;
+        if (w.kp == 32) rc = distill::run_fused<32, 4>(a, w, base, stream);
+        else if (w.kp == 64) rc = distill::run_fused<64, 4>(a, w, base, stream);
+        else if (w.kp == 96) rc = distill::run_fused<96, 8>(a, w, base, stream);
+        else rc = distill::run_fused<128, 8>(a, w, base, stream);
     }
+    if (rc != RFM_OK) return rc;
     return hipGetLastError() == hipSuccess ? RFM_OK : RFM_ERR_HIP;
 }
 

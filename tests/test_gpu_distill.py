@@ -227,3 +227,35 @@ def test_refusals():
     many = torch.zeros(4, 1025, dtype=torch.int32).cuda()
     with pytest.raises(ValueError):
         distill_loss(u, v, b, many, many.float())
+
+
+def test_padding_rows_do_not_reach_the_gradients_whatever_they_hold():
+    for factors in (20, 200):                                                     # both paths
+        p = Problem(rows=70, items=400, factors=factors, n=6, seed=11)
+        p.ti = np.abs(p.ti) % 400
+        args, kw = p.given()
+        weight = torch.from_numpy(p.g).cuda()
+        pad = [3, 31, 32, 69]
+        keep = [r for r in range(70) if r not in pad]
+        ti = args[3].clone()
+        ti[pad] = -1
+        clean = distill_gradients(*args[:3], ti, args[4], row_weight=weight, **kw)
+        u, t, g = args[0].clone(), args[4].clone(), weight.clone()
+        u[pad[0]], u[pad[1]], u[pad[2]], u[pad[3]] = NAN, INF, -INF, 3e38
+        t[pad] = NAN
+        g[pad] = NAN
+        got = distill_gradients(u, args[1], args[2], ti, t, row_weight=g, **kw)
+        assert (got.loss[pad] == 0).all() and (got.users[pad] == 0).all()
+        for a, b in zip(got, clean):
+            assert torch.equal(a[keep], b[keep]) if a.shape[0] == 70 else torch.equal(a, b)
+
+
+def test_many_entries_in_one_tile_and_items_twice():
+    """every row's list in the same 32 items, some of them several times: the teacher's patch is full"""
+    p = Problem(rows=100, items=5000, factors=40, n=60, seed=12)
+    p.ti = 640 + np.random.default_rng(0).integers(0, 32, (100, 60)).astype(np.int32)
+    want, tol = p.exact()
+    args, kw = p.given()
+    got = distill_gradients(*args, row_weight=torch.from_numpy(p.g).cuda(), **kw)
+    for g, w, t in zip(got, want, tol):
+        assert (np.abs(g.cpu().numpy() - w) <= t).all()
