@@ -338,7 +338,7 @@ static int pick_splits(int blocks, int tiles, int slots) {
 
 struct FusedLayout {
     int kp, waves, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, splits_i;
-    size_t part, mass, ids, ps, acc, user_frag, user_frag_t, item_frag, item_frag_t, bias2, mask_row, part_m, part_l, part_o, row_data, entry, entry_at, part_items, part_bias, bytes;
+    size_t part, mass, ids, ps, acc, user_frag, user_frag_t, item_frag, item_frag_t, item_data, user_data, user_data_t, mask_row, part_m, part_l, part_o, entry, entry_at, part_items, part_bias, bytes;
 };
 static FusedLayout fused_layout(const rfm_distill_args *a) {
     FusedLayout w;
@@ -350,7 +350,7 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     w.item_tiles = (a->n_items + 31) / 32;
     w.user_blocks = (w.user_tiles + w.waves - 1) / w.waves;
     w.item_blocks = (w.item_tiles + w.waves - 1) / w.waves;
-    const int slots = kCus * (w.waves == 4 ? 2 : 1);
+    const int slots = kCus * (w.kp == 32 ? 4 : w.kp == 64 ? 3 : 1);              // workgroups that fit on the chip at once, by registers and LDS
     w.splits_f = pick_splits(w.user_blocks, w.item_tiles, slots);
     w.splits_i = grad ? pick_splits(w.item_blocks, w.user_tiles, slots) : 1;
     const size_t ur = (size_t)w.user_tiles * 32, ir = (size_t)w.item_tiles * 32;
@@ -358,11 +358,11 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     auto take = [&](size_t bytes) { const size_t at = off; off += up(bytes ? bytes : 1); return at; };
     w.part = take(4 * R); w.mass = take(4 * R);
     w.ids = take(grad ? 4 * R * n : 0); w.ps = take(grad ? 4 * R * n : 0); w.acc = take(grad ? 4 * R * kp : 0);
-    w.user_frag = take(6 * ur * kp); w.item_frag = take(6 * ir * kp);
-    w.user_frag_t = take(grad ? 6 * ur * kp : 0); w.item_frag_t = take(grad ? 6 * ir * kp : 0);
-    w.bias2 = take(4 * (ir + 64)); w.mask_row = take(a->allowed ? 4 * ur : 0);
+    w.user_frag = take(4 * ur * kp); w.item_frag = take(4 * ir * kp);
+    w.user_frag_t = take(grad ? 4 * ur * kp : 0); w.item_frag_t = take(grad ? 4 * ir * kp : 0);
+    w.item_data = take((size_t)w.item_tiles * kItemData * 4); w.user_data = take((size_t)w.user_tiles * kUserData * 4); w.user_data_t = take((size_t)w.user_tiles * kUserData * 4);
+    w.mask_row = take(a->allowed ? 4 * ur : 0);
     w.part_m = take(4 * w.splits_f * ur); w.part_l = take(4 * w.splits_f * ur); w.part_o = take(grad ? 4 * w.splits_f * ur * kp : 0);
-    w.row_data = take(grad ? (size_t)w.user_tiles * kRowData * 4 : 0);
     w.entry = take(grad ? ur * n * 8 : 0); w.entry_at = take(grad ? 4 * (size_t)w.user_tiles * (w.item_blocks + 1) : 0);
     w.part_items = take(grad ? 4 * w.splits_i * ir * kp : 0); w.part_bias = take(grad ? 4 * w.splits_i * ir : 0);
     w.bytes = off;
@@ -383,14 +383,12 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     f.a = *a;
     f.user_tiles = w.user_tiles; f.item_tiles = w.item_tiles; f.item_blocks = w.item_blocks;
     f.user_frag = at(w.user_frag); f.user_frag_t = at(w.user_frag_t); f.item_frag = at(w.item_frag); f.item_frag_t = at(w.item_frag_t);
-    f.bias2 = (const float *)at(w.bias2); f.mask_row = (const int32_t *)at(w.mask_row);
+    f.item_data = (float *)at(w.item_data); f.user_data = (float *)at(w.user_data); f.user_data_t = (float *)at(w.user_data_t); f.mask_row = (int32_t *)at(w.mask_row);
     f.part_m = (float *)at(w.part_m); f.part_l = (float *)at(w.part_l); f.part_o = (float *)at(w.part_o);
-    f.row_data = (const float *)at(w.row_data);
-    f.entry = (const uint2 *)at(w.entry); f.entry_at = (const int32_t *)at(w.entry_at);
+    f.entry = (uint2 *)at(w.entry); f.entry_at = (int32_t *)at(w.entry_at);
     f.part_items = (float *)at(w.part_items); f.part_bias = (float *)at(w.part_bias);
     const float c = 1.4426950408889634f / a->temperature;
-    frags_kernel<KP><<<dim3((unsigned)(w.user_tiles + w.item_tiles)), dim3(256), 0, stream>>>(*a, w.user_tiles, w.item_tiles, c, mass, (char *)f.user_frag, grad ? (char *)f.user_frag_t : nullptr,
-                                                                                              (char *)f.item_frag, grad ? (char *)f.item_frag_t : nullptr, (float *)f.bias2, (int32_t *)f.mask_row);
+    frags_kernel<KP><<<dim3((unsigned)(w.user_tiles + w.item_tiles)), dim3(256), 0, stream>>>(f, c, mass);
     f.splits = w.splits_f;
     f.chunk = (w.item_tiles + w.splits_f - 1) / w.splits_f;
     const dim3 grid_f((unsigned)(w.user_blocks * w.splits_f)), threads(WAVES * 64);
@@ -398,11 +396,11 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     else if (grad) forward_kernel<KP, true, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
     else if (a->allowed) forward_kernel<KP, false, true, WAVES><<<grid_f, threads, 0, stream>>>(f);
     else forward_kernel<KP, false, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
-    join_rows_kernel<KP><<<dim3((unsigned)(w.user_tiles * 8)), dim3(256), 0, stream>>>(f, part, mass, acc, (float *)f.row_data);
+    join_rows_kernel<KP><<<dim3((unsigned)(w.user_tiles * 8)), dim3(256), 0, stream>>>(f, part, mass, acc);
     if (!grad) return RFM_OK;
     int p2 = 64;
     while (p2 < 32 * a->n_teacher) p2 <<= 1;
-    sort_entries_kernel<<<dim3((unsigned)w.user_tiles), dim3(256), (size_t)p2 * 8, stream>>>(a->n_rows, a->n_teacher, WAVES * 32, w.item_blocks, p2, ids, ps, (uint2 *)f.entry, (int32_t *)f.entry_at);
+    sort_entries_kernel<<<dim3((unsigned)w.user_tiles), dim3(256), (size_t)p2 * 8, stream>>>(a->n_rows, a->n_teacher, WAVES * 32, w.item_blocks, p2, ids, ps, f.entry, f.entry_at);
     f.splits = w.splits_i;
     f.chunk = (w.user_tiles + w.splits_i - 1) / w.splits_i;
     const dim3 grid_i((unsigned)(w.item_blocks * w.splits_i));
