@@ -5,7 +5,7 @@
 //   loss[r] = tau^2 sum_j p_j (log p_j - z[r, t_j] / tau + lse_r),   lse_r = log sum_i exp(z[r, i] / tau)
 //   dz = tau * weight[r] * (q - p);   d_users = dz . items;   d_items = dz^T . users;   d_bias = column sums of dz
 //
-// Two paths.  Up to 128 factors and 256 teacher entries the scores never leave the registers: one pass over the items per block of rows keeps a
+// Two paths.  Up to 128 factors the scores never leave the registers: one pass over the items per block of rows keeps a
 // running maximum and sum (and, for the gradients, the weighted sum of item rows), a second one over the rows per block of items gives the
 // items' gradient (rfm_distill_fused.hpp).  Beyond, the matrix path: the scores of a block of rows are written out, turned into dz in place
 // and multiplied.  Every sum has a fixed order on both.
@@ -42,17 +42,33 @@ __device__ __forceinline__ const uint32_t *row_mask(const rfm_distill_args &a, l
     return m < 0 ? nullptr : a.allowed + (size_t)m * (size_t)((a.n_items + 31) / 32);
 }
 
+// whether a teacher's entry counts
+__device__ __forceinline__ bool usable(const rfm_distill_args &a, const uint32_t *mask, int item, float score) {
+    return item >= 0 && item < a.n_items && !(score == -INFINITY) && (!mask || ((mask[item >> 5] >> (item & 31)) & 1u));
+}
+
+struct __attribute__((packed, aligned(4))) Four { float v[4]; };
+// factors 4 f .. 4 f + 3 of a row, zeros behind its end; rows start anywhere, the hardware takes 16 bytes at any address
+__device__ __forceinline__ Four load_four(const float *row, int k, int factors) {
+    Four x;
+    if (k + 4 <= factors) __builtin_memcpy(&x, reinterpret_cast<const Four *>(row + k), sizeof(x));
+    else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.v[j] = k + j < factors ? row[k + j] : 0.0f;
+    }
+    return x;
+}
+
 // One wavefront per row: the teacher's distribution over the usable entries, and its part of the loss.
 //   part[r] = sum_j p_j (log p_j - z[r, t_j] / tau)     mass[r] = 1, 0 without a usable entry, NaN where the row's mask does not exist
 // For the gradients the list is left with the usable entries' p (-1, 0 elsewhere).  MERGE: merged too -- an item's first entry holds the sum of
-// its entries' p, the others are off, so that no two entries of a row meet in one element of dz.  acc [rows, kp]: sum_j p_j items[t_j].
+// its entries' p, the others are off, so that no two entries of a row meet in one element of dz.  ACC > 0 (quarters of 64 factors, rounded up):
+// acc [rows, kp] = sum_j p_j items[t_j].  s_dyn: per wavefront ids [n] and p [n].  No barrier: a wavefront works by itself.
 template <bool MERGE, int ACC>
-__global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ merged_item,
-                                                      float *__restrict__ merged_p, float *__restrict__ acc_out) {
-    extern __shared__ int s_dyn[];               // per wavefront: ids [n], p [n]
+__device__ void teacher_row(const rfm_distill_args &a, long long r, int kp, int *s_dyn, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ merged_item,
+                            float *__restrict__ merged_p, float *__restrict__ acc_out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = a.n_teacher;
-    const long long r = (long long)blockIdx.x * 4 + wave;
-    if (r >= a.n_rows) return;                   // (no barrier below: a wavefront works by itself)
+    if (r >= a.n_rows) return;
     int *id = s_dyn + wave * 2 * n;
     float *pr = reinterpret_cast<float *>(id + n);
     bool bad = false;
@@ -66,14 +82,13 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
     for (int j = lane; j < n; j += 64) {
         const int i = ti[j];
         const float t = ts[j];
-        const bool use = i >= 0 && i < a.n_items && !(t == -INFINITY) && (!mask || ((mask[i >> 5] >> (i & 31)) & 1u));
+        const bool use = usable(a, mask, i, t);
         id[j] = use ? i : -1;
         if (use) { some = 1; nan |= isnan(t); top = fmaxf(top, t); }
     }
     some = __any(some);
-    if (__any(nan)) top = __uint_as_float(0x7fc00000u);
     top = wave_max(top);
-    if (__any(isnan(top))) top = __uint_as_float(0x7fc00000u);
+    if (__any(nan)) top = __uint_as_float(0x7fc00000u);
     float sum = 0.0f;
     for (int j = lane; j < n; j += 64) {
         const float e = id[j] >= 0 ? expf((ts[j] - top) * inv_tau) : 0.0f;
@@ -82,36 +97,57 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
     }
     sum = wave_sum(sum);
     const float log_sum = logf(sum), inv = 1.0f / sum;
-    // the student's scores of the entries: one dot product per entry, 16 lanes each
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // the student's scores of the entries: 16 lanes per entry, two entries of each group of lanes at a time so that their loads overlap
     const float *u = a.users + (size_t)r * a.user_stride;
     const int sub = lane & 15, grp = lane >> 4;
-    float acc = 0.0f, wsum[ACC > 0 ? ACC : 1] = {0.0f};
-    for (int j0 = 0; j0 < n; j0 += 4) {
-        const int j = j0 + grp;
-        const int i = j < n ? id[j] : -1;
-        float d = 0.0f;
-        if (i >= 0) {
-            const float *v = a.items + (size_t)i * a.item_stride;
+    float acc = 0.0f;
+    Four mine[ACC > 0 ? ACC : 1], wsum[ACC > 0 ? ACC : 1];
+    if constexpr (ACC > 0) {
+#pragma unroll
+        for (int q = 0; q < ACC; ++q) {
+            mine[q] = load_four(u, 64 * q + 4 * sub, a.n_factors);
+            wsum[q] = Four{{0.0f, 0.0f, 0.0f, 0.0f}};
+        }
+    }
+    for (int j0 = 0; j0 < n; j0 += 8) {
+        float d[2] = {0.0f, 0.0f};
+        int item[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int j = j0 + 4 * h + grp;
+            item[h] = j < n ? id[j] : -1;
+            if (item[h] < 0) continue;
+            const float *v = a.items + (size_t)item[h] * a.item_stride;
             if constexpr (ACC > 0) {
                 const float e = pr[j];
 #pragma unroll
                 for (int q = 0; q < ACC; ++q) {
-                    const int f = sub + 16 * q;
-                    if (f < a.n_factors) {
-                        const float x = v[f];
-                        d = fmaf(u[f], x, d);
-                        wsum[q] = fmaf(e, x, wsum[q]);
+                    const Four x = load_four(v, 64 * q + 4 * sub, a.n_factors);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        d[h] = fmaf(mine[q].v[k], x.v[k], d[h]);
+                        wsum[q].v[k] = fmaf(e, x.v[k], wsum[q].v[k]);
                     }
                 }
             } else {
-                for (int f = sub; f < a.n_factors; f += 16) d = fmaf(u[f], v[f], d);
+                for (int f = 4 * sub; f < a.n_factors; f += 64) {
+                    const Four x = load_four(v, f, a.n_factors), y = load_four(u, f, a.n_factors);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) d[h] = fmaf(y.v[k], x.v[k], d[h]);
+                }
             }
         }
 #pragma unroll
-        for (int m = 8; m > 0; m >>= 1) d += __shfl_xor(d, m);
-        if (i >= 0 && sub == 0) {
-            const float e = pr[j], z = d + (a.bias ? a.bias[i] : 0.0f);
-            if (!(e == 0.0f)) acc += e * inv * ((ts[j] - top) * inv_tau - log_sum - z * inv_tau);
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int m = 8; m > 0; m >>= 1) d[h] += __shfl_xor(d[h], m);
+            if (item[h] >= 0 && sub == 0) {
+                const int j = j0 + 4 * h + grp;
+                const float e = pr[j], z = d[h] + (a.bias ? a.bias[item[h]] : 0.0f);
+                if (!(e == 0.0f)) acc += e * inv * ((ts[j] - top) * inv_tau - log_sum - z * inv_tau);
+            }
         }
     }
     acc = wave_sum(acc);
@@ -121,12 +157,15 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
     }
     if constexpr (ACC > 0) {
 #pragma unroll
-        for (int q = 0; q < ACC; ++q) {
-            float x = wsum[q];
-            x += __shfl_xor(x, 16);
-            x += __shfl_xor(x, 32);
-            if (grp == 0) acc_out[(size_t)r * (16 * ACC) + sub + 16 * q] = some ? x * inv : 0.0f;
-        }
+        for (int q = 0; q < ACC; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float x = wsum[q].v[k];
+                x += __shfl_xor(x, 16);
+                x += __shfl_xor(x, 32);
+                const int at = 64 * q + 4 * sub + k;
+                if (grp == 0 && at < kp) acc_out[(size_t)r * kp + at] = some ? x * inv : 0.0f;
+            }
     }
     if (!merged_item) return;
     for (int j = lane; j < n; j += 64) {
@@ -143,6 +182,11 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
         merged_item[(size_t)r * n + j] = bad ? -1 : i;
         merged_p[(size_t)r * n + j] = p;
     }
+}
+__global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ merged_item,
+                                                      float *__restrict__ merged_p) {
+    extern __shared__ int s_dyn[];
+    teacher_row<true, 0>(a, (long long)blockIdx.x * 4 + (threadIdx.x >> 6), 0, s_dyn, part, mass, merged_item, merged_p, nullptr);
 }
 
 // C[m, n] (+)= sum_k A[m, k] B[k, n] (+ bias[n]), any strides; slices of k (blockIdx.y) go to slices of C.  live: rows k of B whose entry is 0
@@ -265,11 +309,8 @@ static int check(const rfm_distill_args *a) {
 
 static size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
-// The fused path holds a wavefront's factors and sums in registers (up to 128 factors) and sorts a tile's teacher entries in LDS (up to 256 per
-// row).  What is larger takes the matrix path.
-static bool fused(const rfm_distill_args *a) {
-    return a->n_factors <= 128 && a->n_teacher <= kFusedTeacher;
-}
+// The fused path holds a wavefront's factors and sums in registers.
+static bool fused(const rfm_distill_args *a) { return a->n_factors <= 128; }
 
 struct MatrixLayout {
     long long block;                             // rows whose scores are kept at once
@@ -300,7 +341,7 @@ static int run_matrix(const rfm_distill_args *a, char *base, hipStream_t stream)
     int32_t *mi = grad ? (int32_t *)(base + w.merged_item) : nullptr;
     float *mp = grad ? (float *)(base + w.merged_p) : nullptr;
     const int I = a->n_items, K = a->n_factors;
-    teacher_kernel<true, 0><<<dim3((unsigned)((a->n_rows + 3) / 4)), dim3(256), (size_t)a->n_teacher * 2 * 4 * 4, stream>>>(*a, part, mass, mi, mp, nullptr);
+    teacher_kernel<<<dim3((unsigned)((a->n_rows + 3) / 4)), dim3(256), (size_t)a->n_teacher * 2 * 4 * 4, stream>>>(*a, part, mass, mi, mp);
     const int it = (I + 63) / 64, kt = (K + 63) / 64;
     const int slice = ((I + w.slices - 1) / w.slices + 31) / 32 * 32;
     const int slices = (I + slice - 1) / slice;
@@ -337,7 +378,7 @@ static int pick_splits(int blocks, int tiles, int slots) {
 }
 
 struct FusedLayout {
-    int kp, waves, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, splits_i;
+    int kp, waves, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, groups_i, units_i;
     size_t part, mass, ids, ps, acc, user_frag, user_frag_t, item_frag, item_frag_t, item_data, user_data, user_data_t, mask_row, part_m, part_l, part_o, entry, entry_at, part_items, part_bias, bytes;
 };
 static FusedLayout fused_layout(const rfm_distill_args *a) {
@@ -350,9 +391,12 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     w.item_tiles = (a->n_items + 31) / 32;
     w.user_blocks = (w.user_tiles + w.waves - 1) / w.waves;
     w.item_blocks = (w.item_tiles + w.waves - 1) / w.waves;
-    const int slots = kCus * (w.kp == 32 ? 4 : w.kp == 64 ? 3 : 1);              // workgroups that fit on the chip at once, by registers and LDS
+    const int slots = kCus * (w.kp <= 64 ? 3 : 1);              // workgroups that fit on the chip at once, by registers and LDS
     w.splits_f = pick_splits(w.user_blocks, w.item_tiles, slots);
-    w.splits_i = grad ? pick_splits(w.item_blocks, w.user_tiles, slots) : 1;
+    // items_kernel: equal ranges for the workgroups that fit on the chip at once, no shorter than 4 tiles (or a block, if that is less)
+    const long long units = (long long)w.item_blocks * w.user_tiles;
+    w.units_i = (int)std::max<long long>((units + slots - 1) / slots, std::min(w.user_tiles, 4));
+    w.groups_i = (int)((units + w.units_i - 1) / w.units_i);
     const size_t ur = (size_t)w.user_tiles * 32, ir = (size_t)w.item_tiles * 32;
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += up(bytes ? bytes : 1); return at; };
@@ -363,8 +407,9 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     w.item_data = take((size_t)w.item_tiles * kItemData * 4); w.user_data = take((size_t)w.user_tiles * kUserData * 4); w.user_data_t = take((size_t)w.user_tiles * kUserData * 4);
     w.mask_row = take(a->allowed ? 4 * ur : 0);
     w.part_m = take(4 * w.splits_f * ur); w.part_l = take(4 * w.splits_f * ur); w.part_o = take(grad ? 4 * w.splits_f * ur * kp : 0);
-    w.entry = take(grad ? ur * n * 8 : 0); w.entry_at = take(grad ? 4 * (size_t)w.user_tiles * (w.item_blocks + 1) : 0);
-    w.part_items = take(grad ? 4 * w.splits_i * ir * kp : 0); w.part_bias = take(grad ? 4 * w.splits_i * ir : 0);
+    w.entry = take(grad ? ur * n * 8 : 0); w.entry_at = take(grad ? 4 * (size_t)w.user_tiles * (kBuckets + 1) : 0);
+    const size_t parts = (size_t)(w.groups_i + w.item_blocks) * w.waves * 32;
+    w.part_items = take(grad ? 4 * parts * kp : 0); w.part_bias = take(grad ? 4 * parts : 0);
     w.bytes = off;
     return w;
 }
@@ -375,10 +420,6 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     auto at = [&](size_t off) { return base + off; };
     float *part = (float *)at(w.part), *mass = (float *)at(w.mass), *acc = (float *)at(w.acc), *ps = (float *)at(w.ps);
     int32_t *ids = (int32_t *)at(w.ids);
-    const size_t lds = (size_t)a->n_teacher * 2 * 4 * 4;
-    const dim3 rows4((unsigned)((a->n_rows + 3) / 4));
-    if (grad) teacher_kernel<false, KP / 16><<<rows4, dim3(256), lds, stream>>>(*a, part, mass, ids, ps, acc);
-    else teacher_kernel<false, 0><<<rows4, dim3(256), lds, stream>>>(*a, part, mass, nullptr, nullptr, nullptr);
     FusedArgs f = {};
     f.a = *a;
     f.user_tiles = w.user_tiles; f.item_tiles = w.item_tiles; f.item_blocks = w.item_blocks;
@@ -388,7 +429,10 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     f.entry = (uint2 *)at(w.entry); f.entry_at = (int32_t *)at(w.entry_at);
     f.part_items = (float *)at(w.part_items); f.part_bias = (float *)at(w.part_bias);
     const float c = 1.4426950408889634f / a->temperature;
-    frags_kernel<KP><<<dim3((unsigned)(w.user_tiles + w.item_tiles)), dim3(256), 0, stream>>>(f, c, mass);
+    const size_t lds = (size_t)a->n_teacher * 2 * 4 * 4;
+    const dim3 grid_p((unsigned)(w.user_tiles + w.item_tiles + (a->n_rows + 3) / 4));
+    if (grad) prepare_kernel<KP, true><<<grid_p, dim3(256), lds, stream>>>(f, c, part, mass, ids, ps, acc);
+    else prepare_kernel<KP, false><<<grid_p, dim3(256), lds, stream>>>(f, c, part, mass, nullptr, nullptr, nullptr);
     f.splits = w.splits_f;
     f.chunk = (w.item_tiles + w.splits_f - 1) / w.splits_f;
     const dim3 grid_f((unsigned)(w.user_blocks * w.splits_f)), threads(WAVES * 64);
@@ -396,18 +440,15 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     else if (grad) forward_kernel<KP, true, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
     else if (a->allowed) forward_kernel<KP, false, true, WAVES><<<grid_f, threads, 0, stream>>>(f);
     else forward_kernel<KP, false, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
-    join_rows_kernel<KP><<<dim3((unsigned)(w.user_tiles * 8)), dim3(256), 0, stream>>>(f, part, mass, acc);
+    const int row_blocks = w.user_tiles * 4;
+    join_rows_kernel<KP><<<dim3((unsigned)(row_blocks + (grad ? w.user_tiles : 0))), dim3(512), 0, stream>>>(f, row_blocks, WAVES * 32, part, mass, acc, ids, ps);
     if (!grad) return RFM_OK;
-    int p2 = 64;
-    while (p2 < 32 * a->n_teacher) p2 <<= 1;
-    sort_entries_kernel<<<dim3((unsigned)w.user_tiles), dim3(256), (size_t)p2 * 8, stream>>>(a->n_rows, a->n_teacher, WAVES * 32, w.item_blocks, p2, ids, ps, f.entry, f.entry_at);
-    f.splits = w.splits_i;
-    f.chunk = (w.user_tiles + w.splits_i - 1) / w.splits_i;
-    const dim3 grid_i((unsigned)(w.item_blocks * w.splits_i));
+    f.units = w.units_i;
+    const dim3 grid_i((unsigned)w.groups_i);
     if (a->allowed) items_kernel<KP, true, WAVES><<<grid_i, threads, 0, stream>>>(f);
     else items_kernel<KP, false, WAVES><<<grid_i, threads, 0, stream>>>(f);
-    const long long n = (long long)a->n_items * a->n_factors;
-    join_items_kernel<KP><<<dim3((unsigned)std::min<long long>(8192, (n + 255) / 256)), dim3(256), 0, stream>>>(f);
+    // (a block is cut where a range ends inside it)
+    if (w.groups_i > 1 && w.units_i % w.user_tiles != 0) join_items_kernel<KP, WAVES><<<dim3((unsigned)(w.item_blocks * WAVES)), dim3(256), 0, stream>>>(f);
     return RFM_OK;
 }
 

@@ -29,8 +29,8 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kItemData = 64;                    // floats that travel with an item tile: 32 biases (log2 units), 2^-e, e, 2^e, for its scale 2^e
-constexpr int kUserData = 64;                    // ... with each copy of a user tile: 32 lse (log2 units) and 2^-e; 32 coefficients, e and 2^e
-constexpr int kFusedTeacher = 256;               // teacher entries of the fused path: a tile's 32 x n entries are sorted in LDS
+constexpr int kUserData = 64;                    // ... with a user tile: 32 lse (log2 units), 2^-e of one copy, e and 2^e of the other; and 32 coefficients
+constexpr int kBuckets = 1024;                   // of a tile's teacher entries, by block of items
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kUnit = 7.0f;                    // a column's largest weight is 2^7 when its maximum is set, and at most 2^15 (fp16 ends at 2^16)
 constexpr float kLimit = 15.0f;
@@ -38,19 +38,22 @@ constexpr float kLimit = 15.0f;
 template <int KP> struct Frag {
     static constexpr int steps = KP / 16, cols = KP / 32;
     static constexpr int bytes = KP * 128;       // one copy of a tile: KP / 16 x 2 parts x 1 KB; the transposed copy has as many
+    static constexpr int waves = KP <= 64 ? 4 : 8;               // wavefronts of a workgroup
+    static constexpr int per_simd = KP <= 64 ? 3 : 2;             // wavefronts per SIMD that the registers are kept to
 };
 
 struct FusedArgs {
     rfm_distill_args a;
     int user_tiles, item_tiles, item_blocks;     // tiles of 32 rows; blocks of items_kernel's workgroups
-    int splits, chunk;                           // of the streamed tiles
+    int splits, chunk;                           // forward: how the item tiles are split
+    int units;                                   // items: (block, user tile) pairs per workgroup
     char *user_frag, *user_frag_t, *item_frag, *item_frag_t;
     float *item_data, *user_data, *user_data_t;  // [item_tiles, kItemData], [user_tiles, kUserData] twice
     int32_t *mask_row;                           // [user_tiles * 32] mask of each row, -1 = none
     float *part_m, *part_l, *part_o;             // forward: [splits, user_tiles * 32 (, KP)]
-    uint2 *entry;                                // [user_tiles, 32 n]: (item << 5 | row, p), ascending
-    int32_t *entry_at;                           // [user_tiles, item_blocks + 1] where a block's entries begin
-    float *part_items, *part_bias;               // items: [splits, item_tiles * 32 (, KP)]
+    uint2 *entry;                                // [user_tiles, 32 n]: (item << 5 | row, p), by bucket
+    int32_t *entry_at;                           // [user_tiles, kBuckets + 1] where a bucket's entries begin
+    float *part_items, *part_bias;               // items: [workgroups + item_blocks, rows of a block (, KP)]
 };
 
 __device__ __forceinline__ void split2(float x, _Float16 &h, _Float16 &m) {
@@ -74,7 +77,7 @@ __device__ __forceinline__ float block_max(float x, float *s_max) {
 }
 
 // One workgroup per tile of 32 rows of a table: its fragments.  One copy holds row * `by`, the transposed one row * weight[row] (1 without), each with
-// a scale of its own.  Rows without a usable teacher entry (live) count as zeros: they may be padding.
+// a scale of its own.  Rows without a usable teacher entry (live [32]) count as zeros: they may be padding.
 template <int KP>
 __device__ void write_frags(const float *__restrict__ x, long long stride, int tile, long long rows, int factors, float by, const float *__restrict__ live,
                             const float *__restrict__ weight, float all_weight, char *frag, char *frag_t, float *lds, float *s_max, int *e_out, int *e_t_out) {
@@ -84,7 +87,7 @@ __device__ void write_frags(const float *__restrict__ x, long long stride, int t
         const int row = e / KP, k = e % KP;
         const long long r = (long long)tile * 32 + row;
         float v = 0.0f;
-        if (r < rows && k < factors && (!live || live[r] > 0.0f)) {
+        if (r < rows && k < factors && (!live || live[row] > 0.0f)) {
             v = x[r * stride + k];
             const float a = fabsf(v * by), b = fabsf(v * (weight ? weight[r] * all_weight : all_weight));
             if (a < INFINITY) big = fmaxf(big, a);
@@ -125,19 +128,34 @@ __device__ void write_frags(const float *__restrict__ x, long long stride, int t
     }
 }
 
-template <int KP>
-__global__ void __launch_bounds__(256) frags_kernel(const FusedArgs f, float c, const float *__restrict__ mass) {
-    __shared__ float lds[32 * (KP + 1)], s_max[4];
+// One launch: the users' tiles, the items' tiles, and (workgroups behind them) the teacher's rows, four per workgroup.
+template <int KP, bool GRAD>
+__global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ ids,
+                                                      float *__restrict__ ps, float *__restrict__ acc) {
+    extern __shared__ int s_dyn[];
+    __shared__ float lds[32 * (KP + 1)], s_max[4], live[32];
     const rfm_distill_args &a = f.a;
-    const bool grad = a.d_users != nullptr;
     const int b = blockIdx.x;
     int e, e_t;
     if (b < f.user_tiles) {
-        write_frags<KP>(a.users, a.user_stride, b, a.n_rows, a.n_factors, c, mass, grad ? a.row_weight : nullptr, a.temperature, f.user_frag, grad ? f.user_frag_t : nullptr, lds, s_max, &e, &e_t);
+        // a row is live when its list has a usable entry (and its mask exists): 8 threads look through each
+        {
+            const int row = threadIdx.x >> 3, sub = threadIdx.x & 7;
+            const long long r = (long long)b * 32 + row;
+            bool some = false, bad = false;
+            if (r < a.n_rows) {
+                const uint32_t *mask = row_mask(a, r, &bad);
+                for (int j = sub; j < a.n_teacher; j += 8) some |= usable(a, mask, a.teacher_items[(size_t)r * a.n_teacher + j], a.teacher_scores[(size_t)r * a.n_teacher + j]);
+            }
+            const unsigned long long any = __ballot(some && !bad);
+            if (sub == 0) live[row] = (any >> ((threadIdx.x & 63) & ~7)) & 0xff ? 1.0f : 0.0f;
+        }
+        __syncthreads();
+        write_frags<KP>(a.users, a.user_stride, b, a.n_rows, a.n_factors, c, live, GRAD ? a.row_weight : nullptr, a.temperature, f.user_frag, GRAD ? f.user_frag_t : nullptr, lds, s_max, &e, &e_t);
         if (threadIdx.x == 0) {
             f.user_data[(size_t)b * kUserData + 32] = ldexpf(1.0f, -e);
-            f.user_data_t[(size_t)b * kUserData + 32] = (float)e_t;
-            f.user_data_t[(size_t)b * kUserData + 33] = ldexpf(1.0f, e_t);
+            f.user_data[(size_t)b * kUserData + 33] = (float)e_t;
+            f.user_data[(size_t)b * kUserData + 34] = ldexpf(1.0f, e_t);
         }
         if (threadIdx.x < 32 && a.allowed) {
             const long long r = (long long)b * 32 + threadIdx.x;
@@ -145,15 +163,17 @@ __global__ void __launch_bounds__(256) frags_kernel(const FusedArgs f, float c, 
             if (r < a.n_rows) m = a.allowed_rows ? (long long)a.allowed_rows[r] : (a.n_allowed == 1 ? 0 : r);
             f.mask_row[r] = m >= 0 && m < a.n_allowed ? (int32_t)m : -1;
         }
-    } else {
+    } else if (b < f.user_tiles + f.item_tiles) {
         const int t = b - f.user_tiles;
-        write_frags<KP>(a.items, a.item_stride, t, a.n_items, a.n_factors, 1.0f, nullptr, nullptr, 1.0f, f.item_frag, grad ? f.item_frag_t : nullptr, lds, s_max, &e, &e_t);
+        write_frags<KP>(a.items, a.item_stride, t, a.n_items, a.n_factors, 1.0f, nullptr, nullptr, 1.0f, f.item_frag, GRAD ? f.item_frag_t : nullptr, lds, s_max, &e, &e_t);
         float *data = f.item_data + (size_t)t * kItemData;
         if (threadIdx.x < 32) {
             const long long i = (long long)t * 32 + threadIdx.x;
             data[threadIdx.x] = i < a.n_items ? (a.bias ? a.bias[i] * c : 0.0f) : -INFINITY;
         }
         if (threadIdx.x == 32) { data[32] = ldexpf(1.0f, -e); data[33] = (float)e_t; data[34] = ldexpf(1.0f, e_t); }
+    } else {
+        teacher_row<GRAD, GRAD ? KP / 64 + (KP % 64 != 0) : 0>(a, (long long)(b - f.user_tiles - f.item_tiles) * 4 + (threadIdx.x >> 6), KP, s_dyn, part, mass, ids, ps, acc);
     }
 }
 
@@ -246,6 +266,24 @@ __device__ __forceinline__ void load_columns(const char *frag, int tile, int lan
 #pragma unroll
         for (int p = 0; p < 2; ++p) x[k][p] = src[k * 128 + p * 64];
 }
+// s where bit (r & 3) + 8 (r >> 2) of w is set for register r, else -inf
+__device__ __forceinline__ void mask16(f32x16 &s, unsigned w) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const unsigned keep = (unsigned)((int)(w << (31 - ((r & 3) + 8 * (r >> 2)))) >> 31);
+        s[r] = __uint_as_float((keep & __float_as_uint(s[r])) | (~keep & 0xff800000u));
+    }
+}
+// ... and where the mask of register r's row holds the bit of this lane's column: lane i holds the word of row i.  Two rows' words, one for each
+// half of the wavefront, are a mask of lanes as they stand
+__device__ __forceinline__ void mask16_rows(f32x16 &s, unsigned word) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int row = (r & 3) + 8 * (r >> 2);
+        const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)word, row), hi = (unsigned)__builtin_amdgcn_readlane((int)word, row + 4);
+        s[r] = __builtin_amdgcn_inverse_ballot_w64((unsigned long long)hi << 32 | lo) ? s[r] : -INFINITY;
+    }
+}
 __device__ __forceinline__ float largest16(const f32x16 &s) {
     float high = s[0];
 #pragma unroll
@@ -266,7 +304,7 @@ __device__ __forceinline__ float sum16(const f32x16 &s) {
 // Block b: split b % splits of the items, columns block b / splits: with a multiple of 8 splits the workgroups of one XCD stream the same items.
 // The loop is one tile deep in flight: while the vector unit turns tile t's scores into weights, the matrix cores make tile t + 1's.
 template <int KP, bool GRAD, bool MASK, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, 2) forward_kernel(const FusedArgs f) {
+__global__ void __launch_bounds__(WAVES * 64, Frag<KP>::per_simd) forward_kernel(const FusedArgs f) {
     constexpr int kBytes = Frag<KP>::bytes, kBuf = kBytes + kItemData * 4;
     __shared__ __attribute__((aligned(16))) char buf[2][kBuf], buf_t[GRAD ? 2 : 1][GRAD ? kBytes : 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5;
@@ -303,9 +341,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) forward_kernel(const FusedArgs 
             for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(s[4 * q + k], by, b[k]);
         }
         if constexpr (MASK) {
-            const unsigned w = word >> (4 * half);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = (w >> ((r & 3) + 8 * (r >> 2))) & 1u ? s[r] : -INFINITY;
+            mask16(s, word >> (4 * half));
         }
         high = largest16(s) - e;
     };
@@ -366,12 +402,11 @@ __global__ void __launch_bounds__(WAVES * 64, 2) forward_kernel(const FusedArgs 
     }
 }
 
-// One wavefront per row: the splits joined; loss, the users' gradient, and what items_kernel needs of the row.
+// One wavefront per row: the splits joined; loss, the users' gradient, and what items_kernel needs of the row.  weight: 64 floats of LDS
 template <int KP>
-__global__ void __launch_bounds__(256) join_rows_kernel(const FusedArgs f, const float *__restrict__ part, const float *__restrict__ mass, const float *__restrict__ acc) {
+__device__ void join_row(const FusedArgs &f, long long r, const float *__restrict__ part, const float *__restrict__ mass, const float *__restrict__ acc, float *weight) {
     const int lane = threadIdx.x & 63;
-    const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), padded = (long long)f.user_tiles * 32;
-    if (r >= padded) return;
+    const long long padded = (long long)f.user_tiles * 32;
     const bool grad = f.a.d_users != nullptr;
     const size_t at = (size_t)(r >> 5) * kUserData + (r & 31);
     const float has = r < f.a.n_rows ? mass[r] : 0.0f;
@@ -387,91 +422,125 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const FusedArgs f, const
     float top = kLowest;
     for (int s = lane; s < f.splits; s += 64) top = fmaxf(top, f.part_m[(size_t)s * padded + r]);
     top = wave_max(top);
-    float total = 0.0f;
-    for (int s = lane; s < f.splits; s += 64) total += f.part_l[(size_t)s * padded + r] * __builtin_amdgcn_exp2f(f.part_m[(size_t)s * padded + r] - top);
+    float total = 0.0f, o[(KP + 63) / 64] = {0.0f};
+    for (int s0 = 0; s0 < f.splits; s0 += 64) {
+        const int s = s0 + lane;
+        const float w = s < f.splits ? __builtin_amdgcn_exp2f(f.part_m[(size_t)s * padded + r] - top) : 0.0f;
+        if (s < f.splits) total += f.part_l[(size_t)s * padded + r] * w;
+        if (!grad) continue;
+        weight[lane] = w;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int count = min(64, f.splits - s0);
+        const float *from = f.part_o + ((size_t)s0 * padded + r) * KP;
+#pragma unroll 4
+        for (int q = 0; q < count; ++q) {
+#pragma unroll
+            for (int k = 0; k < (KP + 63) / 64; ++k)
+                if (KP % 64 == 0 || k * 64 + lane < KP) o[k] = fmaf(from[(size_t)q * padded * KP + k * 64 + lane], weight[q], o[k]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
     total = wave_sum(total);
     const float lse2 = top - kUnit + log2f(total);
     if (lane == 0) f.a.loss[r] = f.a.temperature * f.a.temperature * (part[r] + lse2 * 0.693147180559945309f);
     if (!grad) return;
     const float coef = f.a.temperature * (f.a.row_weight ? f.a.row_weight[r] : 1.0f);
     if (lane == 0) { f.user_data[at] = lse2; f.user_data_t[at] = coef; }
-    for (int k = lane; k < f.a.n_factors; k += 64) {
-        float o = 0.0f;
-        for (int s = 0; s < f.splits; ++s) o += f.part_o[((size_t)s * padded + r) * KP + k] * __builtin_amdgcn_exp2f(f.part_m[(size_t)s * padded + r] - top);
-        f.a.d_users[(size_t)r * f.a.n_factors + k] = coef * (o / total - acc[(size_t)r * KP + k]);
+#pragma unroll
+    for (int k = 0; k < (KP + 63) / 64; ++k)
+        if (k * 64 + lane < f.a.n_factors) f.a.d_users[(size_t)r * f.a.n_factors + k * 64 + lane] = coef * (o[k] / total - acc[(size_t)r * KP + k * 64 + lane]);
+}
+
+// One workgroup per tile of 32 rows: the tile's teacher entries by the block of items_kernel that they fall into, modulo kBuckets (a block skips what
+// is not its own).  Their order inside a bucket is whatever it comes to: no two of them are the same item of the same row, and all that is done
+// with them is to be written to that place.  count: kBuckets + 8 ints of LDS.
+__device__ void bucket_entries(const FusedArgs &f, int tile, int block_items, const int32_t *__restrict__ item, const float *__restrict__ p, int *count) {
+    const int n = f.a.n_teacher, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long r0 = (long long)tile * 32;
+    const int entries = (int)min(32ll, f.a.n_rows - r0) * n;
+    static_assert(kBuckets == 1024, "two counters per thread of 512");
+    count[threadIdx.x] = 0;
+    count[threadIdx.x + 512] = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < entries; e += 512) {
+        const int i = item[r0 * n + e];
+        if (i >= 0) atomicAdd(count + (i / block_items) % kBuckets, 1);
+    }
+    __syncthreads();
+    const int c0 = count[2 * threadIdx.x], c1 = count[2 * threadIdx.x + 1];
+    int before = c0 + c1;                                        // inclusive prefix over the wavefront, then over the wavefronts
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(before, d);
+        if (lane >= d) before += o;
+    }
+    if (lane == 63) count[kBuckets + wave] = before;
+    __syncthreads();
+    int add = 0;
+    for (int w = 0; w < wave; ++w) add += count[kBuckets + w];
+    const int at1 = add + before - c1, at0 = at1 - c0;
+    count[2 * threadIdx.x] = at0;
+    count[2 * threadIdx.x + 1] = at1;
+    int32_t *at = f.entry_at + (size_t)tile * (kBuckets + 1);
+    at[2 * threadIdx.x] = at0;
+    at[2 * threadIdx.x + 1] = at1;
+    if (threadIdx.x == 511) at[kBuckets] = at1 + c1;
+    __syncthreads();
+    uint2 *out = f.entry + (size_t)tile * 32 * n;
+    for (int e = threadIdx.x; e < entries; e += 512) {
+        const int i = item[r0 * n + e];
+        if (i >= 0) out[atomicAdd(count + (i / block_items) % kBuckets, 1)] = make_uint2((unsigned)i << 5 | (unsigned)(e / n), __float_as_uint(p[r0 * n + e]));
     }
 }
 
-// One workgroup per tile of 32 rows: the tile's usable teacher entries by item (and row), an item that stands in a row's list more than once as one
-// entry, and where each block of items_kernel begins in them.
-__global__ void __launch_bounds__(256) sort_entries_kernel(long long rows, int n, int block_items, int blocks, int p2, const int32_t *__restrict__ item,
-                                                           const float *__restrict__ p, uint2 *__restrict__ entry, int32_t *__restrict__ entry_at) {
-    extern __shared__ unsigned long long s_key[];
-    const long long r0 = (long long)blockIdx.x * 32;
-    const int count = (int)min(32ll, rows - r0) * n;
-    for (int e = threadIdx.x; e < p2; e += 256) {
-        const int i = e < count ? item[r0 * n + e] : -1;
-        s_key[e] = i >= 0 ? ((unsigned long long)(unsigned)i << 13) | (unsigned)(e / n) << 8 | (unsigned)(e % n) : ~0ull;
+// Two things that wait for different kernels and for nothing of each other, in one launch: the rows joined (8 per workgroup), and the tiles' entries
+// (workgroups behind the rows').
+template <int KP>
+__global__ void __launch_bounds__(512) join_rows_kernel(const FusedArgs f, int row_blocks, int block_items, const float *__restrict__ part, const float *__restrict__ mass,
+                                                        const float *__restrict__ acc, const int32_t *__restrict__ item, const float *__restrict__ p) {
+    __shared__ int lds[kBuckets + 8];
+    if ((int)blockIdx.x >= row_blocks) {
+        bucket_entries(f, (int)blockIdx.x - row_blocks, block_items, item, p, lds);
+        return;
     }
-    __syncthreads();
-    for (int k = 2; k <= p2; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int t = threadIdx.x; t < p2 / 2; t += 256) {
-                const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1)), l = i + j;
-                const unsigned long long a = s_key[i], b = s_key[l];
-                if ((a > b) == ((i & k) == 0)) { s_key[i] = b; s_key[l] = a; }
-            }
-            __syncthreads();
-        }
-    uint2 *out = entry + (size_t)blockIdx.x * 32 * n;
-    for (int e = threadIdx.x; e < 32 * n; e += 256) {
-        const unsigned long long key = s_key[e];
-        if (key == ~0ull) { out[e] = make_uint2(0xffffffffu, 0); continue; }
-        auto value = [&](unsigned long long k) { return p[(r0 + ((k >> 8) & 31)) * n + (k & 255)]; };
-        float v = 0.0f;
-        if (e == 0 || (s_key[e - 1] >> 8) != (key >> 8)) {       // the first of its item and row takes the others
-            v = value(key);
-            for (int q = e + 1; q < 32 * n && (s_key[q] >> 8) == (key >> 8); ++q) v += value(s_key[q]);
-            out[e] = make_uint2((unsigned)(key >> 8), __float_as_uint(v));
-        } else out[e] = make_uint2(0xffffffffu, 0);
-    }
-    int32_t *at = entry_at + (size_t)blockIdx.x * (blocks + 1);
-    for (int b = threadIdx.x; b <= blocks; b += 256) {
-        const unsigned long long first = (unsigned long long)b * block_items << 13;
-        int lo = 0, hi = 32 * n;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (s_key[mid] < first) lo = mid + 1; else hi = mid;
-        }
-        at[b] = lo;
-    }
+    const int wave = threadIdx.x >> 6;
+    join_row<KP>(f, (long long)blockIdx.x * 8 + wave, part, mass, acc, reinterpret_cast<float *>(lds) + wave * 64);
 }
 
 // The items' gradient.  p of the teacher enters through a 32 x 32 patch of LDS per wavefront: the few entries that fall into the tile are written
 // there, read back as the lanes hold dz, and cleared; a wavefront's LDS operations run in order, so no barrier is needed.
 constexpr int kPatch = 36;                       // floats per item of the patch: 32 rows, and 16-byte reads without bank conflicts
+// The work is cut into equal ranges of (block of items, user tile) pairs, one per workgroup that fits on the chip: no workgroup waits for a last
+// round.  A block that lies inside one range is written out as it is; the others' parts go to slot workgroup + block -- workgroups and blocks
+// both ascend along the ranges, so no two parts share one -- and are joined in that order.
 template <int KP, bool MASK, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, 2) items_kernel(const FusedArgs f) {
+__global__ void __launch_bounds__(WAVES * 64, Frag<KP>::per_simd) items_kernel(const FusedArgs f) {
     constexpr int kBytes = Frag<KP>::bytes, kBuf = kBytes + kUserData * 4;
     __shared__ __attribute__((aligned(16))) char buf[2][kBuf], buf_t[2][kBuf];
     __shared__ __attribute__((aligned(16))) float patches[WAVES][32 * kPatch];
-    __shared__ __attribute__((aligned(16))) unsigned words[MASK ? WAVES : 1][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
-    const int split = (int)blockIdx.x % f.splits, block = (int)blockIdx.x / f.splits, tile = block * WAVES + wave;
-    const int mine = tile < f.item_tiles ? tile : f.item_tiles - 1;
-    const int t0 = split * f.chunk, t1 = min(t0 + f.chunk, f.user_tiles), n32 = 32 * f.a.n_teacher;
+    const int n32 = 32 * f.a.n_teacher;
     float *patch = patches[wave];
     for (int k = lane; k < 32 * kPatch; k += 64) patch[k] = 0.0f;
+    const long long last_unit = min((long long)(blockIdx.x + 1) * f.units, (long long)f.item_blocks * f.user_tiles);
+    for (long long unit = (long long)blockIdx.x * f.units; unit < last_unit;) {
+    const int block = (int)(unit / f.user_tiles), t0 = (int)(unit - (long long)block * f.user_tiles);
+    const int t1 = (int)min((long long)f.user_tiles, t0 + (last_unit - unit));
+    unit += t1 - t0;
+    const int tile = block * WAVES + wave, mine = tile < f.item_tiles ? tile : f.item_tiles - 1;
     f16x8 x[Frag<KP>::steps][2];
     load_columns<KP>(f.item_frag, mine, lane, x);
     const float bias = f.item_data[(size_t)mine * kItemData + col], unscale = f.item_data[(size_t)mine * kItemData + 32];
     const unsigned base = (unsigned)tile * 32u;
     f32x16 o[Frag<KP>::cols];
     for (int c = 0; c < Frag<KP>::cols; ++c) o[c] = f32x16{0};
-    float top = kLowest, d_bias = 0.0f;
+    // `gate`: what an exponent may reach before `top` is moved -- anything at first, so that the first weight of a column sets it
+    float top = 0.0f, gate = kLowest, d_bias = 0.0f;
     auto mask_word = [&](int t) {                                // of row `col` of the tile, the bits of this wavefront's items
         const int m = f.mask_row[t * 32 + col];
-        return m < 0 ? 0xffffffffu : f.a.allowed[(size_t)m * (size_t)f.item_tiles + mine];
+        return f.a.allowed[(size_t)max(m, 0) * (size_t)f.item_tiles + mine] | (unsigned)(m >> 31);
     };
     auto stage_scores = [&](int t) {
         stage_copy<KP, WAVES>(f.user_frag, t, buf[t & 1], wave, lane);
@@ -482,66 +551,58 @@ __global__ void __launch_bounds__(WAVES * 64, 2) items_kernel(const FusedArgs f)
         stage_data(f.user_data_t + (size_t)t * kUserData, buf_t[t & 1] + kBytes, wave, lane);
     };
     unsigned word = 0, next_word = 0;
-    auto finish = [&](int t, f32x16 &s, float &high) {           // log2 of q of tile t out of its products
+    // the exponents of tile t's weights, for `top` as it stands, out of its products; and the tile's scale
+    auto finish = [&](int t, f32x16 &s, float &high, float &e, float &scale) {
         const f32x4 *data = reinterpret_cast<const f32x4 *>(buf[t & 1] + kBytes);
-        const float by = data[8][0] * unscale;
+        const f32x4 last = data[8];
+        const float by = last[0] * unscale;
+        e = last[1];
+        scale = last[2];
+        const float shift = bias - (top + (e - kUnit));
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const f32x4 lse = data[half + 2 * q];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(s[4 * q + k], by, bias) - lse[k];
+            for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(s[4 * q + k], by, shift) - lse[k];
         }
-        if constexpr (MASK) {
-            if (half == 0) words[wave][col] = word;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const u32x4 w = reinterpret_cast<const u32x4 *>(words[wave])[2 * q + half];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[4 * q + k] = (w[k] >> col) & 1u ? s[4 * q + k] : -INFINITY;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
+        if constexpr (MASK) mask16_rows(s, word);
         high = largest16(s);
     };
     if constexpr (MASK) { word = mask_word(t0); next_word = mask_word(min(t0 + 1, t1 - 1)); }
-    int begin = f.entry_at[(size_t)t0 * (f.item_blocks + 1) + block], end = f.entry_at[(size_t)t0 * (f.item_blocks + 1) + block + 1];
+    const int bucket = block % kBuckets;
+    int begin = f.entry_at[(size_t)t0 * (kBuckets + 1) + bucket], end = f.entry_at[(size_t)t0 * (kBuckets + 1) + bucket + 1];
     stage_scores(t0);
     stage_rest(t0);
     staged();
     if (t0 + 1 < t1) stage_scores(t0 + 1);
-    auto step = [&](int t, f32x16 &s, float high, f32x16 &next, float &next_high) {
+    auto step = [&](int t, f32x16 &s, float high, float e, float scale, f32x16 &next, float &next_high, float &next_e, float &next_scale) {
         staged();
         const int from = begin, to = end;
         uint2 entry = make_uint2(0xffffffffu, 0);
         if (from + lane < to) entry = f.entry[(size_t)t * n32 + from + lane];
         if (t + 1 < t1) {
-            begin = f.entry_at[(size_t)(t + 1) * (f.item_blocks + 1) + block];
-            end = f.entry_at[(size_t)(t + 1) * (f.item_blocks + 1) + block + 1];
+            begin = f.entry_at[(size_t)(t + 1) * (kBuckets + 1) + bucket];
+            end = f.entry_at[(size_t)(t + 1) * (kBuckets + 1) + bucket + 1];
             if constexpr (MASK) {
                 word = next_word;
-                if (t + 2 < t1) next_word = mask_word(t + 2);
+                next_word = mask_word(min(t + 2, t1 - 1));
             }
             if (t + 2 < t1) stage_scores(t + 2);
             stage_rest(t + 1);
         }
         const f32x4 *data = reinterpret_cast<const f32x4 *>(buf_t[t & 1] + kBytes);
-        const float e = data[8][0], scale = data[8][1];
         float by = 1.0f;
-        high -= e;
-        if (__any(high > top + (kLimit - kUnit))) {
-            const float now = fmaxf(top, ceilf(fmaxf(high, __shfl_xor(high, 32))));
-            by = __builtin_amdgcn_exp2f(top - now);
-            top = now;
+        if (__any(high > gate)) {
+            const float h = fmaxf(high, __shfl_xor(high, 32)), more = h > gate ? ceilf(h - kUnit) : 0.0f;
+            by = gate == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);         // (1: there is nothing to scale yet)
+            gate = h > gate ? kLimit : gate;
+            top += more;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] -= more;
         }
         next = tile_scores<KP>(buf[(t + 1) & 1], lane, x);       // (behind the last tile: of what is left in LDS, and not used)
-        {
-            const float off = top + (e - kUnit);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - off);
-        }
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
         // the teacher's share
         bool any = false;
         for (int k = from; k < to; k += 64) {
@@ -556,27 +617,29 @@ __global__ void __launch_bounds__(WAVES * 64, 2) items_kernel(const FusedArgs f)
             __builtin_amdgcn_wave_barrier();
             f32x4 *cell = reinterpret_cast<f32x4 *>(patch + col * kPatch + 4 * half);
             f32x4 p[4];
-            float most = 0.0f;
+            unsigned most = 0;                                   // (p is never negative: its bits order like its value)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 p[q] = cell[2 * q];
                 cell[2 * q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                most = fmaxf(fmaxf(most, fmaxf(p[q][0], p[q][1])), fmaxf(p[q][2], p[q][3]));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(p[q][k]));
             }
-            const float log_p = log2f(most) - e;                 // (-inf where there is none)
-            if (__any(log_p > top + (kLimit - kUnit))) {
-                const float now = fmaxf(top, ceilf(fmaxf(log_p, __shfl_xor(log_p, 32))));
-                const float by_p = __builtin_amdgcn_exp2f(top - now);
+            const float log_p = __builtin_amdgcn_logf(__uint_as_float(most)) - (top + (e - kUnit));          // (-inf where there is none)
+            if (__any(log_p > gate)) {
+                const float h = fmaxf(log_p, __shfl_xor(log_p, 32)), more = h > gate ? ceilf(h - kUnit) : 0.0f;
+                const float by_p = gate == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] *= by_p;
                 by *= by_p;
-                top = now;
+                gate = h > gate ? kLimit : gate;
+                top += more;
             }
-            const float unit = __builtin_amdgcn_exp2f(kUnit - e - top);
+            const float unit = fminf(__builtin_amdgcn_exp2f(kUnit - e - top), -kLowest);     // (finite where a column has no weight yet: 0 stays 0)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s[4 * q + k] -= p[q][k] == 0.0f ? 0.0f : p[q][k] * unit;
+                for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(p[q][k], -unit, s[4 * q + k]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
@@ -591,45 +654,72 @@ __global__ void __launch_bounds__(WAVES * 64, 2) items_kernel(const FusedArgs f)
         f16x8 p[2][2];
         split_weights(s, p);
         weighted_sum<KP>(buf_t[t & 1], lane, p, by, o);
-        finish(t + 1, next, next_high);
+        finish(t + 1, next, next_high, next_e, next_scale);
     };
     f32x16 s0 = tile_scores<KP>(buf[t0 & 1], lane, x), s1;
-    float h0, h1;
-    finish(t0, s0, h0);
+    float h0, h1, e0, e1, c0, c1;
+    finish(t0, s0, h0, e0, c0);
     for (int t = t0; t < t1; t += 2) {
-        step(t, s0, h0, s1, h1);
+        step(t, s0, h0, e0, c0, s1, h1, e1, c1);
         if (t + 1 >= t1) break;
-        step(t + 1, s1, h1, s0, h0);
+        step(t + 1, s1, h1, e1, c1, s0, h0, e0, c0);
     }
-    if (tile >= f.item_tiles) return;
+    __syncthreads();                                             // the buffers are free for the next block
     d_bias += __shfl_xor(d_bias, 32);
-    const float unit = __builtin_amdgcn_exp2f(top - kUnit);
-    const size_t at = (size_t)split * f.item_tiles * 32 + (size_t)tile * 32 + col;
-    if (half == 0) f.part_bias[at] = d_bias * unit;
+    const float unit_of = __builtin_amdgcn_exp2f(top - kUnit);
+    const bool whole = t0 == 0 && t1 == f.user_tiles;
+    const int item = tile * 32 + col, K = f.a.n_factors;
+    if (whole && item < f.a.n_items) {
+        float *out = f.a.d_items + (size_t)item * K;
+        const bool vector = (K & 3) == 0 && ((uintptr_t)f.a.d_items & 15) == 0;
+        if (half == 0 && f.a.d_bias) f.a.d_bias[item] = d_bias * unit_of;
 #pragma unroll
-    for (int c = 0; c < Frag<KP>::cols; ++c)
+        for (int c = 0; c < Frag<KP>::cols; ++c)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 v = {o[c][4 * q], o[c][4 * q + 1], o[c][4 * q + 2], o[c][4 * q + 3]};
-            *reinterpret_cast<f32x4 *>(f.part_items + at * KP + 32 * c + 8 * q + 4 * half) = v * unit;
-        }
+            for (int q = 0; q < 4; ++q) {
+                const int k = 32 * c + 8 * q + 4 * half;
+                const f32x4 v = f32x4{o[c][4 * q], o[c][4 * q + 1], o[c][4 * q + 2], o[c][4 * q + 3]} * unit_of;
+                if (vector) {
+                    if (k < K) *reinterpret_cast<f32x4 *>(out + k) = v;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (k + j < K) out[k + j] = v[j];
+                }
+            }
+    } else if (!whole) {
+        const size_t at = ((size_t)(blockIdx.x + block) * WAVES + wave) * 32 + col;
+        if (half == 0) f.part_bias[at] = d_bias * unit_of;
+#pragma unroll
+        for (int c = 0; c < Frag<KP>::cols; ++c)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<f32x4 *>(f.part_items + at * KP + 32 * c + 8 * q + 4 * half) = f32x4{o[c][4 * q], o[c][4 * q + 1], o[c][4 * q + 2], o[c][4 * q + 3]} * unit_of;
+    }
+    }
 }
 
-template <int KP>
+// One workgroup per tile of items: the parts of a block that was cut, in the order of its user tiles.
+template <int KP, int WAVES>
 __global__ void __launch_bounds__(256) join_items_kernel(const FusedArgs f) {
-    const long long padded = (long long)f.item_tiles * 32, n = (long long)f.a.n_items * f.a.n_factors;
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
-        const long long i = e / f.a.n_factors;
-        const int k = (int)(e - i * f.a.n_factors);
-        float s = 0.0f;
-        for (int q = 0; q < f.splits; ++q) s += f.part_items[((size_t)q * padded + i) * KP + k];
-        f.a.d_items[e] = s;
-        if (k == 0 && f.a.d_bias) {
-            float b = 0.0f;
-            for (int q = 0; q < f.splits; ++q) b += f.part_bias[(size_t)q * padded + i];
-            f.a.d_bias[i] = b;
-        }
+    const int block = (int)blockIdx.x / WAVES, in_block = (int)blockIdx.x % WAVES * 32, K = f.a.n_factors;
+    const int first = (int)((long long)block * f.user_tiles / f.units), last = (int)(((long long)(block + 1) * f.user_tiles - 1) / f.units);
+    if (first == last) return;
+    const int i0 = block * WAVES * 32 + in_block;
+    for (int e = threadIdx.x; e < 32 * KP / 4; e += 256) {
+        const int row = e / (KP / 4), k = e % (KP / 4) * 4;
+        if (i0 + row >= f.a.n_items || k >= K) continue;
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int g = first; g <= last; ++g) s += *reinterpret_cast<const f32x4 *>(f.part_items + ((size_t)(g + block) * WAVES * 32 + in_block + row) * KP + k);
+        float *out = f.a.d_items + (size_t)(i0 + row) * K + k;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (k + j < K) out[j] = s[j];
     }
+    if (!f.a.d_bias || threadIdx.x >= 32 || i0 + (int)threadIdx.x >= f.a.n_items) return;
+    float s = 0.0f;
+    for (int g = first; g <= last; ++g) s += f.part_bias[(size_t)(g + block) * WAVES * 32 + in_block + threadIdx.x];
+    f.a.d_bias[i0 + threadIdx.x] = s;
 }
 
 __global__ void __launch_bounds__(256) zero_kernel(float *x, long long n) {
