@@ -13,14 +13,13 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/rankfm_hip.h"
 
 namespace rfm {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 2048;                      // scores a workgroup holds in registers at a time: 8 per thread
-constexpr int kPer = kTile / kThreads;
 
 // one row's share of the rules; every index is checked against the array it points into, so no list can lead a read astray
 struct RowRules {
@@ -82,17 +81,17 @@ __device__ __forceinline__ void store_vec(T *p, const float *in) {
     __builtin_memcpy(reinterpret_cast<Chunk<T> *>(p), &c, sizeof(c));
 }
 
-// the eight scores of this thread out of items [first, first + kTile): vector j of the tile belongs to thread j % 256
+// The P scores of this thread out of items [first, first + 256 P): vector j of the tile belongs to thread j % 256.
 template <typename T>
 __device__ __forceinline__ int element(int slot) {               // position inside the tile of this thread's slot-th score
     constexpr int ve = Vec<T>::n;
     return ((slot / ve) * kThreads + (int)threadIdx.x) * ve + slot % ve;
 }
-template <typename T>
+template <typename T, int P>
 __device__ __forceinline__ void load_tile(const T *row, int first, int n_items, float *s) {
     constexpr int ve = Vec<T>::n;
 #pragma unroll
-    for (int j = 0; j < kPer / ve; ++j) {
+    for (int j = 0; j < P / ve; ++j) {
         const int i = first + (j * kThreads + (int)threadIdx.x) * ve;
         if (i + ve <= n_items) load_vec(row + i, s + j * ve);
         else {
@@ -102,26 +101,60 @@ __device__ __forceinline__ void load_tile(const T *row, int first, int n_items, 
     }
 }
 
-// where the row's lists name an item of the tile: count[item] of the history, and 1 + the position of the last bias entry
-__device__ __forceinline__ void scan_lists(const RowRules &w, int first, int *count, int *last) {
-    for (int k = threadIdx.x; k < kTile; k += kThreads) { count[k] = 0; last[k] = 0; }
+// x[k] of a lane's own k
+template <int N>
+__device__ __forceinline__ float pick(const float (&x)[N], int k) {
+    if constexpr (N == 1) return x[0];
+    else {
+        const unsigned upper = 0u - (unsigned)((k / (N / 2)) & 1);             // (bits, not an index: an indexed array would live in memory)
+        float half[N / 2];
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) half[j] = __uint_as_float((__float_as_uint(x[j + N / 2]) & upper) | (__float_as_uint(x[j]) & ~upper));
+        return pick<N / 2>(half, k);
+    }
+}
+
+// where the row's lists name an item of the tile: count[item] of the history, and 1 + the position of the last bias entry.  False (and nothing
+// written): they name none.
+template <int P>
+__device__ __forceinline__ bool scan_lists(const RowRules &w, int first, int *count, int *last) {
+    constexpr int tile = P * kThreads;
+    int here = 0;
+    for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) here |= (unsigned)(w.hist[k] - first) < (unsigned)tile;
+    for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) here |= (unsigned)(w.bias_item[k] - first) < (unsigned)tile;
+    if (!__syncthreads_or(here)) return false;
+    for (int k = threadIdx.x; k < tile; k += kThreads) { count[k] = 0; last[k] = 0; }
     __syncthreads();
     for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) {
         const unsigned at = (unsigned)(w.hist[k] - first);
-        if (at < (unsigned)kTile) atomicAdd(count + at, 1);
+        if (at < (unsigned)tile) atomicAdd(count + at, 1);
     }
     for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) {
         const unsigned at = (unsigned)(w.bias_item[k] - first);
-        if (at < (unsigned)kTile) atomicMax(last + at, (int)k + 1);
+        if (at < (unsigned)tile) atomicMax(last + at, (int)k + 1);
     }
     __syncthreads();
+    return true;
 }
 
-template <typename T, bool LISTS>
-__device__ __forceinline__ void apply_rules(const rfm_score_rules &u, const RowRules &w, int first, int n_items, const int *count, const int *last, float *s) {
+// the rules of an item that the row's lists name (an allowed one)
+__device__ __forceinline__ float listed_score(const rfm_score_rules &u, const RowRules &w, int item, int count, int last, float x) {
+    if (count > 0) {
+        x = x > 0.0f ? x / w.rho : x * w.rho;
+        x = x - w.phi * (float)count;
+        x = x - w.pi;
+    }
+    if (u.item_bias) x = x + u.item_bias[item];
+    if (last > 0) x = x + w.bias_value[last - 1];
+    return x;
+}
+
+template <typename T, int P, bool LISTS>
+__device__ __forceinline__ void apply_rules(const rfm_score_rules &u, const RowRules &w, int first, int n_items, const int *count, const int *last, float *s,
+                                            unsigned done = 0) {
     constexpr int ve = Vec<T>::n;
 #pragma unroll
-    for (int j = 0; j < kPer / ve; ++j) {
+    for (int j = 0; j < P / ve; ++j) {
         const int at = (j * kThreads + (int)threadIdx.x) * ve, i = first + at;
         if (i >= n_items) continue;
         unsigned bits = 0xffffffffu;
@@ -130,50 +163,104 @@ __device__ __forceinline__ void apply_rules(const rfm_score_rules &u, const RowR
             const unsigned long long both = ((unsigned long long)w.mask[word + 1 < words ? word + 1 : word] << 32) | w.mask[word];
             bits = (unsigned)(both >> (i & 31));
         }
+        float bias[ve];
+        if (!LISTS && u.item_bias) {
+            if (i + ve <= n_items) {
+#pragma unroll
+                for (int k = 0; k < ve; k += 4) load_vec(u.item_bias + i + k, bias + k);
+            } else {
+#pragma unroll
+                for (int k = 0; k < ve; ++k) bias[k] = i + k < n_items ? u.item_bias[i + k] : 0.0f;
+            }
+        }
 #pragma unroll
         for (int k = 0; k < ve; ++k) {
             float x = s[j * ve + k];
             if constexpr (LISTS) {
-                const int c = count[at + k];
-                if (c > 0) {
-                    x = x > 0.0f ? x / w.rho : x * w.rho;
-                    x = x - w.phi * (float)c;
-                    x = x - w.pi;
-                }
-            }
-            if (u.item_bias && i + k < n_items) x = x + u.item_bias[i + k];
-            if constexpr (LISTS) {
-                const int l = last[at + k];
-                if (l > 0) x = x + w.bias_value[l - 1];
+                if (i + k < n_items) x = listed_score(u, w, i + k, count[at + k], last[at + k], x);
+            } else {
+                if (u.item_bias) x = (done >> (j * ve + k)) & 1u ? x : x + bias[k];
             }
             s[j * ve + k] = (bits >> k) & 1u ? x : -INFINITY;
         }
     }
 }
 
-// One workgroup per (row, tile of 2048 items): the row is read and written once, which is the floor.  The lists cost a scan per tile.
-template <typename T>
+constexpr int kHits = 64;                        // list entries of a tile that are looked through one by one
+constexpr int kCounted = 2048;                   // items whose counts are in LDS at a time, where there are more
+struct Hits {
+    int n, item[kHits], entry[kHits];            // entry: 0 of the history, else 1 + the position of the bias
+};
+struct Counted {
+    int count[kCounted], last[kCounted];
+};
+
+// One workgroup per (row, tile of 256 P items): the row is read and written once, which is the floor.  The scores are asked for before the lists:
+// their way through three dependent loads passes meanwhile.  A tile's few list entries are gathered in LDS and looked through by the thread that
+// holds their item; where there are more than 64, counts per item are made, 2048 items at a time.
+template <typename T, int P>
 __global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score_rules u, long long row0, int tiles, int n_items, const T *__restrict__ scores,
                                                                  long long stride, T *out, long long out_stride) {
-    __shared__ int count[kTile], last[kTile];
+    __shared__ union { Hits hits; Counted counted; } lists;
     const long long r = row0 + blockIdx.x / tiles;
-    const int first = (int)(blockIdx.x % tiles) * kTile;
+    const int first = (int)(blockIdx.x % tiles) * P * kThreads;
+    if (threadIdx.x == 0) lists.hits.n = 0;
+    float s[P];
+    load_tile<T, P>(scores + r * stride, first, n_items, s);
     const RowRules w = row_rules(u, r, n_items);
-    float s[kPer];
-    load_tile(scores + r * stride, first, n_items, s);
     if (w.bad) {
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) s[k] = __uint_as_float(0x7fc00000u);
-    } else if (w.hist_n > 0 || w.bias_n > 0) {
-        scan_lists(w, first, count, last);
-        apply_rules<T, true>(u, w, first, n_items, count, last, s);
+        for (int k = 0; k < P; ++k) s[k] = __uint_as_float(0x7fc00000u);
     } else {
-        apply_rules<T, false>(u, w, first, n_items, count, last, s);
+        unsigned done = 0;                                       // the scores that the lists name: theirs are made here
+        bool many = false;
+        if (w.hist_n > 0 || w.bias_n > 0) {
+            __syncthreads();
+            auto note = [&](int item, int entry) {
+                if ((unsigned)(item - first) >= (unsigned)(P * kThreads)) return;
+                const int at = atomicAdd(&lists.hits.n, 1);
+                if (at < kHits) { lists.hits.item[at] = item; lists.hits.entry[at] = entry; }
+            };
+            for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) note(w.hist[k], 0);
+            for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) note(w.bias_item[k], (int)k + 1);
+            __syncthreads();
+            const int n = lists.hits.n;
+            many = n > kHits;
+            constexpr int ve = Vec<T>::n;
+            for (int h = 0; h < n && !many; ++h) {
+                const int item = lists.hits.item[h], vec = (item - first) / ve;
+                if (vec % kThreads != (int)threadIdx.x || item >= n_items) continue;
+                const int slot = vec / kThreads * ve + (item - first) % ve;
+                if ((done >> slot) & 1u) continue;
+                int c = 0, l = 0;
+                for (int k = h; k < n; ++k)
+                    if (lists.hits.item[k] == item) {
+                        c += lists.hits.entry[k] == 0;
+                        l = max(l, lists.hits.entry[k]);
+                    }
+                const float x = listed_score(u, w, item, c, l, pick<P>(*reinterpret_cast<const float (*)[P]>(s), slot));
+#pragma unroll
+                for (int k = 0; k < P; ++k) s[k] = k == slot ? x : s[k];
+                done |= 1u << slot;
+            }
+        }
+        if (!many) apply_rules<T, P, false>(u, w, first, n_items, nullptr, nullptr, s, done);
+        else {
+            constexpr int per = kCounted / kThreads;             // (tiles of P scores per thread lie in tiles of `per`: vectors of a tile come in order)
+#pragma unroll
+            for (int q = 0; q < P / per; ++q) {
+                __syncthreads();
+                const int from = first + q * kCounted;
+                if (scan_lists<per>(w, from, lists.counted.count, lists.counted.last))
+                    apply_rules<T, per, true>(u, w, from, n_items, lists.counted.count, lists.counted.last, s + q * per);
+                else apply_rules<T, per, false>(u, w, from, n_items, nullptr, nullptr, s + q * per);
+            }
+        }
     }
     constexpr int ve = Vec<T>::n;
     T *o = out + r * out_stride;
 #pragma unroll
-    for (int j = 0; j < kPer / ve; ++j) {
+    for (int j = 0; j < P / ve; ++j) {
         const int i = first + (j * kThreads + (int)threadIdx.x) * ve;
         if (i + ve <= n_items) store_vec(o + i, s + j * ve);
         else {
@@ -198,181 +285,289 @@ __device__ __forceinline__ float key_score(u64 key) {
 }
 __device__ __forceinline__ int key_item(u64 key) { return (int)~(unsigned)key; }
 
-constexpr int kBuf = 2 * kTile;                  // candidates a workgroup holds: a tile's worth on top of what is kept
-constexpr int kRound = 1024;                     // most entries kept at a time; a longer list is taken in rounds of this many
-constexpr int kSuper = 4;                        // tiles whose scores are in registers at once
+constexpr int kWaves = kThreads / 64;
+constexpr int kPer = 8, kTile = kPer * kThreads; // scores per thread of a tile
+// Under rules, half as many tiles are in registers at once (their biases and masks are too) and half as many candidates in LDS (it holds what the
+// lists name as well): four workgroups per CU either way.
+template <bool RULED> struct Top {
+    static constexpr int super = RULED ? 2 : 4;  // tiles whose scores are in registers at once
+    static constexpr int buf = RULED ? 512 : 1024;               // candidates a wavefront holds
+    static constexpr int round = buf / 2;        // most entries kept at a time; a longer list is taken in rounds of this many
+};
+constexpr int kSlots = 1024, kShort = 512;       // hash slots for the items that a row's lists name; lists of more entries than kShort are scanned per tile
+constexpr int kWindow = 65536;                   // items whose membership bits are in LDS at a time
 
-// descending bitonic sort of buf[0 .. p2), p2 a power of two
-__device__ __forceinline__ void sort_keys(u64 *buf, int p2) {
+// descending bitonic sort of buf[0 .. p2) by `threads` threads, p2 a power of two.  The 64 pairs of a wavefront lie in 128 keys as long as the
+// distance is at most 64: such steps follow each other without a barrier (a wavefront's LDS operations run in order).
+template <bool BLOCK>
+__device__ __forceinline__ void sort_keys(u64 *buf, int p2, int thread) {
+    constexpr int threads = BLOCK ? kThreads : 64;
     for (int k = 2; k <= p2; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int t = threadIdx.x; t < p2 / 2; t += kThreads) {
-                const int i = (t / j) * 2 * j + t % j, l = i + j;
+            if (BLOCK && (j > 64 || (j == 64 && k > 128) || k == 2)) __syncthreads();
+            for (int t = thread; t < p2 / 2; t += threads) {
+                const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1)), l = i + j;
                 const u64 a = buf[i], b = buf[l];
                 if ((a < b) == ((i & k) == 0)) { buf[i] = b; buf[l] = a; }
             }
-            __syncthreads();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
+    if (BLOCK) __syncthreads();
 }
 
-// keeps the best `keep` of the m candidates, sorted; returns how many there are now.  m <= kBuf.
-__device__ __forceinline__ int compact(u64 *buf, int m, int keep) {
-    int p2 = 2;
-    while (p2 < m) p2 <<= 1;
-    for (int k = m + threadIdx.x; k < p2; k += kThreads) buf[k] = 0;
+// what a row's lists name, when they are short: a hash table of the items with their counts and last bias entries, and a bit per item of a window
+struct Listed {
+    int id[kSlots], count[kSlots], last[kSlots];
+    unsigned bits[kWindow / 32];
+};
+struct Tiled {
+    int count[kTile], last[kTile];               // (one tile at a time)
+};
+union ListMemory {
+    Listed listed;
+    Tiled tiled;
+};
+
+__device__ __forceinline__ void hash_lists(const RowRules &w, int n_items, Listed &m) {
+    for (int k = threadIdx.x; k < kSlots; k += kThreads) { m.id[k] = -1; m.count[k] = 0; m.last[k] = 0; }
     __syncthreads();
-    sort_keys(buf, p2);
-    return m < keep ? m : keep;
+    auto slot_of = [&](int item) {                               // (at most kShort of kSlots are taken: the walk ends)
+        unsigned at = (unsigned)item * 2654435761u >> 22;
+        for (;;) {
+            const int was = atomicCAS(m.id + at, -1, item);
+            if (was == -1 || was == item) return at;
+            at = (at + 1) & (kSlots - 1);
+        }
+    };
+    for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) {
+        const int i = w.hist[k];
+        if (i >= 0 && i < n_items) atomicAdd(m.count + slot_of(i), 1);
+    }
+    for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) {
+        const int i = w.bias_item[k];
+        if (i >= 0 && i < n_items) atomicMax(m.last + slot_of(i), (int)k + 1);
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void window_bits(Listed &m, int first) {
+    __syncthreads();                                             // (nobody reads the last window's any more)
+    for (int k = threadIdx.x; k < kWindow / 32; k += kThreads) m.bits[k] = 0;
+    __syncthreads();
+    for (int k = threadIdx.x; k < kSlots; k += kThreads) {
+        const int i = m.id[k];
+        if (i >= first && i - first < kWindow) atomicOr(m.bits + ((i - first) >> 5), 1u << (i & 31));
+    }
+    __syncthreads();
 }
 
-// One workgroup per (row, segment of the row): ONE pass over the scores.  Candidates above the running threshold go to LDS; when they no
-// longer fit, they are sorted and the threshold becomes the n-th best.  The first threshold comes from the first 8192 scores: each of the
-// 1024 groups of eight holds its maximum in a register, a wavefront finds by bisection over ballots the value that ceil(n / 4) of its group
-// maxima reach, and the least of the four wavefronts' values is reached by at least n scores.  So the sort sees a few times n keys, not the
-// row.  FROM_KEYS: the "scores" are the sorted keys that the segments of a row left behind.
+// One workgroup per (row, segment of the row): ONE pass over the scores.  Scores at or above the running threshold become keys in the wavefront's
+// own part of LDS -- no barrier in the loop; when it is full, it is sorted and the threshold becomes the n-th best.  The first threshold comes
+// from the first 8192 scores (4096 under rules): each group of eight holds its maximum in a register, a wavefront finds by bisection over ballots the
+// value that ceil(n / 4) of its group maxima reach, and the least of the four wavefronts' values is reached by at least n scores.  So the final
+// sort sees a few times n keys, not the row.  Under rules, items that the row's lists name are left out of the pass (a bit per item in LDS) and
+// looked at by themselves afterwards.  FROM_KEYS: the "scores" are the sorted keys that the segments of a row left behind.
 template <typename T, bool RULED, bool FROM_KEYS>
-__global__ void __launch_bounds__(kThreads) top_scores_kernel(const rfm_score_rules u, long long row0, int segments, int segment, int n_items,
+__global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score_rules u, long long row0, int segments, int segment, int n_items,
                                                               const T *__restrict__ scores, long long stride, const u64 *__restrict__ keys_in, int n_keys,
                                                               int n, u64 *__restrict__ keys_out, int32_t *__restrict__ items, float *__restrict__ values) {
-    __shared__ u64 buf[kBuf];
-    __shared__ int count[RULED ? kTile : 1], last[RULED ? kTile : 1];
-    __shared__ int appended[3];
-    __shared__ unsigned wave_t[4];
+    constexpr int kSuper = Top<RULED>::super, kBuf = Top<RULED>::buf, kRound = Top<RULED>::round;
+    constexpr int kAll = kSuper * kPer, ve = FROM_KEYS ? 1 : Vec<T>::n;
+    __shared__ u64 buf[kWaves * kBuf];
+    __shared__ typename std::conditional<RULED, ListMemory, int>::type lists_memory;
+    __shared__ unsigned wave_t[kWaves];
+    __shared__ int wave_m[kWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long r = row0 + blockIdx.x / segments;
     const int seg = (int)(blockIdx.x % segments);
     const int begin = FROM_KEYS ? 0 : seg * segment, end = FROM_KEYS ? n_keys : min(n_items - begin, segment) + begin;
     RowRules w;
     if constexpr (RULED) w = row_rules(u, r, n_items);
-    const bool lists = RULED && (w.hist_n > 0 || w.bias_n > 0);
+    const bool listed = RULED && (w.hist_n > 0 || w.bias_n > 0), hashed = listed && w.hist_n + w.bias_n <= kShort;
     const T *row = FROM_KEYS ? nullptr : scores + r * stride;
     const u64 *krow = FROM_KEYS ? keys_in + (size_t)(r - row0) * n_keys : nullptr;
+    u64 *mine = buf + wave * kBuf;
+    if constexpr (RULED)
+        if (hashed) hash_lists(w, n_items, lists_memory.listed);
     u64 ceiling = ~0ull;                                         // keys of earlier rounds are at or above it
     for (int base = 0; base < n; base += kRound) {
         const int want = min(n - base, kRound);
-        u64 thr = 0;                                             // a key passes when it is above
-        int m = 0, step = 0;
-        if (threadIdx.x < 3) appended[threadIdx.x] = 0;
-        __syncthreads();
+        u64 thr = 0;                                             // a key passes when it is above; a score is looked at when it is `reach` or more
+        float reach = -3.402823466e38f;
+        int m = 0;
+        auto keep = [&](bool pass, u64 key) {                    // (by whole wavefronts)
+            pass = pass && key > thr && key < ceiling;
+            const unsigned long long who = __ballot(pass);
+            if (!who) return;
+            if (m > kBuf - 64) {
+                int p2 = 2;
+                while (p2 < m) p2 <<= 1;
+                for (int k = m + lane; k < p2; k += 64) mine[k] = 0;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                sort_keys<false>(mine, p2, lane);
+                m = want;                                        // (m > kBuf - 64 >= want)
+                thr = max(thr, mine[want - 1]);
+                reach = key_score(thr);
+                pass = pass && key > thr;
+            }
+            const unsigned long long still = __ballot(pass);
+            if (pass) mine[m + __popcll(still & ((1ull << lane) - 1))] = key;
+            m += __popcll(still);
+        };
+        int window = -1;
         for (int t0 = begin; t0 < end && !(RULED && w.bad); t0 += kSuper * kTile) {
-            u64 key[kSuper * kPer];
+            float x[kAll];
+            if constexpr (FROM_KEYS) {
 #pragma unroll
-            for (int q = 0; q < kSuper; ++q) {
-                const int first = t0 + q * kTile;
-                if constexpr (FROM_KEYS) {
+                for (int k = 0; k < kAll; ++k) {
+                    const int e = t0 + k * kThreads + (int)threadIdx.x;
+                    const u64 key = e < end ? krow[e] : 0;
+                    x[k] = key && key < ceiling ? key_score(key) : -INFINITY;
+                }
+            } else {
 #pragma unroll
-                    for (int k = 0; k < kPer; ++k) {
-                        const int e = first + k * kThreads + (int)threadIdx.x;
-                        const u64 x = e < end ? krow[e] : 0;
-                        key[q * kPer + k] = x < ceiling ? x : 0;
-                    }
-                } else {
-                    float s[kPer];
+                for (int q = 0; q < kSuper; ++q) load_tile<T, kPer>(row, t0 + q * kTile, end, x + q * kPer);
+                if constexpr (RULED) {
+                    if (!listed || hashed) {
 #pragma unroll
-                    for (int k = 0; k < kPer; ++k) s[k] = -INFINITY;
-                    if (first < end) {
-                        load_tile(row, first, end, s);
-                        if constexpr (RULED) {
-                            if (lists) {
-                                scan_lists(w, first, count, last);
-                                apply_rules<T, true>(u, w, first, n_items, count, last, s);
-                                __syncthreads();                 // (the next tile's scan clears the counts)
-                            } else apply_rules<T, false>(u, w, first, n_items, count, last, s);
+                        for (int q = 0; q < kSuper; ++q) apply_rules<T, kPer, false>(u, w, t0 + q * kTile, n_items, nullptr, nullptr, x + q * kPer);
+                        if (hashed) {
+                            if (t0 / kWindow != window) { window = t0 / kWindow; window_bits(lists_memory.listed, window * kWindow); }
+#pragma unroll
+                            for (int j = 0; j < kAll / ve; ++j) {
+                                const int at = t0 - window * kWindow + (j * kThreads + (int)threadIdx.x) * ve;       // (ve divides 32: one word)
+                                const unsigned bits = lists_memory.listed.bits[at >> 5] >> (at & 31);
+#pragma unroll
+                                for (int k = 0; k < ve; ++k) x[j * ve + k] = (bits >> k) & 1u ? -INFINITY : x[j * ve + k];
+                            }
                         }
-                    }
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < kPer; ++k) {
-                        const int i = first + element<T>(k);
-                        const unsigned v = i < end ? score_key(s[k]) : 0u;
-                        const u64 x = v ? ((u64)v << 32) | (unsigned)~i : 0;
-                        key[q * kPer + k] = x < ceiling ? x : 0;
+                        for (int q = 0; q < kSuper; ++q) {
+                            if (t0 + q * kTile >= end) break;    // (the same for all)
+                            if (scan_lists<kPer>(w, t0 + q * kTile, lists_memory.tiled.count, lists_memory.tiled.last))
+                                apply_rules<T, kPer, true>(u, w, t0 + q * kTile, n_items, lists_memory.tiled.count, lists_memory.tiled.last, x + q * kPer);
+                            else apply_rules<T, kPer, false>(u, w, t0 + q * kTile, n_items, nullptr, nullptr, x + q * kPer);
+                            __syncthreads();                     // (the next tile's scan clears the counts)
+                        }
                     }
                 }
             }
-            if (t0 == begin) {                                   // the first threshold
+            auto key_of = [&](int k, float value) {
+                if constexpr (FROM_KEYS) {
+                    const int e = t0 + k * kThreads + (int)threadIdx.x;
+                    return e < end ? krow[e] : 0ull;
+                } else {
+                    const int i = t0 + (k / kPer) * kTile + element<T>(k % kPer);
+                    const unsigned v = i < end ? score_key(value) : 0u;
+                    return v ? ((u64)v << 32) | (unsigned)~i : 0ull;
+                }
+            };
+            if (t0 == begin && base == 0) {                      // the first threshold (later rounds: what earlier ones took is among these)
                 unsigned g[kSuper];
 #pragma unroll
                 for (int q = 0; q < kSuper; ++q) {
-                    g[q] = 0;
+                    float high = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < kPer; ++k) g[q] = max(g[q], (unsigned)(key[q * kPer + k] >> 32));
+                    for (int k = 0; k < kPer; ++k) high = fmaxf(high, x[q * kPer + k]);
+                    g[q] = score_key(high);
                 }
-                const int need = (want + 3) / 4;
-                if (need <= 32) { g[0] = max(max(g[0], g[1]), max(g[2], g[3])); g[1] = g[2] = g[3] = 0; }
-                unsigned t = 0;
-                for (int bit = 31; bit >= 0; --bit) {
-                    const unsigned c = t | (1u << bit);
-                    int reach = 0;
+                const int need = (want + kWaves - 1) / kWaves;
+                if (need <= 32) {                                // few are wanted: one group per lane
 #pragma unroll
-                    for (int q = 0; q < kSuper; ++q) reach += __popcll(__ballot(g[q] >= c));
-                    if (reach >= need) t = c;
+                    for (int q = 1; q < kSuper; ++q) { g[0] = max(g[0], g[q]); g[q] = 0; }
+                }
+                unsigned t = 0;
+                for (int bit = 31; bit >= 12; --bit) {             // (cut to 20 bits: a little below the exact value)
+                    const unsigned c = t | (1u << bit);
+                    int found = 0;
+#pragma unroll
+                    for (int q = 0; q < kSuper; ++q) found += __popcll(__ballot(g[q] >= c));
+                    if (found >= need) t = c;
                 }
                 if (lane == 0) wave_t[wave] = t;
                 __syncthreads();
                 t = min(min(wave_t[0], wave_t[1]), min(wave_t[2], wave_t[3]));
-                thr = t ? ((u64)t << 32) - 1 : 0;
+                if (t) { thr = ((u64)t << 32) - 1; reach = key_score((u64)t << 32); }
             }
+            // a bit per score that reaches the threshold (bit 31 - k for slot k); then one score of every lane at a time, picked out of the registers
+            unsigned reached = 0;
 #pragma unroll
-            for (int q = 0; q < kSuper; ++q) {                   // at most kTile of them pass, and there is room for that many
-                if (t0 + q * kTile >= end) break;                // (the same for all)
-                const int slot = step % 3;
-                if (threadIdx.x == 0) appended[(step + 1) % 3] = 0;
-                int mine = 0;
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) mine += key[q * kPer + k] > thr;
-                int before = mine;                               // inclusive prefix over the wavefront
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const int o = __shfl_up(before, d);
-                    if (lane >= d) before += o;
-                }
-                const int total = __shfl(before, 63);
-                if (total > 0) {
-                    int at = 0;
-                    if (lane == 63) at = atomicAdd(appended + slot, total);
-                    at = m + __shfl(at, 63) + before - mine;
-#pragma unroll
-                    for (int k = 0; k < kPer; ++k)
-                        if (key[q * kPer + k] > thr) buf[at++] = key[q * kPer + k];
-                }
-                __syncthreads();
-                m += appended[slot];
-                ++step;
-                if (m > kBuf - kTile) {
-                    m = compact(buf, m, want);
-                    if (m == want) thr = buf[want - 1];
-                    __syncthreads();
+            for (int k = 0; k < kAll; ++k) reached = reached + reached + (x[k] >= reach ? 1u : 0u);
+            reached <<= 32 - kAll;
+            while (__any(reached != 0)) {
+                const int k = __clz((int)reached) & (kAll - 1);
+                const bool pass = reached != 0;
+                reached &= ~(0x80000000u >> k);
+                keep(pass, key_of(k, pick(x, k)));
+            }
+        }
+        if constexpr (RULED) {
+            if (hashed && !w.bad) {                              // the items left out
+                const Listed &l = lists_memory.listed;
+#pragma unroll 1
+                for (int k = 0; k < kSlots / kThreads; ++k) {
+                    const int at = k * kThreads + (int)threadIdx.x, i = l.id[at];
+                    const bool here = i >= begin && i < end;
+                    float s = -INFINITY;
+                    if (here && (!w.mask || ((w.mask[i >> 5] >> (i & 31)) & 1u))) {
+                        s = (float)row[i];
+                        s = listed_score(u, w, i, l.count[at], l.last[at], s);
+                    }
+                    const unsigned v = score_key(s);
+                    keep(v != 0, ((u64)v << 32) | (unsigned)~i);
                 }
             }
         }
+        // the wavefronts' candidates side by side, sorted
+        if (lane == 0) wave_m[wave] = m;
         __syncthreads();
-        m = compact(buf, m, want);
+        int total = 0, at = 0;
+        for (int k = 0; k < kWaves; ++k) {
+            at = k == wave ? total : at;
+            total += wave_m[k];
+        }
+        {
+            u64 held[kBuf / 64];
+#pragma unroll
+            for (int k = 0; k < kBuf / 64; ++k)
+                if (k * 64 < m) held[k] = mine[k * 64 + lane];   // (what is read behind m is not written)
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kBuf / 64; ++k)
+                if (k * 64 + lane < m) buf[at + k * 64 + lane] = held[k];
+        }
+        int p2 = 2;
+        while (p2 < total) p2 <<= 1;
+        for (int k = total + threadIdx.x; k < p2; k += kThreads) buf[k] = 0;
+        sort_keys<true>(buf, p2, threadIdx.x);
+        const int got = total < want ? total : want;
         const size_t row_out = FROM_KEYS || segments == 1 ? (size_t)r * n : ((size_t)(r - row0) * segments + seg) * n;
         for (int k = threadIdx.x; k < want; k += kThreads) {
-            const u64 x = k < m ? buf[k] : 0;
-            if (!FROM_KEYS && segments > 1) keys_out[row_out + base + k] = x;
+            const u64 key = k < got ? buf[k] : 0;
+            if (!FROM_KEYS && segments > 1) keys_out[row_out + base + k] = key;
             else {
-                items[row_out + base + k] = x ? key_item(x) : -1;
-                values[row_out + base + k] = x ? key_score(x) : -INFINITY;
+                items[row_out + base + k] = key ? key_item(key) : -1;
+                values[row_out + base + k] = key ? key_score(key) : -INFINITY;
             }
         }
-        ceiling = m == want ? buf[want - 1] : 0;                 // 0: nothing is left for further rounds
+        ceiling = got == want ? buf[want - 1] : 0;               // 0: nothing is left for further rounds
         __syncthreads();
     }
 }
 
-// how many segments a row is cut into: with few rows, enough to give every CU work, of at least one 8192-score block each.  A list longer
-// than one round is not cut.
-static int top_segments(long long n_rows, int n_items, int n) {
-    constexpr int block = kSuper * kTile;
-    if (n > kRound || n_rows >= 512) return 1;
-    const long long blocks = ((long long)n_items + block - 1) / block;
+// how many segments a row is cut into: with few rows, enough to give every CU work, of at least one block of 8192 scores each.  A list longer than
+// one round is not cut.
+constexpr int kBlock = 8192;
+static int top_segments(long long n_rows, int n_items, int n, bool ruled) {
+    if (n > (ruled ? Top<true>::round : Top<false>::round) || n_rows >= 512) return 1;
+    const long long blocks = ((long long)n_items + kBlock - 1) / kBlock;
     return (int)std::max<long long>(1, std::min<long long>(blocks, (512 + n_rows - 1) / n_rows));
 }
 static int top_segment(int n_items, int segments) {
-    constexpr int block = kSuper * kTile;
-    const long long blocks = ((long long)n_items + block - 1) / block;
-    return (int)std::min<long long>(n_items, (blocks + segments - 1) / segments * block);
+    const long long blocks = ((long long)n_items + kBlock - 1) / kBlock;
+    return (int)std::min<long long>(n_items, (blocks + segments - 1) / segments * kBlock);
 }
 
 // a launch holds fewer than 2^32 threads per dimension
@@ -394,17 +589,18 @@ static int check_rules(const rfm_score_rules *u, int64_t n_rows) {
 
 template <typename T>
 static void launch_adjust(const rfm_score_rules &u, long long n_rows, int n_items, const void *in, long long in_stride, void *out, long long out_stride, hipStream_t stream) {
-    const int tiles = (n_items + kTile - 1) / kTile;
+    constexpr int per = sizeof(T) == 4 ? 8 : 16; // 32 bytes of a row per thread either way
+    const int tiles = (n_items + per * kThreads - 1) / (per * kThreads);
     const long long step = std::max<long long>(1, kMaxBlocks / tiles);
     for (long long r = 0; r < n_rows; r += step)
-        adjust_scores_kernel<T><<<dim3((unsigned)(std::min(step, n_rows - r) * tiles)), dim3(kThreads), 0, stream>>>(u, r, tiles, n_items, (const T *)in, in_stride,
+        adjust_scores_kernel<T, per><<<dim3((unsigned)(std::min(step, n_rows - r) * tiles)), dim3(kThreads), 0, stream>>>(u, r, tiles, n_items, (const T *)in, in_stride,
                                                                                                                       (T *)out, out_stride);
 }
 
 template <typename T, bool RULED>
 static void launch_top(const rfm_score_rules &u, long long n_rows, int n_items, const void *in, long long stride, int n, int32_t *items, float *values, u64 *keys,
                        hipStream_t stream) {
-    int segments = top_segments(n_rows, n_items, n);
+    int segments = top_segments(n_rows, n_items, n, RULED);
     const int segment = top_segment(n_items, segments);
     segments = (n_items + segment - 1) / segment;
     const long long step = std::max<long long>(1, kMaxBlocks / segments);
@@ -440,7 +636,7 @@ int rfm_adjust_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_
 
 size_t rfm_top_scores_workspace_bytes(int64_t n_rows, int32_t n_items, int32_t n) {
     if (n_rows < 0 || n_items < 1 || n < 1 || n > n_items) return 0;
-    const int segments = top_segments(n_rows, n_items, n);
+    const int segments = top_segments(n_rows, n_items, n, false);         // (without rules rows are cut no less than with them)
     return segments > 1 ? sizeof(u64) * (size_t)n_rows * (size_t)segments * (size_t)n : 8;
 }
 
