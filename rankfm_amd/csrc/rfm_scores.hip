@@ -377,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
     __shared__ typename std::conditional<RULED, ListMemory, int>::type lists_memory;
     __shared__ unsigned wave_t[kWaves];
     __shared__ int wave_m[kWaves];
+    __shared__ u64 last_key;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long r = row0 + blockIdx.x / segments;
     const int seg = (int)(blockIdx.x % segments);
@@ -464,13 +465,14 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
                     return v ? ((u64)v << 32) | (unsigned)~i : 0ull;
                 }
             };
-            if (t0 == begin && base == 0) {                      // the first threshold (later rounds: what earlier ones took is among these)
+            if (t0 == begin) {                                   // the first threshold (in later rounds, of the scores below what was taken)
+                const float taken = base == 0 ? INFINITY : key_score(ceiling);
                 unsigned g[kSuper];
 #pragma unroll
                 for (int q = 0; q < kSuper; ++q) {
                     float high = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < kPer; ++k) high = fmaxf(high, x[q * kPer + k]);
+                    for (int k = 0; k < kPer; ++k) high = fmaxf(high, base == 0 || x[q * kPer + k] < taken ? x[q * kPer + k] : -INFINITY);
                     g[q] = score_key(high);
                 }
                 const int need = (want + kWaves - 1) / kWaves;
@@ -520,15 +522,42 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
                 }
             }
         }
-        // the wavefronts' candidates side by side, sorted
+        // The candidates in order: put side by side and sorted.  Where rows are few and one workgroup's way to the end is what counts, up to 256 of them
+        // are placed by counting instead -- a key's place is the number of larger ones (keys are unique): no barriers, but the square of the work
+        // (one row of 200 k: 23.5 -> 17.6 us; at 4096 rows of 50 k it would be 196 -> 309).
         if (lane == 0) wave_m[wave] = m;
+        if (threadIdx.x == 0) last_key = 0;
         __syncthreads();
         int total = 0, at = 0;
+#pragma unroll
         for (int k = 0; k < kWaves; ++k) {
             at = k == wave ? total : at;
             total += wave_m[k];
         }
-        {
+        const int got = total < want ? total : want;
+        const size_t row_out = FROM_KEYS || segments == 1 ? (size_t)r * n : ((size_t)(r - row0) * segments + seg) * n;
+        auto put = [&](int place, u64 key) {
+            if (!FROM_KEYS && segments > 1) keys_out[row_out + base + place] = key;
+            else {
+                items[row_out + base + place] = key ? key_item(key) : -1;
+                values[row_out + base + place] = key ? key_score(key) : -INFINITY;
+            }
+        };
+        if ((FROM_KEYS || segments > 1) && total <= 256) {
+            for (int k = lane; k < m; k += 64) {
+                const u64 key = mine[k];
+                int place = 0;
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v) {
+                    const u64 *other = buf + v * kBuf;
+                    const int count = wave_m[v];
+#pragma unroll 4
+                    for (int q = 0; q < count; ++q) place += other[q] > key;
+                }
+                if (place < want) put(place, key);
+                if (place == want - 1) last_key = key;
+            }
+        } else {
             u64 held[kBuf / 64];
 #pragma unroll
             for (int k = 0; k < kBuf / 64; ++k)
@@ -537,31 +566,25 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
 #pragma unroll
             for (int k = 0; k < kBuf / 64; ++k)
                 if (k * 64 + lane < m) buf[at + k * 64 + lane] = held[k];
+            int p2 = 2;
+            while (p2 < total) p2 <<= 1;
+            for (int k = total + threadIdx.x; k < p2; k += kThreads) buf[k] = 0;
+            sort_keys<true>(buf, p2, threadIdx.x);
+            for (int k = threadIdx.x; k < got; k += kThreads) put(k, buf[k]);
+            if (threadIdx.x == 0 && got == want) last_key = buf[want - 1];
         }
-        int p2 = 2;
-        while (p2 < total) p2 <<= 1;
-        for (int k = total + threadIdx.x; k < p2; k += kThreads) buf[k] = 0;
-        sort_keys<true>(buf, p2, threadIdx.x);
-        const int got = total < want ? total : want;
-        const size_t row_out = FROM_KEYS || segments == 1 ? (size_t)r * n : ((size_t)(r - row0) * segments + seg) * n;
-        for (int k = threadIdx.x; k < want; k += kThreads) {
-            const u64 key = k < got ? buf[k] : 0;
-            if (!FROM_KEYS && segments > 1) keys_out[row_out + base + k] = key;
-            else {
-                items[row_out + base + k] = key ? key_item(key) : -1;
-                values[row_out + base + k] = key ? key_score(key) : -INFINITY;
-            }
-        }
-        ceiling = got == want ? buf[want - 1] : 0;               // 0: nothing is left for further rounds
+        for (int k = got + threadIdx.x; k < want; k += kThreads) put(k, 0);
+        __syncthreads();
+        ceiling = last_key;                                      // 0: nothing is left for further rounds
         __syncthreads();
     }
 }
 
-// how many segments a row is cut into: with few rows, enough to give every CU work, of at least one block of 8192 scores each.  A list longer than
-// one round is not cut.
+// how many segments a row is cut into: with few rows, enough to give every CU work, of at least one block of 8192 scores each.  Lists of more than 1024
+// are not cut: every segment would hand that many on.
 constexpr int kBlock = 8192;
-static int top_segments(long long n_rows, int n_items, int n, bool ruled) {
-    if (n > (ruled ? Top<true>::round : Top<false>::round) || n_rows >= 512) return 1;
+static int top_segments(long long n_rows, int n_items, int n) {
+    if (n > 1024 || n_rows >= 512) return 1;
     const long long blocks = ((long long)n_items + kBlock - 1) / kBlock;
     return (int)std::max<long long>(1, std::min<long long>(blocks, (512 + n_rows - 1) / n_rows));
 }
@@ -600,7 +623,7 @@ static void launch_adjust(const rfm_score_rules &u, long long n_rows, int n_item
 template <typename T, bool RULED>
 static void launch_top(const rfm_score_rules &u, long long n_rows, int n_items, const void *in, long long stride, int n, int32_t *items, float *values, u64 *keys,
                        hipStream_t stream) {
-    int segments = top_segments(n_rows, n_items, n, RULED);
+    int segments = top_segments(n_rows, n_items, n);
     const int segment = top_segment(n_items, segments);
     segments = (n_items + segment - 1) / segment;
     const long long step = std::max<long long>(1, kMaxBlocks / segments);
@@ -636,7 +659,7 @@ int rfm_adjust_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_
 
 size_t rfm_top_scores_workspace_bytes(int64_t n_rows, int32_t n_items, int32_t n) {
     if (n_rows < 0 || n_items < 1 || n < 1 || n > n_items) return 0;
-    const int segments = top_segments(n_rows, n_items, n, false);         // (without rules rows are cut no less than with them)
+    const int segments = top_segments(n_rows, n_items, n);
     return segments > 1 ? sizeof(u64) * (size_t)n_rows * (size_t)segments * (size_t)n : 8;
 }
 
@@ -654,9 +677,10 @@ int rfm_top_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_t n
     u64 *keys = (u64 *)workspace;
     const rfm_score_rules none = {};
     const rfm_score_rules &u = rules ? *rules : none;
+    const bool ruled = u.history_offsets || u.item_bias || u.bias_offsets || u.allowed;
     auto go = [&](auto type) {
         using T = decltype(type);
-        if (rules) launch_top<T, true>(u, n_rows, n_items, scores, stride, n, items, values, keys, stream);
+        if (ruled) launch_top<T, true>(u, n_rows, n_items, scores, stride, n, items, values, keys, stream);
         else launch_top<T, false>(u, n_rows, n_items, scores, stride, n, items, values, keys, stream);
     };
     if (dtype == RFM_F32) go(float(0));

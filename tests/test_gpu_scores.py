@@ -206,7 +206,7 @@ def plain_top(s, n):
 
 @pytest.mark.parametrize("rows, items, n", [(1, 1, 1), (3, 2, 2), (2, 33, 5), (5, 2047, 10), (4, 2048, 2048), (3, 2049, 64), (2, 8192, 256), (2, 8193, 257),
                                             (3, 9000, 129), (2, 20_001, 1024), (2, 20_001, 1025), (1, 5000, 5000), (1, 200_000, 100), (7, 50_001, 10),
-                                            (600, 3001, 33), (40, 30_000, 500)])
+                                            (600, 3001, 33), (40, 30_000, 500), (2, 48_034, 390), (1, 120_000, 1024), (3, 700, 700)])
 @pytest.mark.parametrize("kind", ["normal", "ties", "ascending", "constant", "gaps"])
 def test_top_scores(rows, items, n, kind):
     rng = np.random.default_rng(items + n)
@@ -242,7 +242,7 @@ def test_top_scores_of_half_width_rows(dtype):
 def test_top_scores_under_rules_are_those_of_the_adjusted_rows(shape, dtype):
     p = Problem(dtype=dtype, seed=shape["items"] + 1, **shape)
     adjusted = p.plain(np.float32)[0]
-    for n in {1, min(10, p.items), min(700, p.items)}:
+    for n in {1, min(10, p.items), min(300, p.items), min(700, p.items)}:
         got = top_scores(p.s.cuda(), n, p.rules())
         want_items, want_values = plain_top(adjusted, n)
         assert np.array_equal(got.items.cpu().numpy(), want_items) and np.array_equal(got.scores.cpu().numpy(), want_values)
