@@ -5,11 +5,14 @@ call site expects.  Long jobs, the benchmark and the multi-GPU trainer instead k
 torch tensors (PyTorch is used for device memory and streams only) and call `rfm_fit_device` on raw pointers.
 """
 import ctypes as C
+from dataclasses import replace
 
 import numpy as np
 import torch
 
 from . import _hip
+from .distill import distill_gradients
+from .scores import ScoreRules, TopScores, adjust_scores, top_scores
 
 WEIGHT_NAMES = ("w_i", "w_if", "v_u", "v_i", "v_uf", "v_if")
 
@@ -225,9 +228,114 @@ class DeviceSession:
         _hip.raise_for_status(rc)
         return scores.cpu().numpy() if to_host else scores
 
-    def recommend(self, users, n_items=10, filter_previous=False, to_host=True):
+    # ---- answers under rules, and with their scores (rankfm_amd/scores.py) ---------------------------------------------------------------
+    SCORE_BYTES = 1 << 30                 # score rows held at a time
+
+    def _known(self, users):
+        """float32 user indexes on the device, NaN for those that are not the model's"""
+        u = self._to_device(users, 1, "users")
+        return torch.where((u >= 0) & (u < self.n_users), u, float("nan"))
+
+    def scores(self, users):
+        """float32 [n] user indexes (NaN = unknown) -> float32 [n, items] score rows on the device, NaN rows for unknown users"""
+        users_d = self._known(users)
+        out = torch.empty((users_d.shape[0], self.n_items), dtype=torch.float32, device=self.device)
+        if users_d.shape[0] == 0:
+            return out
+        mv = self._model_view()
+        with torch.cuda.device(self.device):
+            ws = torch.empty(int(_hip.lib().rfm_scores_workspace_bytes(C.byref(mv), users_d.shape[0])), dtype=torch.uint8, device=self.device)
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            rc = _hip.lib().rfm_scores_device(C.byref(mv), users_d.shape[0], C.c_void_p(users_d.data_ptr()), C.c_void_p(out.data_ptr()),
+                                              C.c_void_p(ws.data_ptr()), ws.numel(), C.c_void_p(stream))
+        _hip.raise_for_status(rc)
+        return out
+
+    def top_scores(self, users, n_items=10, rules=None, filter_previous=False):
+        """`TopScores` (int32 items, float32 scores, [n, n_items], on the device) of the users' best items under `rules` (a ScoreRules whose
+        rows are the users of this call): what a teacher hands to `distill`.  Penalties without a history of their own count the session's own
+        CSR lists; `filter_previous` leaves those lists out.  Unknown users and exhausted rows end in (-1, -inf)."""
+        users_d = self._known(users)
+        n, n_items = int(users_d.shape[0]), int(n_items)
+        if n_items < 1 or n_items > self.n_items:
+            raise ValueError("[n_items] must be between 1 and the number of training items")
+        rows_d = torch.where(torch.isnan(users_d), -1.0, users_d).to(torch.int32)
+        if rules is not None and rules.penalises() and rules.history is None:
+            rules = replace(rules, history=(self.csr_offsets, self.csr_items), history_rows=rows_d)
+        gone = None
+        if filter_previous:
+            gone = ScoreRules(history=(self.csr_offsets, self.csr_items), history_rows=rows_d,
+                              presence=torch.full((n,), float("inf"), dtype=torch.float32, device=self.device))
+        items = torch.empty((n, n_items), dtype=torch.int32, device=self.device)
+        values = torch.empty((n, n_items), dtype=torch.float32, device=self.device)
+        step = max(1, self.SCORE_BYTES // (4 * self.n_items))
+        for a in range(0, n, step):
+            b = min(a + step, n)
+            rows = self.scores(users_d[a:b])
+            if gone is not None:
+                adjust_scores(rows, gone.rows(a, b), out=rows)
+            best = top_scores(rows, n_items, None if rules is None else rules.rows(a, b))
+            items[a:b], values[a:b] = best.items, best.scores
+        return TopScores(items, values)
+
+    def distill(self, users, teacher_items, teacher_scores, *, temperature=1.0, allowed=None, allowed_rows=None, row_weight=None,
+                learning_rate=None):
+        """one step of learning from another model's top scores (rankfm_amd/distill.py): the loss of each user and the gradients of
+        sum(row_weight * loss) with respect to the model's weights -- {'w_i', 'v_u', 'v_i'} and, where the model has features, 'w_if', 'v_uf',
+        'v_if'; 'v_u' has one row per user of the call.  With `learning_rate` the weights are moved against them, in place.
+
+        users: distinct indexes of the model's users; teacher_items int32 [n, k] (-1 = padding), teacher_scores float32 [n, k], on the device,
+        such as another session's `top_scores` returns them.  The gradients come back as device tensors."""
+        host = np.asarray(users.cpu() if isinstance(users, torch.Tensor) else users)
+        index = np.asarray(host, dtype=np.float64)
+        if index.ndim != 1 or not np.all((index >= 0) & (index < self.n_users) & (index == np.floor(index))):
+            raise ValueError("[users] must be indexes of the model's users")
+        if len(np.unique(index)) != len(index):
+            raise ValueError("[users] must not name a user twice")
+        if self.n_users > 1 << 24:
+            raise ValueError("[distill] names users by float32 index: more than 2^24 users are not supported")
+        if learning_rate is not None and not 0.0 < float(learning_rate) < float("inf"):
+            raise ValueError("[learning_rate] must be a finite number above 0")
+        at = torch.from_numpy(index.astype(np.int64)).to(self.device)
+        mv, n, F = self._model_view(), len(index), self.n_factors
+        K = int(_hip.lib().rfm_effective_factors(C.byref(mv)))
+        used = 2 * F if self.has_if else F
+        users_d = at.to(torch.float32)
+        rows = torch.empty((n, K), dtype=torch.float32, device=self.device)
+        table = torch.empty((self.n_items, K), dtype=torch.float32, device=self.device)
+        bias = torch.empty(self.n_items, dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            rc = _hip.lib().rfm_effective_factors_device(C.byref(mv), n, C.c_void_p(users_d.data_ptr()), C.c_void_p(rows.data_ptr()),
+                                                         C.c_void_p(table.data_ptr()), C.c_void_p(bias.data_ptr()), C.c_void_p(stream))
+        _hip.raise_for_status(rc)
+        got = distill_gradients(rows[:, :used], table[:, :used], bias, teacher_items, teacher_scores, temperature=temperature, allowed=allowed,
+                                allowed_rows=allowed_rows, row_weight=row_weight)
+        # score = w_i + x_if.w_if + <v_u + x_uf.v_uf, v_i> + <v_u, x_if.v_if>: the chain rule behind the two effective tables
+        grad = {"w_i": got.bias, "v_u": got.users[:, :F], "v_i": got.items[:, :F]}
+        if self.has_if:
+            grad["v_u"] = got.users[:, :F] + got.users[:, F:]
+            grad["v_if"] = self.x_if.t() @ got.items[:, F:]
+            grad["w_if"] = self.x_if.t() @ got.bias
+        if self.has_uf:
+            grad["v_uf"] = self.x_uf[at].t() @ got.users[:, :F]
+        if learning_rate is not None and n:
+            for name, g in grad.items():
+                if name == "v_u":
+                    self.weights[name].index_add_(0, at, g, alpha=-float(learning_rate))
+                else:
+                    self.weights[name].sub_(g, alpha=float(learning_rate))
+            self.invalidate_layout()
+        return got.loss, grad
+
+    def recommend(self, users, n_items=10, filter_previous=False, to_host=True, rules=None):
         """float32 [n] user indexes (NaN = unknown) -> float32 [n, n_items] item indexes by descending utility (NaN rows for unknown
-        users); `filter_previous` skips the items of the session's own CSR lists"""
+        users); `filter_previous` skips the items of the session's own CSR lists; `rules` (ScoreRules) say what else holds (`top_scores`,
+        which then ranks: equal scores in the order of the items)"""
+        if rules is not None:
+            best = self.top_scores(users, n_items, rules, filter_previous).items
+            rec = torch.where(best < 0, float("nan"), best.to(torch.float32))
+            return rec.cpu().numpy() if to_host else rec
         users_d = self._to_device(users, 1, "users")
         n_items = int(n_items)
         if n_items < 1 or n_items > self.n_items:

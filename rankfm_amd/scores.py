@@ -46,6 +46,18 @@ class ScoreRules:
     allowed: Optional[torch.Tensor] = None
     allowed_rows: Optional[torch.Tensor] = None
 
+    def rows(self, begin, end):
+        """the rules of rows begin .. end - 1 of a call"""
+        def cut(v):
+            return v[begin:end] if isinstance(v, torch.Tensor) else v
+        per_row = self.allowed is not None and self.allowed_rows is None and self.allowed.shape[0] > 1
+        history = self.history
+        if history is not None and self.history_rows is None:
+            history = (history[0][begin:end + 1], history[1])
+        return ScoreRules(history, cut(self.history_rows), cut(self.repetition), cut(self.frequency), cut(self.presence), self.item_bias,
+                          None if self.row_bias is None else (self.row_bias[0][begin:end + 1],) + tuple(self.row_bias[1:]),
+                          cut(self.allowed) if per_row else self.allowed, cut(self.allowed_rows))
+
     def penalises(self):
         """whether the rules look at a history at all"""
         return any(isinstance(v, torch.Tensor) or v != off for v, off in ((self.repetition, 1.0), (self.frequency, 0.0), (self.presence, 0.0)))
