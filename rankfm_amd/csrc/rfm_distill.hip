@@ -190,12 +190,13 @@ __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, 
 }
 
 // C[m, n] (+)= sum_k A[m, k] B[k, n] (+ bias[n]), any strides; slices of k (blockIdx.y) go to slices of C.  live: rows k of B whose entry is 0
-// or NaN count as zeros, whatever they hold (rows without a usable teacher entry may be padding).  64 x 64 tile per workgroup, four
-// wavefronts of one 32 x 32 accumulator each (v_mfma_f32_32x32x2_f32, exact fp32), k in LDS stages of 32.
+// or NaN count as zeros, whatever they hold (rows without a usable teacher entry may be padding).  finite: so do elements of B that are not
+// finite -- in the products with dz: where they count that row of dz is NaN already, where a mask has taken them out dz is 0.  64 x 64 tile per
+// workgroup, four wavefronts of one 32 x 32 accumulator each (v_mfma_f32_32x32x2_f32, exact fp32), k in LDS stages of 32.
 constexpr int kKT = 32, kLd = kKT + 1;
 __global__ void __launch_bounds__(256) gemm_kernel(const float *__restrict__ A, long long am, long long ak, const float *__restrict__ B, long long bk, long long bn,
                                                    const float *__restrict__ bias, float *__restrict__ C, long long cm, long long slice_stride, long long M, int N, int K,
-                                                   int k_slice, int n_tiles, int accumulate, const float *__restrict__ live) {
+                                                   int k_slice, int n_tiles, int accumulate, const float *__restrict__ live, int finite) {
     __shared__ float sA[64 * kLd], sB[64 * kLd];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave >> 1, wc = wave & 1;
     const long long m0 = (long long)(blockIdx.x / n_tiles) * 64;
@@ -210,7 +211,8 @@ __global__ void __launch_bounds__(256) gemm_kernel(const float *__restrict__ A, 
             const int ra = ak == 1 ? e >> 5 : e & 63, ca = ak == 1 ? e & 31 : e >> 6;      // (consecutive threads along the contiguous side)
             const int rb = bk == 1 ? e >> 5 : e & 63, cb = bk == 1 ? e & 31 : e >> 6;
             sA[ra * kLd + ca] = m0 + ra < M && k0 + ca < ke ? A[(m0 + ra) * am + (long long)(k0 + ca) * ak] : 0.0f;
-            sB[rb * kLd + cb] = n0 + rb < N && k0 + cb < ke && (!live || live[k0 + cb] > 0.0f) ? B[(long long)(k0 + cb) * bk + (long long)(n0 + rb) * bn] : 0.0f;
+            const float b = n0 + rb < N && k0 + cb < ke && (!live || live[k0 + cb] > 0.0f) ? B[(long long)(k0 + cb) * bk + (long long)(n0 + rb) * bn] : 0.0f;
+            sB[rb * kLd + cb] = finite && !(fabsf(b) < INFINITY) ? 0.0f : b;
         }
         __syncthreads();
         const float *pa = sA + (wr * 32 + (lane & 31)) * kLd + (lane >> 5), *pb = sB + (wc * 32 + (lane & 31)) * kLd + (lane >> 5);
@@ -350,12 +352,12 @@ static int run_matrix(const rfm_distill_args *a, char *base, hipStream_t stream)
         const float *u = a->users + (size_t)r0 * a->user_stride;
         const unsigned rt = (unsigned)((nr + 63) / 64);
         const int more = r0 > 0;
-        gemm_kernel<<<dim3(rt * (unsigned)it), dim3(256), 0, stream>>>(u, a->user_stride, 1, a->items, 1, a->item_stride, a->bias, z, I, 0, nr, I, K, K, it, 0, nullptr);
+        gemm_kernel<<<dim3(rt * (unsigned)it), dim3(256), 0, stream>>>(u, a->user_stride, 1, a->items, 1, a->item_stride, a->bias, z, I, 0, nr, I, K, K, it, 0, nullptr, 0);
         softmax_rows_kernel<<<dim3((unsigned)nr), dim3(256), 0, stream>>>(*a, r0, z, part, mass, mi, mp);
         if (!grad) continue;
-        gemm_kernel<<<dim3(rt * (unsigned)kt, (unsigned)slices), dim3(256), 0, stream>>>(z, I, 1, a->items, a->item_stride, 1, nullptr, d_part, K, nr * K, nr, K, I, slice, kt, 0, nullptr);
+        gemm_kernel<<<dim3(rt * (unsigned)kt, (unsigned)slices), dim3(256), 0, stream>>>(z, I, 1, a->items, a->item_stride, 1, nullptr, d_part, K, nr * K, nr, K, I, slice, kt, 0, nullptr, 1);
         sum_slices_kernel<<<dim3(1024), dim3(256), 0, stream>>>(d_part, nr * K, slices, a->d_users + (size_t)r0 * K);
-        gemm_kernel<<<dim3((unsigned)it * (unsigned)kt), dim3(256), 0, stream>>>(z, 1, I, u, a->user_stride, 1, nullptr, a->d_items, K, 0, I, K, (int)nr, 1 << 20, kt, more, mass + r0);
+        gemm_kernel<<<dim3((unsigned)it * (unsigned)kt), dim3(256), 0, stream>>>(z, 1, I, u, a->user_stride, 1, nullptr, a->d_items, K, 0, I, K, (int)nr, 1 << 20, kt, more, mass + r0, 1);
         if (a->d_bias) column_sum_kernel<<<dim3((unsigned)((I + 255) / 256)), dim3(256), 0, stream>>>(z, nr, I, a->d_bias, more);
     }
     return RFM_OK;
@@ -378,21 +380,26 @@ static int pick_splits(int blocks, int tiles, int slots) {
 }
 
 struct FusedLayout {
-    int kp, waves, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, groups_i, units_i;
+    int kp, columns, block_tiles, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, groups_i, units_i;
     size_t part, mass, ids, ps, acc, user_frag, user_frag_t, item_frag, item_frag_t, item_data, user_data, user_data_t, mask_row, part_m, part_l, part_o, entry, entry_at, part_items, part_bias, bytes;
 };
 static FusedLayout fused_layout(const rfm_distill_args *a) {
     FusedLayout w;
     const bool grad = a->d_users != nullptr;
     w.kp = (a->n_factors + 31) / 32 * 32;
-    w.waves = w.kp <= 64 ? 4 : 8;
     const size_t R = (size_t)a->n_rows, n = (size_t)a->n_teacher, kp = (size_t)w.kp;
     w.user_tiles = (int)((a->n_rows + 31) / 32);
     w.item_tiles = (a->n_items + 31) / 32;
-    w.user_blocks = (w.user_tiles + w.waves - 1) / w.waves;
-    w.item_blocks = (w.item_tiles + w.waves - 1) / w.waves;
-    const int slots = kCus * (w.kp <= 64 ? 3 : 1);              // workgroups that fit on the chip at once, by registers and LDS
-    w.splits_f = pick_splits(w.user_blocks, w.item_tiles, slots);
+    // Column tiles per wavefront: two read LDS half as often, one leaves more workgroups to spread.  Measured with two against one, k = 64, gradients / loss
+    // alone: 512 rows x 50 k items 1.10 / 1.13, 2048 x 50 k 1.01 / 0.96, 4096 x 20 k 1.00 / 0.95, 4096 x 50 k 0.95 / 0.93, 2048 x 200 k 0.96 / 0.93; k = 20
+    // crosses at the same place; with masks one is the faster throughout (2048 x 50 k 1.06).
+    w.columns = w.kp <= 64 && !a->allowed && (long long)w.user_tiles * w.item_tiles >= (1 << 17) ? 2 : 1;
+    w.block_tiles = (w.kp <= 64 ? 4 : 8) * w.columns;
+    w.user_blocks = (w.user_tiles + w.block_tiles - 1) / w.block_tiles;
+    w.item_blocks = (w.item_tiles + w.block_tiles - 1) / w.block_tiles;
+    // workgroups that fit on the chip at once, by registers and LDS (the loss alone needs fewer of both)
+    const int slots = kCus * (w.kp > 64 ? 1 : w.columns == 2 ? 2 : 3), slots_loss = kCus * (w.kp <= 64 && w.columns == 1 ? 4 : 2);
+    w.splits_f = pick_splits(w.user_blocks, w.item_tiles, grad ? slots : slots_loss);
     // items_kernel: equal ranges for the workgroups that fit on the chip at once, no shorter than 4 tiles (or a block, if that is less)
     const long long units = (long long)w.item_blocks * w.user_tiles;
     w.units_i = (int)std::max<long long>((units + slots - 1) / slots, std::min(w.user_tiles, 4));
@@ -408,13 +415,13 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     w.mask_row = take(a->allowed ? 4 * ur : 0);
     w.part_m = take(4 * w.splits_f * ur); w.part_l = take(4 * w.splits_f * ur); w.part_o = take(grad ? 4 * w.splits_f * ur * kp : 0);
     w.entry = take(grad ? ur * n * 8 : 0); w.entry_at = take(grad ? 4 * (size_t)w.user_tiles * (kBuckets + 1) : 0);
-    const size_t parts = (size_t)(w.groups_i + w.item_blocks) * w.waves * 32;
+    const size_t parts = (size_t)(w.groups_i + w.item_blocks) * w.block_tiles * 32;
     w.part_items = take(grad ? 4 * parts * kp : 0); w.part_bias = take(grad ? 4 * parts : 0);
     w.bytes = off;
     return w;
 }
 
-template <int KP, int WAVES>
+template <int KP, int NC>
 static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base, hipStream_t stream) {
     const bool grad = a->d_users != nullptr;
     auto at = [&](size_t off) { return base + off; };
@@ -435,20 +442,23 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     else prepare_kernel<KP, false><<<grid_p, dim3(256), lds, stream>>>(f, c, part, mass, nullptr, nullptr, nullptr);
     f.splits = w.splits_f;
     f.chunk = (w.item_tiles + w.splits_f - 1) / w.splits_f;
-    const dim3 grid_f((unsigned)(w.user_blocks * w.splits_f)), threads(WAVES * 64);
-    if (grad && a->allowed) forward_kernel<KP, true, true, WAVES><<<grid_f, threads, 0, stream>>>(f);
-    else if (grad) forward_kernel<KP, true, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
-    else if (a->allowed) forward_kernel<KP, false, true, WAVES><<<grid_f, threads, 0, stream>>>(f);
-    else forward_kernel<KP, false, false, WAVES><<<grid_f, threads, 0, stream>>>(f);
+    const dim3 grid_f((unsigned)(w.user_blocks * w.splits_f)), threads(Frag<KP>::waves * 64);
+    if constexpr (NC == 1) {
+        if (grad && a->allowed) forward_kernel<KP, NC, true, true><<<grid_f, threads, 0, stream>>>(f);
+        if (!grad && a->allowed) forward_kernel<KP, NC, false, true><<<grid_f, threads, 0, stream>>>(f);
+    }
+    if (grad && !a->allowed) forward_kernel<KP, NC, true, false><<<grid_f, threads, 0, stream>>>(f);
+    if (!grad && !a->allowed) forward_kernel<KP, NC, false, false><<<grid_f, threads, 0, stream>>>(f);
     const int row_blocks = w.user_tiles * 4;
-    join_rows_kernel<KP><<<dim3((unsigned)(row_blocks + (grad ? w.user_tiles : 0))), dim3(512), 0, stream>>>(f, row_blocks, WAVES * 32, part, mass, acc, ids, ps);
+    join_rows_kernel<KP><<<dim3((unsigned)(row_blocks + (grad ? w.user_tiles : 0))), dim3(512), 0, stream>>>(f, row_blocks, w.block_tiles * 32, part, mass, acc, ids, ps);
     if (!grad) return RFM_OK;
     f.units = w.units_i;
     const dim3 grid_i((unsigned)w.groups_i);
-    if (a->allowed) items_kernel<KP, true, WAVES><<<grid_i, threads, 0, stream>>>(f);
-    else items_kernel<KP, false, WAVES><<<grid_i, threads, 0, stream>>>(f);
+    if constexpr (NC == 1)
+        if (a->allowed) items_kernel<KP, NC, true><<<grid_i, threads, 0, stream>>>(f);
+    if (!a->allowed) items_kernel<KP, NC, false><<<grid_i, threads, 0, stream>>>(f);
     // (a block is cut where a range ends inside it)
-    if (w.groups_i > 1 && w.units_i % w.user_tiles != 0) join_items_kernel<KP, WAVES><<<dim3((unsigned)(w.item_blocks * WAVES)), dim3(256), 0, stream>>>(f);
+    if (w.groups_i > 1 && w.units_i % w.user_tiles != 0) join_items_kernel<KP><<<dim3((unsigned)(w.item_blocks * w.block_tiles)), dim3(256), 0, stream>>>(f, w.block_tiles);
     return RFM_OK;
 }
 
@@ -478,10 +488,10 @@ int rfm_distill_device(const rfm_distill_args *a, void *workspace, size_t worksp
     } else {
         const distill::FusedLayout w = distill::fused_layout(a);
         char *base = (char *)workspace;
-        if (w.kp == 32) rc = distill::run_fused<32, 4>(a, w, base, stream);
-        else if (w.kp == 64) rc = distill::run_fused<64, 4>(a, w, base, stream);
-        else if (w.kp == 96) rc = distill::run_fused<96, 8>(a, w, base, stream);
-        else rc = distill::run_fused<128, 8>(a, w, base, stream);
+        if (w.kp == 32) rc = w.columns == 2 ? distill::run_fused<32, 2>(a, w, base, stream) : distill::run_fused<32, 1>(a, w, base, stream);
+        else if (w.kp == 64) rc = w.columns == 2 ? distill::run_fused<64, 2>(a, w, base, stream) : distill::run_fused<64, 1>(a, w, base, stream);
+        else if (w.kp == 96) rc = distill::run_fused<96, 1>(a, w, base, stream);
+        else rc = distill::run_fused<128, 1>(a, w, base, stream);
     }
     if (rc != RFM_OK) return rc;
     return hipGetLastError() == hipSuccess ? RFM_OK : RFM_ERR_HIP;

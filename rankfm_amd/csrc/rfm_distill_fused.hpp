@@ -3,7 +3,7 @@
 // fp32 products on the fp16 matrix cores.  Every fp32 factor is the sum of two fp16 parts, x = h + m: 11 bits of the significand each, rounded to
 // nearest at each cut, so that 2^-24 of x is left over -- half a step of fp32.  Of the four products of two such sums m m' is left out, 2^-24 of
 // |x x'| at most and 2^-27 in the mean: an fp32 product rounds away as much.  Three v_mfma_f32_32x32x16_f16 take 3 / 16 of the time of the
-// fp32 matrix instructions (six with bf16 parts, which hold 8 bits: measured, 1.16 -> 0.66 ms for the k = 64 step of 8192 rows x 50 k items).
+// fp32 matrix instructions (six with bf16 parts, which hold 8 bits: the step of 8192 rows x 50 k items at k = 64 took 1164 us with those, 794 with these).
 // fp16 has little range, so every tile of 32 rows is scaled by a power of two, its largest finite value to 2^14 .. 2^15: what is 2^-16 of that
 // or more keeps its 22 bits, what is less an absolute error of 2^-40 of it.  The scales are taken back exactly where the sums are used.
 //
@@ -15,9 +15,15 @@
 // The sum over k does not care in which order the k's come as long as both sides agree, so the transposed copy is written in that order, and the
 // weights go from one product to the next without leaving their lane.
 //
-//   forward_kernel   columns: 32 users per wavefront, fixed; streams item tiles through LDS.  z^T = items . users^T; a column's maximum and sum are
+//   forward_kernel   columns: 32 or 64 users per wavefront, fixed; streams item tiles through LDS.  z^T = items . users^T; a column's maximum and sum are
 //                    in-lane; weighted sums O^T += items^T . exp2(z^T - max).
-//   items_kernel     columns: 32 items per wavefront, fixed; streams user tiles.  z = users . items^T, dz from the row's lse, O^T += users^T . dz.
+//   items_kernel     columns: 32 or 64 items per wavefront, fixed; streams user tiles.  z = users . items^T, dz from the row's lse, O^T += users^T . dz.
+//
+// What bounds them: the matrix instructions, at the clock that their power leaves.  8192 rows x 50 k items at k = 64, gradients: 0.69 ms in all, of which
+// forward_kernel 318 us, items_kernel 385, prepare 34; 2 x 6 x 8192 x 50 k x 64 x 2 operations are 0.63 TFLOP and 393 us at the 1.6 PFLOP/s that a
+// loop of nothing but these instructions reaches.  The rest are LDS reads of the streamed tiles (-18 .. -27 % in a copy without them), the exponentials
+// and the cuts into parts, which do not overlap with them where power is the limit.  The loss alone, k = 64: 187 us.  2048 rows x 200 k items at k = 128:
+// 1.28 ms, of which 564 + 659.
 #pragma once
 
 namespace rfm {
@@ -39,8 +45,11 @@ template <int KP> struct Frag {
     static constexpr int steps = KP / 16, cols = KP / 32;
     static constexpr int bytes = KP * 128;       // one copy of a tile: KP / 16 x 2 parts x 1 KB; the transposed copy has as many
     static constexpr int waves = KP <= 64 ? 4 : 8;               // wavefronts of a workgroup
-    static constexpr int per_simd = KP <= 64 ? 3 : 2;             // wavefronts per SIMD that the registers are kept to
 };
+// Wavefronts per SIMD that the registers are kept to.  Up to 64 factors a wavefront may have two tiles of 32 columns, NC = 2: what it reads of a streamed
+// tile from LDS then serves both, at two wavefronts per SIMD instead of three and half as many workgroups (8192 rows x 50 k items at k = 64: 728 -> 689 us;
+// at k = 128, where it would leave one, 12 % slower).
+template <int KP, int NC> constexpr int kPerSimd = KP <= 64 && NC == 1 ? 3 : 2;
 
 struct FusedArgs {
     rfm_distill_args a;
@@ -49,7 +58,7 @@ struct FusedArgs {
     int units;                                   // items: (block, user tile) pairs per workgroup
     char *user_frag, *user_frag_t, *item_frag, *item_frag_t;
     float *item_data, *user_data, *user_data_t;  // [item_tiles, kItemData], [user_tiles, kUserData] twice
-    int32_t *mask_row;                           // [user_tiles * 32] mask of each row, -1 = none
+    int32_t *mask_row;                           // [user_tiles * 32] mask of each row, -1 = none, -2 = a row that counts nowhere
     float *part_m, *part_l, *part_o;             // forward: [splits, user_tiles * 32 (, KP)]
     uint2 *entry;                                // [user_tiles, 32 n]: (item << 5 | row, p), by bucket
     int32_t *entry_at;                           // [user_tiles, kBuckets + 1] where a bucket's entries begin
@@ -77,7 +86,9 @@ __device__ __forceinline__ float block_max(float x, float *s_max) {
 }
 
 // One workgroup per tile of 32 rows of a table: its fragments.  One copy holds row * `by`, the transposed one row * weight[row] (1 without), each with
-// a scale of its own.  Rows without a usable teacher entry (live [32]) count as zeros: they may be padding.
+// a scale of its own.  Rows without a usable teacher entry (live [32]) count as zeros: they may be padding.  In the transposed copy, which the weights
+// multiply, so does a factor that is not finite: where it counts the score and with it the row's sum is NaN already, where a mask has taken it out its
+// weight is 0.
 template <int KP>
 __device__ void write_frags(const float *__restrict__ x, long long stride, int tile, long long rows, int factors, float by, const float *__restrict__ live,
                             const float *__restrict__ weight, float all_weight, char *frag, char *frag_t, float *lds, float *s_max, int *e_out, int *e_t_out) {
@@ -120,7 +131,7 @@ __device__ void write_frags(const float *__restrict__ x, long long stride, int t
             const long long r = (long long)tile * 32 + row;
             const float v = lds[row * ld + 32 * (ct >> 1) + (lane & 31)], g = weight && r < rows ? weight[r] * all_weight : all_weight;
             _Float16 a, b;
-            split2(v == 0.0f ? 0.0f : ldexpf(v * g, ex_t), a, b);
+            split2(v == 0.0f || !(fabsf(v) < INFINITY) ? 0.0f : ldexpf(v * g, ex_t), a, b);
             h[j] = a; m[j] = b;
         }
         f16x8 *out = reinterpret_cast<f16x8 *>(frag_t + (size_t)tile * Frag<KP>::bytes) + ct * 128 + lane;
@@ -159,9 +170,9 @@ __global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c
         }
         if (threadIdx.x < 32 && a.allowed) {
             const long long r = (long long)b * 32 + threadIdx.x;
-            long long m = -1;
-            if (r < a.n_rows) m = a.allowed_rows ? (long long)a.allowed_rows[r] : (a.n_allowed == 1 ? 0 : r);
-            f.mask_row[r] = m >= 0 && m < a.n_allowed ? (int32_t)m : -1;
+            long long m = -2;
+            if (live[threadIdx.x] > 0.0f) m = max(a.allowed_rows ? (long long)a.allowed_rows[r] : (a.n_allowed == 1 ? 0 : r), -1ll);
+            f.mask_row[r] = (int32_t)m;                          // (below n_allowed: the row would not be live)
         }
     } else if (b < f.user_tiles + f.item_tiles) {
         const int t = b - f.user_tiles;
@@ -177,30 +188,37 @@ __global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c
     }
 }
 
-// ---- LDS staging: a kilobyte per instruction straight from memory (global_load_lds, 16 bytes per lane) --------------------------------------------
-__device__ __forceinline__ void stage16(const char *from, char *to) {            // `to` is the wavefront's own kilobyte, `from` the lane's 16 bytes
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+// ---- LDS staging: a kilobyte per instruction straight from memory (global_load_lds, 16 bytes per lane).  Written out rather than by the builtin:
+// the compiler holds every later LDS read of the step back until such loads have arrived (s_waitcnt vmcnt(0): it cannot tell the buffers apart), which
+// is the latency they are meant to hide (the step of 2048 rows x 200 k items at k = 128: 1338 -> 1292 us).  Nothing but LDS is written by them; what
+// waits for them is staged() below.  `to`: the wavefront's own place in LDS, `from`: the lane's own bytes.
+__device__ __forceinline__ unsigned lds_offset(const void *p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) char *)p; }
+__device__ __forceinline__ void stage16(const char *from, char *to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds_offset(to))), "v"(from) : "memory", "m0");
 }
 __device__ __forceinline__ void stage4(const char *from, char *to) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 4, 0, 0);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds_offset(to))), "v"(from) : "memory", "m0");
 }
-// one copy of a tile, and the floats that go with it
+// One copy of a tile, and the floats that go with it.  Every wavefront issues the same number of instructions (some fetch what another fetches too):
+// that number is what a wavefront may leave in flight when it waits for the group before.
+template <int KP, int WAVES> constexpr int kCopyLoads = (Frag<KP>::bytes / 1024 + WAVES - 1) / WAVES;
 template <int KP, int WAVES>
 __device__ __forceinline__ void stage_copy(const char *frag, int tile, char *buf, int wave, int lane) {
     constexpr int bytes = Frag<KP>::bytes, kb = bytes / 1024;
     const char *src = frag + (size_t)tile * bytes + lane * 16;
 #pragma unroll
-    for (int q = 0; q < (kb + WAVES - 1) / WAVES; ++q) {
-        const int k = q * WAVES + wave;
-        if (kb % WAVES == 0 || k < kb) stage16(src + k * 1024, buf + k * 1024);
+    for (int q = 0; q < kCopyLoads<KP, WAVES>; ++q) {
+        const int k = kb % WAVES == 0 ? q * WAVES + wave : min(q * WAVES + wave, kb - 1);
+        stage16(src + k * 1024, buf + k * 1024);
     }
 }
-__device__ __forceinline__ void stage_data(const float *data, char *buf, int wave, int lane) {
-    if (wave == 0) stage4(reinterpret_cast<const char *>(data + lane), buf);
-}
-__device__ __forceinline__ void staged() {       // this wavefront's staging is in LDS
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+__device__ __forceinline__ void stage_data(const float *data, char *buf, int lane) { stage4(reinterpret_cast<const char *>(data + lane), buf); }
+// all but the last LEFT loads of this wavefront have arrived, and everyone else's too
+template <int LEFT>
+__device__ __forceinline__ void staged() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");       // (its reads of the buffer that is fetched into next are over, too)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -230,33 +248,39 @@ __device__ __forceinline__ void split_weights(const f32x16 &w, f16x8 (*p)[2]) {
         p[t][1] = __builtin_bit_cast(f16x8, m);
     }
 }
-// o[c] = o[c] * by + rows of the transposed tile . weights.  A tile's 32 terms are summed by themselves first: the running sum sees one
-// operation per tile
-template <int KP>
-__device__ __forceinline__ void weighted_sum(const char *tile_t, int lane, const f16x8 (*p)[2], float by, f32x16 *o) {
+// o[n][c] = o[n][c] * by[n] + rows of the transposed tile . weights of column tile n.  A tile's 32 terms are summed by themselves first: the running sum
+// sees one operation per tile
+template <int KP, int NC>
+__device__ __forceinline__ void weighted_sum(const char *tile_t, int lane, const f16x8 (*p)[2][2], const float *by, f32x16 (*o)[Frag<KP>::cols]) {
 #pragma unroll
     for (int c = 0; c < Frag<KP>::cols; ++c) {
-        f32x16 sum = {0};
+        f32x16 sum[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) sum[n] = f32x16{0};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const f16x8 *at = reinterpret_cast<const f16x8 *>(tile_t) + (c * 2 + t) * 128 + lane;
             const f16x8 a[2] = {at[0], at[64]};
-            sum = mfma3(a, p[t], sum);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) sum[n] = mfma3(a, p[n][t], sum[n]);
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[c][r] = fmaf(o[c][r], by, sum[r]);
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[n][c][r] = fmaf(o[n][c][r], by[n], sum[n][r]);
     }
 }
-template <int KP>
-__device__ __forceinline__ f32x16 tile_scores(const char *tile, int lane, const f16x8 (*x)[2]) {
-    f32x16 s = {0};
+template <int KP, int NC>
+__device__ __forceinline__ void tile_scores(const char *tile, int lane, const f16x8 (*x)[Frag<KP>::steps][2], f32x16 *s) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) s[n] = f32x16{0};
 #pragma unroll
     for (int k = 0; k < Frag<KP>::steps; ++k) {
         const f16x8 *at = reinterpret_cast<const f16x8 *>(tile) + k * 128 + lane;
         const f16x8 a[2] = {at[0], at[64]};
-        s = mfma3(a, x[k], s);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n] = mfma3(a, x[n][k], s[n]);
     }
-    return s;
 }
 template <int KP>
 __device__ __forceinline__ void load_columns(const char *frag, int tile, int lane, f16x8 (*x)[2]) {
@@ -302,103 +326,108 @@ __device__ __forceinline__ float sum16(const f32x16 &s) {
 // is an exact power of two (a fractional one rounds differently where it is put in and where it is taken out: up to 7e-7 of a column).
 //
 // Block b: split b % splits of the items, columns block b / splits: with a multiple of 8 splits the workgroups of one XCD stream the same items.
-// The loop is one tile deep in flight: while the vector unit turns tile t's scores into weights, the matrix cores make tile t + 1's.
-template <int KP, bool GRAD, bool MASK, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, Frag<KP>::per_simd) forward_kernel(const FusedArgs f) {
-    constexpr int kBytes = Frag<KP>::bytes, kBuf = kBytes + kItemData * 4;
-    __shared__ __attribute__((aligned(16))) char buf[2][kBuf], buf_t[GRAD ? 2 : 1][GRAD ? kBytes : 16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5;
-    const int split = (int)blockIdx.x % f.splits, tile = (int)blockIdx.x / f.splits * WAVES + wave;
-    const int mine = tile < f.user_tiles ? tile : f.user_tiles - 1;              // (a wavefront without users works on the last ones and writes nothing)
+template <int KP, int NC, bool GRAD, bool MASK>
+__global__ void __launch_bounds__(Frag<KP>::waves * 64, (GRAD ? kPerSimd<KP, NC> : NC == 1 ? 4 : 2)) forward_kernel(const FusedArgs f) {
+    constexpr int WAVES = Frag<KP>::waves;
+    constexpr int kBytes = Frag<KP>::bytes, kBuf = kBytes * (GRAD ? 2 : 1) + kItemData * 4, kGroup = kCopyLoads<KP, WAVES> * (GRAD ? 2 : 1) + 1;
+    __shared__ __attribute__((aligned(16))) char buf[3][kBuf];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int split = (int)blockIdx.x % f.splits, tile = ((int)blockIdx.x / f.splits * WAVES + wave) * NC;
     const int t0 = split * f.chunk, t1 = min(t0 + f.chunk, f.item_tiles);
-    f16x8 x[Frag<KP>::steps][2];
-    load_columns<KP>(f.user_frag, mine, lane, x);
-    const float unscale = f.user_data[(size_t)mine * kUserData + 32];
-    const uint32_t *mask = nullptr;
-    if constexpr (MASK) {
-        const int m = f.mask_row[mine * 32 + (lane & 31)];
-        if (m >= 0) mask = f.a.allowed + (size_t)m * (size_t)f.item_tiles;
-    }
-    float top = kLowest, total = 0.0f;
-    f32x16 o[GRAD ? Frag<KP>::cols : 1];
-    if constexpr (GRAD)
-        for (int c = 0; c < Frag<KP>::cols; ++c) o[c] = f32x16{0};
-    auto stage_scores = [&](int t) {
-        stage_copy<KP, WAVES>(f.item_frag, t, buf[t & 1], wave, lane);
-        stage_data(f.item_data + (size_t)t * kItemData, buf[t & 1] + kBytes, wave, lane);
-    };
-    unsigned word = 0xffffffffu, next_word = 0xffffffffu;
-    auto finish = [&](int t, f32x16 &s, float &high, float &e, float &scale) {       // z of tile t (log2 units) out of its products, and the tile's scale
-        const f32x4 *data = reinterpret_cast<const f32x4 *>(buf[t & 1] + kBytes);
-        const f32x4 last = data[8];
-        const float by = last[0] * unscale;
-        e = last[1];
-        scale = last[2];
+    f16x8 x[NC][Frag<KP>::steps][2];
+    float unscale[NC], top[NC], total[NC];
+    const uint32_t *mask[NC];
+    unsigned next_word[NC];
+    f32x16 o[NC][GRAD ? Frag<KP>::cols : 1];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 b = data[half + 2 * q];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(s[4 * q + k], by, b[k]);
-        }
+    for (int n = 0; n < NC; ++n) {
+        const int mine = min(tile + n, f.user_tiles - 1);        // (where there are no users left, the last ones are worked on and nothing is written)
+        load_columns<KP>(f.user_frag, mine, lane, x[n]);
+        unscale[n] = f.user_data[(size_t)mine * kUserData + 32];
+        top[n] = kLowest;
+        total[n] = 0.0f;
+        mask[n] = nullptr;
+        next_word[n] = 0xffffffffu;
         if constexpr (MASK) {
-            mask16(s, word >> (4 * half));
+            const int m = f.mask_row[mine * 32 + col];
+            if (m >= 0) { mask[n] = f.a.allowed + (size_t)m * (size_t)f.item_tiles; next_word[n] = mask[n][t0]; }
         }
-        high = largest16(s) - e;
-    };
-    if constexpr (MASK)
-        if (mask) { word = mask[t0]; next_word = mask[min(t0 + 1, t1 - 1)]; }
-    stage_scores(t0);
-    if constexpr (GRAD) stage_copy<KP, WAVES>(f.item_frag_t, t0, buf_t[t0 & 1], wave, lane);
-    staged();
-    if (t0 + 1 < t1) stage_scores(t0 + 1);
-    // one tile: its z is in `s`; that of the next one is left in `next`
-    auto step = [&](int t, f32x16 &s, float high, float e, float scale, f32x16 &next, float &next_high, float &next_e, float &next_scale) {
-        staged();                                                // tile t + 1's scores copy and tile t's other copy are in LDS; the buffers of before are free
-        if (t + 1 < t1) {
-            word = next_word;
-            if constexpr (MASK)
-                if (mask && t + 2 < t1) next_word = mask[t + 2];
-            if (t + 2 < t1) stage_scores(t + 2);
-            if constexpr (GRAD) stage_copy<KP, WAVES>(f.item_frag_t, t + 1, buf_t[(t + 1) & 1], wave, lane);
-        }
-        float by = 1.0f;
-        if (__any(high > top + (kLimit - kUnit))) {
-            const float to = fmaxf(top, ceilf(fmaxf(high, __shfl_xor(high, 32))));
-            by = __builtin_amdgcn_exp2f(top - to);
-            top = to;
-        }
-        const float off = top + (e - kUnit);
-        next = tile_scores<KP>(buf[(t + 1) & 1], lane, x);       // (behind the last tile: of what is left in LDS, and not used)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - off);
-        total = fmaf(sum16(s), scale, total * by);
-        if constexpr (GRAD) {
-            f16x8 p[2][2];
-            split_weights(s, p);
-            weighted_sum<KP>(buf_t[t & 1], lane, p, by, o);
-        }
-        finish(t + 1, next, next_high, next_e, next_scale);
-    };
-    f32x16 s0 = tile_scores<KP>(buf[t0 & 1], lane, x), s1;
-    float h0, h1, e0, e1, c0, c1;
-    finish(t0, s0, h0, e0, c0);
-    for (int t = t0; t < t1; t += 2) {
-        step(t, s0, h0, e0, c0, s1, h1, e1, c1);
-        if (t + 1 >= t1) break;
-        step(t + 1, s1, h1, e1, c1, s0, h0, e0, c0);
+        if constexpr (GRAD)
+            for (int c = 0; c < Frag<KP>::cols; ++c) o[n][c] = f32x16{0};
     }
-    if (tile >= f.user_tiles) return;
-    total += __shfl_xor(total, 32);
-    const size_t at = (size_t)split * f.user_tiles * 32 + (size_t)tile * 32 + (lane & 31);
-    if (half == 0) { f.part_m[at] = top; f.part_l[at] = total; }
-    if constexpr (GRAD) {
+    // Three buffers: what a step needs was asked for two steps before.  Behind the last tile the last one is fetched again, so that a group always has
+    // the same number of loads.
+    auto stage = [&](int t, int at) {
+        const int from = min(t, t1 - 1);
+        stage_copy<KP, WAVES>(f.item_frag, from, buf[at], wave, lane);
+        if constexpr (GRAD) stage_copy<KP, WAVES>(f.item_frag_t, from, buf[at] + kBytes, wave, lane);
+        stage_data(f.item_data + (size_t)from * kItemData, buf[at] + kBuf - kItemData * 4, lane);
+    };
+    stage(t0, 0);
+    stage(t0 + 1, 1);
+    for (int t = t0, i = 0; t < t1; ++t, i = i == 2 ? 0 : i + 1) {
+        staged<kGroup>();                                        // tile t is in LDS, and nobody reads tile t - 1 any more
+        unsigned word[NC];
 #pragma unroll
-        for (int c = 0; c < Frag<KP>::cols; ++c)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 v = {o[c][4 * q], o[c][4 * q + 1], o[c][4 * q + 2], o[c][4 * q + 3]};
-                *reinterpret_cast<f32x4 *>(f.part_o + at * KP + 32 * c + 8 * q + 4 * half) = v;
+        for (int n = 0; n < NC; ++n) {
+            word[n] = next_word[n];
+            if constexpr (MASK) {
+                asm volatile("" : "+v"(word[n]));                // (no instruction: it is here, and is taken before anything else is asked for)
+                if (mask[n]) next_word[n] = mask[n][min(t + 1, t1 - 1)];
             }
+        }
+        stage(t + 2, i == 0 ? 2 : i - 1);
+        f32x16 s[NC];
+        tile_scores<KP, NC>(buf[i], lane, x, s);
+        const f32x4 *data = reinterpret_cast<const f32x4 *>(buf[i] + kBuf - kItemData * 4);
+        const f32x4 last = data[8];
+        const float e = last[1], scale = last[2];
+        float by[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const float unit = last[0] * unscale[n];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {                        // z in log2 units
+                const f32x4 b = data[half + 2 * q];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unit, b[k]);
+            }
+            if constexpr (MASK) mask16(s[n], word[n] >> (4 * half));
+            const float high = largest16(s[n]) - e;
+            by[n] = 1.0f;
+            if (__any(high > top[n] + (kLimit - kUnit))) {
+                const float to = fmaxf(top[n], ceilf(fmaxf(high, __shfl_xor(high, 32))));
+                by[n] = __builtin_amdgcn_exp2f(top[n] - to);
+                top[n] = to;
+            }
+            const float off = top[n] + (e - kUnit);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - off);
+            total[n] = fmaf(sum16(s[n]), scale, total[n] * by[n]);
+        }
+        if constexpr (GRAD) {
+            f16x8 p[NC][2][2];
+#pragma unroll
+            for (int n = 0; n < NC; ++n) split_weights(s[n], p[n]);
+            weighted_sum<KP, NC>(buf[i] + kBytes, lane, p, by, o);
+        }
+    }
+    staged<0>();                                                 // nothing is on its way into this workgroup's LDS when it ends
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        if (tile + n >= f.user_tiles) return;
+        const float sum = total[n] + __shfl_xor(total[n], 32);
+        const size_t at = (size_t)split * f.user_tiles * 32 + (size_t)(tile + n) * 32 + col;
+        if (half == 0) { f.part_m[at] = top[n]; f.part_l[at] = sum; }
+        if constexpr (GRAD) {
+#pragma unroll
+            for (int c = 0; c < Frag<KP>::cols; ++c)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 v = {o[n][c][4 * q], o[n][c][4 * q + 1], o[n][c][4 * q + 2], o[n][c][4 * q + 3]};
+                    *reinterpret_cast<f32x4 *>(f.part_o + at * KP + 32 * c + 8 * q + 4 * half) = v;
+                }
+        }
     }
 }
 
@@ -433,7 +462,7 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
         __builtin_amdgcn_wave_barrier();
         const int count = min(64, f.splits - s0);
         const float *from = f.part_o + ((size_t)s0 * padded + r) * KP;
-#pragma unroll 4
+#pragma unroll 16                                                // (loads in flight: they are far apart)
         for (int q = 0; q < count; ++q) {
 #pragma unroll
             for (int k = 0; k < (KP + 63) / 64; ++k)
@@ -515,202 +544,226 @@ constexpr int kPatch = 36;                       // floats per item of the patch
 // The work is cut into equal ranges of (block of items, user tile) pairs, one per workgroup that fits on the chip: no workgroup waits for a last
 // round.  A block that lies inside one range is written out as it is; the others' parts go to slot workgroup + block -- workgroups and blocks
 // both ascend along the ranges, so no two parts share one -- and are joined in that order.
-template <int KP, bool MASK, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, Frag<KP>::per_simd) items_kernel(const FusedArgs f) {
-    constexpr int kBytes = Frag<KP>::bytes, kBuf = kBytes + kUserData * 4;
-    __shared__ __attribute__((aligned(16))) char buf[2][kBuf], buf_t[2][kBuf];
-    __shared__ __attribute__((aligned(16))) float patches[WAVES][32 * kPatch];
+template <int KP, int NC, bool MASK>
+__global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) items_kernel(const FusedArgs f) {
+    constexpr int WAVES = Frag<KP>::waves;
+    constexpr int kBytes = Frag<KP>::bytes, kBuf = 2 * kBytes + 2 * kUserData * 4;
+    __shared__ __attribute__((aligned(16))) char buf[2][kBuf];
+    __shared__ __attribute__((aligned(16))) float patches[WAVES][NC * 32 * kPatch];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int n32 = 32 * f.a.n_teacher;
     float *patch = patches[wave];
-    for (int k = lane; k < 32 * kPatch; k += 64) patch[k] = 0.0f;
+    for (int k = lane; k < NC * 32 * kPatch; k += 64) patch[k] = 0.0f;
     const long long last_unit = min((long long)(blockIdx.x + 1) * f.units, (long long)f.item_blocks * f.user_tiles);
     for (long long unit = (long long)blockIdx.x * f.units; unit < last_unit;) {
-    const int block = (int)(unit / f.user_tiles), t0 = (int)(unit - (long long)block * f.user_tiles);
-    const int t1 = (int)min((long long)f.user_tiles, t0 + (last_unit - unit));
-    unit += t1 - t0;
-    const int tile = block * WAVES + wave, mine = tile < f.item_tiles ? tile : f.item_tiles - 1;
-    f16x8 x[Frag<KP>::steps][2];
-    load_columns<KP>(f.item_frag, mine, lane, x);
-    const float bias = f.item_data[(size_t)mine * kItemData + col], unscale = f.item_data[(size_t)mine * kItemData + 32];
-    const unsigned base = (unsigned)tile * 32u;
-    f32x16 o[Frag<KP>::cols];
-    for (int c = 0; c < Frag<KP>::cols; ++c) o[c] = f32x16{0};
-    // `gate`: what an exponent may reach before `top` is moved -- anything at first, so that the first weight of a column sets it
-    float top = 0.0f, gate = kLowest, d_bias = 0.0f;
-    auto mask_word = [&](int t) {                                // of row `col` of the tile, the bits of this wavefront's items
-        const int m = f.mask_row[t * 32 + col];
-        return f.a.allowed[(size_t)max(m, 0) * (size_t)f.item_tiles + mine] | (unsigned)(m >> 31);
-    };
-    auto stage_scores = [&](int t) {
-        stage_copy<KP, WAVES>(f.user_frag, t, buf[t & 1], wave, lane);
-        stage_data(f.user_data + (size_t)t * kUserData, buf[t & 1] + kBytes, wave, lane);
-    };
-    auto stage_rest = [&](int t) {
-        stage_copy<KP, WAVES>(f.user_frag_t, t, buf_t[t & 1], wave, lane);
-        stage_data(f.user_data_t + (size_t)t * kUserData, buf_t[t & 1] + kBytes, wave, lane);
-    };
-    unsigned word = 0, next_word = 0;
-    // the exponents of tile t's weights, for `top` as it stands, out of its products; and the tile's scale
-    auto finish = [&](int t, f32x16 &s, float &high, float &e, float &scale) {
-        const f32x4 *data = reinterpret_cast<const f32x4 *>(buf[t & 1] + kBytes);
-        const f32x4 last = data[8];
-        const float by = last[0] * unscale;
-        e = last[1];
-        scale = last[2];
-        const float shift = bias - (top + (e - kUnit));
+        const int block = (int)(unit / f.user_tiles), t0 = (int)(unit - (long long)block * f.user_tiles);
+        const int t1 = (int)min((long long)f.user_tiles, t0 + (last_unit - unit));
+        unit += t1 - t0;
+        const int tile = (block * WAVES + wave) * NC;
+        const unsigned base = (unsigned)tile * 32u;
+        f16x8 x[NC][Frag<KP>::steps][2];
+        // `gate`: what an exponent may reach before `top` is moved -- anything at first, so that the first weight of a column sets it
+        float bias[NC], unscale[NC], top[NC], gate[NC], d_bias[NC];
+        unsigned next_word[NC];
+        f32x16 o[NC][Frag<KP>::cols];
+        auto mask_word = [&](int t, int n) {                     // of row `col` of the tile, the bits of this wavefront's items
+            const int m = f.mask_row[min(t, t1 - 1) * 32 + col];
+            const unsigned word = f.a.allowed[(size_t)max(m, 0) * (size_t)f.item_tiles + min(tile + n, f.item_tiles - 1)];
+            return m >= 0 ? word : (unsigned)(-2 - m);           // (-1: all of them, -2: none)
+        };
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 lse = data[half + 2 * q];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(s[4 * q + k], by, shift) - lse[k];
+        for (int n = 0; n < NC; ++n) {
+            const int mine = min(tile + n, f.item_tiles - 1);
+            load_columns<KP>(f.item_frag, mine, lane, x[n]);
+            bias[n] = f.item_data[(size_t)mine * kItemData + col];
+            unscale[n] = f.item_data[(size_t)mine * kItemData + 32];
+            top[n] = 0.0f;
+            gate[n] = kLowest;
+            d_bias[n] = 0.0f;
+            next_word[n] = 0;
+            if constexpr (MASK) next_word[n] = mask_word(t0, n);
+            for (int c = 0; c < Frag<KP>::cols; ++c) o[n][c] = f32x16{0};
         }
-        if constexpr (MASK) mask16_rows(s, word);
-        high = largest16(s);
-    };
-    if constexpr (MASK) { word = mask_word(t0); next_word = mask_word(min(t0 + 1, t1 - 1)); }
-    const int bucket = block % kBuckets;
-    int begin = f.entry_at[(size_t)t0 * (kBuckets + 1) + bucket], end = f.entry_at[(size_t)t0 * (kBuckets + 1) + bucket + 1];
-    stage_scores(t0);
-    stage_rest(t0);
-    staged();
-    if (t0 + 1 < t1) stage_scores(t0 + 1);
-    auto step = [&](int t, f32x16 &s, float high, float e, float scale, f32x16 &next, float &next_high, float &next_e, float &next_scale) {
-        staged();
-        const int from = begin, to = end;
-        uint2 entry = make_uint2(0xffffffffu, 0);
-        if (from + lane < to) entry = f.entry[(size_t)t * n32 + from + lane];
-        if (t + 1 < t1) {
-            begin = f.entry_at[(size_t)(t + 1) * (kBuckets + 1) + bucket];
-            end = f.entry_at[(size_t)(t + 1) * (kBuckets + 1) + bucket + 1];
-            if constexpr (MASK) {
-                word = next_word;
-                next_word = mask_word(min(t + 2, t1 - 1));
-            }
-            if (t + 2 < t1) stage_scores(t + 2);
-            stage_rest(t + 1);
-        }
-        const f32x4 *data = reinterpret_cast<const f32x4 *>(buf_t[t & 1] + kBytes);
-        float by = 1.0f;
-        if (__any(high > gate)) {
-            const float h = fmaxf(high, __shfl_xor(high, 32)), more = h > gate ? ceilf(h - kUnit) : 0.0f;
-            by = gate == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);         // (1: there is nothing to scale yet)
-            gate = h > gate ? kLimit : gate;
-            top += more;
+        auto stage = [&](int t) {
+            stage_copy<KP, WAVES>(f.user_frag, t, buf[t & 1], wave, lane);
+            stage_copy<KP, WAVES>(f.user_frag_t, t, buf[t & 1] + kBytes, wave, lane);
+            stage_data(f.user_data + (size_t)t * kUserData, buf[t & 1] + 2 * kBytes, lane);
+            stage_data(f.user_data_t + (size_t)t * kUserData, buf[t & 1] + 2 * kBytes + kUserData * 4, lane);
+        };
+        // the tile's teacher entries: where they are is known two steps ahead (scalar loads), the first 64 are asked for one step ahead
+        const int bucket = block % kBuckets;
+        typedef const __attribute__((address_space(4))) int32_t *scalar_ptr;
+        auto bounds = [&](int t, int &begin, int &end) {
+            const scalar_ptr at = (scalar_ptr)(f.entry_at + (size_t)min(t, t1 - 1) * (kBuckets + 1) + bucket);
+            begin = at[0];
+            end = at[1];
+        };
+        auto entry_of = [&](int t, int begin) { return f.entry[(size_t)min(t, t1 - 1) * n32 + min(begin + lane, n32 - 1)]; };
+        int begin, end, begin1, end1;
+        bounds(t0, begin, end);
+        bounds(t0 + 1, begin1, end1);
+        uint2 next_entry = entry_of(t0, begin);
+        stage(t0);
+        for (int t = t0; t < t1; ++t) {
+            staged<0>();
+            const char *now = buf[t & 1];
+            const int from = begin, to = end;
+            uint2 entry = next_entry;
+            unsigned word[NC];
+            // (no instructions: what was asked for a step ago is here, and is taken before anything else is asked for)
+            asm volatile("" : "+v"(entry.x), "+v"(entry.y));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] -= more;
-        }
-        next = tile_scores<KP>(buf[(t + 1) & 1], lane, x);       // (behind the last tile: of what is left in LDS, and not used)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
-        // the teacher's share
-        bool any = false;
-        for (int k = from; k < to; k += 64) {
-            if (k > from) entry = k + lane < to ? f.entry[(size_t)t * n32 + k + lane] : make_uint2(0xffffffffu, 0);
-            const unsigned at = (entry.x >> 5) - base;
-            const bool hit = entry.x != 0xffffffffu && at < 32u;
-            if (hit) patch[at * kPatch + (entry.x & 31)] = __uint_as_float(entry.y);
-            any |= __any(hit);
-        }
-        if (any) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            f32x4 *cell = reinterpret_cast<f32x4 *>(patch + col * kPatch + 4 * half);
-            f32x4 p[4];
-            unsigned most = 0;                                   // (p is never negative: its bits order like its value)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                p[q] = cell[2 * q];
-                cell[2 * q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(p[q][k]));
-            }
-            const float log_p = __builtin_amdgcn_logf(__uint_as_float(most)) - (top + (e - kUnit));          // (-inf where there is none)
-            if (__any(log_p > gate)) {
-                const float h = fmaxf(log_p, __shfl_xor(log_p, 32)), more = h > gate ? ceilf(h - kUnit) : 0.0f;
-                const float by_p = gate == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] *= by_p;
-                by *= by_p;
-                gate = h > gate ? kLimit : gate;
-                top += more;
-            }
-            const float unit = fminf(__builtin_amdgcn_exp2f(kUnit - e - top), -kLowest);     // (finite where a column has no weight yet: 0 stays 0)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(p[q][k], -unit, s[4 * q + k]);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 coef = data[half + 2 * q];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) sum[k] = fmaf(s[4 * q + k], coef[k], sum[k]);
-        }
-        d_bias = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), scale, d_bias * by);
-        f16x8 p[2][2];
-        split_weights(s, p);
-        weighted_sum<KP>(buf_t[t & 1], lane, p, by, o);
-        finish(t + 1, next, next_high, next_e, next_scale);
-    };
-    f32x16 s0 = tile_scores<KP>(buf[t0 & 1], lane, x), s1;
-    float h0, h1, e0, e1, c0, c1;
-    finish(t0, s0, h0, e0, c0);
-    for (int t = t0; t < t1; t += 2) {
-        step(t, s0, h0, e0, c0, s1, h1, e1, c1);
-        if (t + 1 >= t1) break;
-        step(t + 1, s1, h1, e1, c1, s0, h0, e0, c0);
-    }
-    __syncthreads();                                             // the buffers are free for the next block
-    d_bias += __shfl_xor(d_bias, 32);
-    const float unit_of = __builtin_amdgcn_exp2f(top - kUnit);
-    const bool whole = t0 == 0 && t1 == f.user_tiles;
-    const int item = tile * 32 + col, K = f.a.n_factors;
-    if (whole && item < f.a.n_items) {
-        float *out = f.a.d_items + (size_t)item * K;
-        const bool vector = (K & 3) == 0 && ((uintptr_t)f.a.d_items & 15) == 0;
-        if (half == 0 && f.a.d_bias) f.a.d_bias[item] = d_bias * unit_of;
-#pragma unroll
-        for (int c = 0; c < Frag<KP>::cols; ++c)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int k = 32 * c + 8 * q + 4 * half;
-                const f32x4 v = f32x4{o[c][4 * q], o[c][4 * q + 1], o[c][4 * q + 2], o[c][4 * q + 3]} * unit_of;
-                if (vector) {
-                    if (k < K) *reinterpret_cast<f32x4 *>(out + k) = v;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (k + j < K) out[k + j] = v[j];
+            for (int n = 0; n < NC; ++n) {
+                word[n] = next_word[n];
+                if constexpr (MASK) {
+                    asm volatile("" : "+v"(word[n]));
+                    next_word[n] = mask_word(t + 1, n);
                 }
             }
-    } else if (!whole) {
-        const size_t at = ((size_t)(blockIdx.x + block) * WAVES + wave) * 32 + col;
-        if (half == 0) f.part_bias[at] = d_bias * unit_of;
+            begin = begin1;
+            end = end1;
+            bounds(t + 2, begin1, end1);
+            next_entry = entry_of(t + 1, begin);
+            if (t + 1 < t1) stage(t + 1);
+            f32x16 s[NC];
+            tile_scores<KP, NC>(now, lane, x, s);
+            const f32x4 *data = reinterpret_cast<const f32x4 *>(now + 2 * kBytes);
+            const f32x4 last = data[8];
+            const float e = last[1], scale = last[2];
+            float by[NC];
 #pragma unroll
-        for (int c = 0; c < Frag<KP>::cols; ++c)
+            for (int n = 0; n < NC; ++n) {
+                // the exponents of the weights, for `top` as it stands
+                const float unscaled = last[0] * unscale[n], shift = bias[n] - (top[n] + (e - kUnit));
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<f32x4 *>(f.part_items + at * KP + 32 * c + 8 * q + 4 * half) = f32x4{o[c][4 * q], o[c][4 * q + 1], o[c][4 * q + 2], o[c][4 * q + 3]} * unit_of;
-    }
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 lse = data[half + 2 * q];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unscaled, shift) - lse[k];
+                }
+                if constexpr (MASK) mask16_rows(s[n], word[n]);
+                const float high = largest16(s[n]);
+                by[n] = 1.0f;
+                if (__any(high > gate[n])) {
+                    const float h = fmaxf(high, __shfl_xor(high, 32)), more = h > gate[n] ? ceilf(h - kUnit) : 0.0f;
+                    by[n] = gate[n] == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);       // (1: there is nothing to scale yet)
+                    gate[n] = h > gate[n] ? kLimit : gate[n];
+                    top[n] += more;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][r] -= more;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r]);
+            }
+            // the teacher's share
+            unsigned any = 0;                                    // a bit per column tile that is hit
+            for (int k = from; k < to; k += 64) {
+                if (k > from) entry = entry_of(t, k);
+                const unsigned at = (entry.x >> 5) - base;
+                const bool hit = k + lane < to && at < 32u * NC;
+                if (hit) patch[at * kPatch + (entry.x & 31)] = __uint_as_float(entry.y);
+#pragma unroll
+                for (int n = 0; n < NC; ++n) any |= __any(hit && (at >> 5) == (unsigned)n) ? 1u << n : 0u;
+            }
+            if (any) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    if (!((any >> n) & 1u)) continue;
+                    f32x4 *cell = reinterpret_cast<f32x4 *>(patch + (n * 32 + col) * kPatch + 4 * half);
+                    f32x4 p[4];
+                    unsigned most = 0;                           // (p is never negative: its bits order like its value)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        p[q] = cell[2 * q];
+                        cell[2 * q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(p[q][k]));
+                    }
+                    const float log_p = __builtin_amdgcn_logf(__uint_as_float(most)) - (top[n] + (e - kUnit));       // (-inf where there is none)
+                    if (__any(log_p > gate[n])) {
+                        const float h = fmaxf(log_p, __shfl_xor(log_p, 32)), more = h > gate[n] ? ceilf(h - kUnit) : 0.0f;
+                        const float by_p = gate[n] == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[n][r] *= by_p;
+                        by[n] *= by_p;
+                        gate[n] = h > gate[n] ? kLimit : gate[n];
+                        top[n] += more;
+                    }
+                    const float unit = fminf(__builtin_amdgcn_exp2f(kUnit - e - top[n]), -kLowest);      // (finite where a column has no weight yet: 0 stays 0)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(p[q][k], -unit, s[n][4 * q + k]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+            f16x8 p[NC][2][2];
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 coef = data[kUserData / 4 + half + 2 * q];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sum[k] = fmaf(s[n][4 * q + k], coef[k], sum[k]);
+                }
+                d_bias[n] = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), scale, d_bias[n] * by[n]);
+                split_weights(s[n], p[n]);
+            }
+            weighted_sum<KP, NC>(now + kBytes, lane, p, by, o);
+        }
+        __syncthreads();                                         // the buffers are free for the next block
+        const bool whole = t0 == 0 && t1 == f.user_tiles, vector = (f.a.n_factors & 3) == 0 && ((uintptr_t)f.a.d_items & 15) == 0;
+        const int K = f.a.n_factors;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const float sum = d_bias[n] + __shfl_xor(d_bias[n], 32), unit_of = __builtin_amdgcn_exp2f(top[n] - kUnit);
+            const int item = (tile + n) * 32 + col;
+            if (whole && item < f.a.n_items) {
+                float *out = f.a.d_items + (size_t)item * K;
+                if (half == 0 && f.a.d_bias) f.a.d_bias[item] = sum * unit_of;
+#pragma unroll
+                for (int c = 0; c < Frag<KP>::cols; ++c)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int k = 32 * c + 8 * q + 4 * half;
+                        const f32x4 v = f32x4{o[n][c][4 * q], o[n][c][4 * q + 1], o[n][c][4 * q + 2], o[n][c][4 * q + 3]} * unit_of;
+                        if (vector) {
+                            if (k < K) *reinterpret_cast<f32x4 *>(out + k) = v;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (k + j < K) out[k + j] = v[j];
+                        }
+                    }
+            } else if (!whole) {
+                const size_t at = ((size_t)(blockIdx.x + block) * WAVES * NC + wave * NC + n) * 32 + col;
+                if (half == 0) f.part_bias[at] = sum * unit_of;
+#pragma unroll
+                for (int c = 0; c < Frag<KP>::cols; ++c)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<f32x4 *>(f.part_items + at * KP + 32 * c + 8 * q + 4 * half) = f32x4{o[n][c][4 * q], o[n][c][4 * q + 1], o[n][c][4 * q + 2], o[n][c][4 * q + 3]} * unit_of;
+            }
+        }
     }
 }
 
 // One workgroup per tile of items: the parts of a block that was cut, in the order of its user tiles.
-template <int KP, int WAVES>
-__global__ void __launch_bounds__(256) join_items_kernel(const FusedArgs f) {
-    const int block = (int)blockIdx.x / WAVES, in_block = (int)blockIdx.x % WAVES * 32, K = f.a.n_factors;
+template <int KP>
+__global__ void __launch_bounds__(256) join_items_kernel(const FusedArgs f, int tiles) {
+    const int block = (int)blockIdx.x / tiles, in_block = (int)blockIdx.x % tiles * 32, K = f.a.n_factors;
     const int first = (int)((long long)block * f.user_tiles / f.units), last = (int)(((long long)(block + 1) * f.user_tiles - 1) / f.units);
     if (first == last) return;
-    const int i0 = block * WAVES * 32 + in_block;
+    const int i0 = block * tiles * 32 + in_block;
     for (int e = threadIdx.x; e < 32 * KP / 4; e += 256) {
         const int row = e / (KP / 4), k = e % (KP / 4) * 4;
         if (i0 + row >= f.a.n_items || k >= K) continue;
         f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int g = first; g <= last; ++g) s += *reinterpret_cast<const f32x4 *>(f.part_items + ((size_t)(g + block) * WAVES * 32 + in_block + row) * KP + k);
+        for (int g = first; g <= last; ++g) s += *reinterpret_cast<const f32x4 *>(f.part_items + ((size_t)(g + block) * tiles * 32 + in_block + row) * KP + k);
         float *out = f.a.d_items + (size_t)(i0 + row) * K + k;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -718,7 +771,7 @@ __global__ void __launch_bounds__(256) join_items_kernel(const FusedArgs f) {
     }
     if (!f.a.d_bias || threadIdx.x >= 32 || i0 + (int)threadIdx.x >= f.a.n_items) return;
     float s = 0.0f;
-    for (int g = first; g <= last; ++g) s += f.part_bias[(size_t)(g + block) * WAVES * 32 + in_block + threadIdx.x];
+    for (int g = first; g <= last; ++g) s += f.part_bias[(size_t)(g + block) * tiles * 32 + in_block + threadIdx.x];
     f.a.d_bias[i0 + threadIdx.x] = s;
 }
 

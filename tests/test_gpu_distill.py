@@ -259,3 +259,70 @@ def test_many_entries_in_one_tile_and_items_twice():
     got = distill_gradients(*args, row_weight=torch.from_numpy(p.g).cuda(), **kw)
     for g, w, t in zip(got, want, tol):
         assert (np.abs(g.cpu().numpy() - w) <= t).all()
+
+
+@pytest.mark.parametrize("factors", [20, 50, 100, 200])
+def test_masked_items_may_hold_anything(factors):
+    """an item that a row's mask takes out reaches neither the row's loss nor its gradient, and the row does not reach the item's.  (Not the bits of a clean
+    call: the power of two that a tile of 32 items is scaled by is that of its largest finite factor, masked or not, and what is below the 22 bits of a
+    weight's two parts is cut elsewhere.  The bounds are those above.)"""
+    p = Problem(rows=70, items=400, factors=factors, n=6, mask="one", seed=13)
+    p.ti = np.abs(p.ti) % 400
+    p.mask[0, [0, 17, 64, 399]] = False
+    args, kw = p.given()
+    want, tol = p.exact()
+    weight = torch.from_numpy(p.g).cuda()
+    v = args[1].clone()
+    v[0], v[17], v[64, 3], v[399] = NAN, INF, -INF, NAN
+    got = distill_gradients(args[0], v, *args[2:], row_weight=weight, **kw)
+    for x, w, t in zip((*got, distill_loss(args[0], v, *args[2:], **kw)), (*want, want[0]), (*tol, tol[0])):
+        assert (np.abs(x.cpu().numpy() - w) <= t).all()
+    u = args[0].clone()
+    u[5, 1], u[40] = NAN, INF
+    got = distill_gradients(u, *args[1:], **kw)
+    off = torch.from_numpy(~p.mask[0]).cuda()
+    assert torch.isnan(got.loss[[5, 40]]).all() and torch.isnan(got.users[[5, 40]]).all()
+    assert (got.items[off] == 0).all() and (got.bias[off] == 0).all() and torch.isnan(got.items[~off]).all() and torch.isnan(got.bias[~off]).all()
+
+
+@pytest.mark.parametrize("rows,items,factors,n,given", [(4129, 32_801, 20, 9, True), (1030, 129_037, 64, 40, True), (4500, 30_001, 33, 6, False)], ids=["long", "wide", "plain"])
+def test_large_problems(rows, items, factors, n, given):
+    """more than 2^17 pairs of tiles of 32 rows and 32 items: wavefronts with two column tiles each.  The reference is the formula in float64 on the device"""
+    tau = 1.5
+    p = Problem(rows, items, factors, n, tau=tau, weight=given, bias=given, seed=factors)
+    args, kw = p.given()
+    dev = lambda a: torch.from_numpy(a).cuda().double()                           # noqa: E731
+    u, v = dev(p.u), dev(p.v)
+    b, g = dev(p.b) if given else torch.zeros(items, dtype=torch.float64, device="cuda"), dev(p.g) if given else torch.ones(rows, dtype=torch.float64, device="cuda")
+    z = (u @ v.T + b) / tau
+    lse = torch.logsumexp(z, 1)
+    ti, t = args[3].long(), args[4].double() / tau
+    ok = (ti >= 0) & (ti < items) & (t > -INF)
+    live = ok.any(1)
+    log_p = torch.where(ok, t, -INF)
+    log_p = torch.where(ok, log_p - torch.logsumexp(torch.where(live[:, None], log_p, 0.0), 1, keepdim=True), 0.0)
+    share = torch.where(ok, log_p.exp(), 0.0)
+    at = torch.where(ok, z.gather(1, ti.clamp(0, items - 1)), 0.0)
+    loss = torch.where(live, tau * tau * (share * (log_p - at + lse[:, None])).sum(1), 0.0)
+    big = float((log_p.abs().amax(1) + at.abs().amax(1) + lse.abs()).max().clamp(min=1.0))
+    s = float((u.abs() @ v.abs().T + b.abs()).max())
+    coef = (tau * g * live)[:, None]
+    q = (z - lse[:, None]).exp_()
+    q *= coef
+    teacher = torch.zeros_like(q).scatter_add_(1, ti.clamp(0, items - 1), share * coef)
+    dz, pq = q - teacher, q + teacher
+    ez = (factors + 6) * E * s / tau
+    eq, ep = 2 * ez + (items / 32 + 80) * E, (n + 80 + 8 * float(np.abs(np.where(np.isinf(p.t), 0, p.t)).max()) / tau) * E
+    rel_i, rel_r = eq + ep + (items + 64) * E, eq + ep + (rows + 64) * E
+    got = distill_gradients(*args, row_weight=torch.from_numpy(p.g).cuda() if given else None, **kw)
+    alone = distill_loss(*args, **kw)
+    tol = tau * tau * (2 * ez + eq + ep + (n + 80) * E * big)
+    for name, x, want, t in (("loss", alone, loss, tol), ("loss", got.loss, loss, tol), ("users", got.users, dz @ v, rel_i * (pq @ v.abs()) + 1e-30),
+                             ("items", got.items, dz.T @ u, rel_r * (pq.T @ u.abs()) + 1e-30), ("bias", got.bias, dz.sum(0), rel_r * pq.sum(0) + 1e-30)):
+        if x is None:
+            assert name == "bias" and not given
+            continue
+        off = float(((x.double() - want).abs() / t).max())
+        assert off <= 1, (name, off)
+    again = distill_gradients(*args, row_weight=torch.from_numpy(p.g).cuda() if given else None, **kw)
+    assert all(torch.equal(x, y) for x, y in zip(got, again) if x is not None)
