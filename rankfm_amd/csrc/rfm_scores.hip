@@ -150,8 +150,7 @@ __device__ __forceinline__ float listed_score(const rfm_score_rules &u, const Ro
 }
 
 template <typename T, int P, bool LISTS>
-__device__ __forceinline__ void apply_rules(const rfm_score_rules &u, const RowRules &w, int first, int n_items, const int *count, const int *last, float *s,
-                                            unsigned done = 0) {
+__device__ __forceinline__ void apply_rules(const rfm_score_rules &u, const RowRules &w, int first, int n_items, const int *count, const int *last, float *s) {
     constexpr int ve = Vec<T>::n;
 #pragma unroll
     for (int j = 0; j < P / ve; ++j) {
@@ -179,72 +178,77 @@ __device__ __forceinline__ void apply_rules(const rfm_score_rules &u, const RowR
             if constexpr (LISTS) {
                 if (i + k < n_items) x = listed_score(u, w, i + k, count[at + k], last[at + k], x);
             } else {
-                if (u.item_bias) x = (done >> (j * ve + k)) & 1u ? x : x + bias[k];
+                if (u.item_bias) x = x + bias[k];
             }
             s[j * ve + k] = (bits >> k) & 1u ? x : -INFINITY;
         }
     }
 }
 
-constexpr int kHits = 64;                        // list entries of a tile that are looked through one by one
+constexpr int kHits = kThreads;                  // list entries of a tile that are looked at by a thread each
 constexpr int kCounted = 2048;                   // items whose counts are in LDS at a time, where there are more
 struct Hits {
-    int n, item[kHits], entry[kHits];            // entry: 0 of the history, else 1 + the position of the bias
+    int n;
+    int2 at[kHits];                              // item; 0 for an entry of the history, else 1 + the position of the bias
 };
 struct Counted {
     int count[kCounted], last[kCounted];
 };
 
 // One workgroup per (row, tile of 256 P items): the row is read and written once, which is the floor.  The scores are asked for before the lists:
-// their way through three dependent loads passes meanwhile.  A tile's few list entries are gathered in LDS and looked through by the thread that
-// holds their item; where there are more than 64, counts per item are made, 2048 items at a time.
+// their way through three dependent loads passes meanwhile.  A tile's few list entries are gathered in LDS; a thread each counts those of its item, makes
+// that item's score and writes it over what the row's pass left there (read before anything of the tile is written: `out` may be `scores`).  Where
+// there are more than 256, counts per item are made, 2048 items at a time.
 template <typename T, int P>
-__global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score_rules u, long long row0, int tiles, int n_items, const T *__restrict__ scores,
+__global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score_rules u, long long row0, int tiles, int n_items, const T *scores,
                                                                  long long stride, T *out, long long out_stride) {
     __shared__ union { Hits hits; Counted counted; } lists;
     const long long r = row0 + blockIdx.x / tiles;
     const int first = (int)(blockIdx.x % tiles) * P * kThreads;
     if (threadIdx.x == 0) lists.hits.n = 0;
-    float s[P];
+    float s[P], value = 0.0f;
+    int hits = 0, mine = -1;                                     // the item that the lists name and this thread sees to, and what becomes of its score
     load_tile<T, P>(scores + r * stride, first, n_items, s);
     const RowRules w = row_rules(u, r, n_items);
     if (w.bad) {
 #pragma unroll
         for (int k = 0; k < P; ++k) s[k] = __uint_as_float(0x7fc00000u);
     } else {
-        unsigned done = 0;                                       // the scores that the lists name: theirs are made here
         bool many = false;
         if (w.hist_n > 0 || w.bias_n > 0) {
             __syncthreads();
             auto note = [&](int item, int entry) {
-                if ((unsigned)(item - first) >= (unsigned)(P * kThreads)) return;
+                if ((unsigned)(item - first) >= (unsigned)(P * kThreads) || item >= n_items) return;
                 const int at = atomicAdd(&lists.hits.n, 1);
-                if (at < kHits) { lists.hits.item[at] = item; lists.hits.entry[at] = entry; }
+                if (at < kHits) lists.hits.at[at] = make_int2(item, entry);
             };
             for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) note(w.hist[k], 0);
             for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) note(w.bias_item[k], (int)k + 1);
             __syncthreads();
-            const int n = lists.hits.n;
-            many = n > kHits;
-            constexpr int ve = Vec<T>::n;
-            for (int h = 0; h < n && !many; ++h) {
-                const int item = lists.hits.item[h], vec = (item - first) / ve;
-                if (vec % kThreads != (int)threadIdx.x || item >= n_items) continue;
-                const int slot = vec / kThreads * ve + (item - first) % ve;
-                if ((done >> slot) & 1u) continue;
+            hits = lists.hits.n;
+            many = hits > kHits;
+            if (!many && (int)threadIdx.x < hits) {
+                const int item = lists.hits.at[threadIdx.x].x;
                 int c = 0, l = 0;
-                for (int k = h; k < n; ++k)
-                    if (lists.hits.item[k] == item) {
-                        c += lists.hits.entry[k] == 0;
-                        l = max(l, lists.hits.entry[k]);
-                    }
-                const float x = listed_score(u, w, item, c, l, pick<P>(*reinterpret_cast<const float (*)[P]>(s), slot));
-#pragma unroll
-                for (int k = 0; k < P; ++k) s[k] = k == slot ? x : s[k];
-                done |= 1u << slot;
+                bool before = false;                             // an earlier entry names the item: that thread sees to it
+#pragma unroll 4
+                for (int k = 0; k < hits; ++k) {
+                    const int2 e = lists.hits.at[k];
+                    const bool same = e.x == item;
+                    before |= same && k < (int)threadIdx.x;
+                    c += same && e.y == 0;
+                    l = same ? max(l, e.y) : l;
+                }
+                if (!before) {
+                    mine = item;
+                    value = (float)scores[r * stride + item];
+                    value = !w.mask || ((w.mask[item >> 5] >> (item & 31)) & 1u) ? listed_score(u, w, item, c, l, value) : -INFINITY;
+                }
             }
+            asm volatile("" : "+v"(value));                      // (no instruction: it is read by now)
+            __syncthreads();                                     // `out` may be `scores`: no store before these reads
         }
-        if (!many) apply_rules<T, P, false>(u, w, first, n_items, nullptr, nullptr, s, done);
+        if (!many) apply_rules<T, P, false>(u, w, first, n_items, nullptr, nullptr, s);
         else {
             constexpr int per = kCounted / kThreads;             // (tiles of P scores per thread lie in tiles of `per`: vectors of a tile come in order)
 #pragma unroll
@@ -268,6 +272,10 @@ __global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score
             for (int k = 0; k < ve; ++k)
                 if (i + k < n_items) o[i + k] = (T)s[j * ve + k];
         }
+    }
+    if (hits > 0) {                                              // (the same for all; none with counts)
+        __syncthreads();                                         // behind the row's own stores
+        if (mine >= 0) o[mine] = (T)value;
     }
 }
 
@@ -297,23 +305,66 @@ template <bool RULED> struct Top {
 constexpr int kSlots = 1024, kShort = 512;       // hash slots for the items that a row's lists name; lists of more entries than kShort are scanned per tile
 constexpr int kWindow = 65536;                   // items whose membership bits are in LDS at a time
 
-// descending bitonic sort of buf[0 .. p2) by `threads` threads, p2 a power of two.  The 64 pairs of a wavefront lie in 128 keys as long as the
-// distance is at most 64: such steps follow each other without a barrier (a wavefront's LDS operations run in order).
-template <bool BLOCK>
-__device__ __forceinline__ void sort_keys(u64 *buf, int p2, int thread) {
-    constexpr int threads = BLOCK ? kThreads : 64;
+// Descending bitonic sort of the `m` keys of a wavefront's buffer, in its registers: key r * 64 + lane is the r-th of its lane, so distances of 64 and
+// more stay inside a lane and shorter ones are a shuffle; nothing waits for another wavefront.
+template <int R>
+__device__ __forceinline__ void sort_in_registers(u64 *buf, int m, int lane) {
+    u64 x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = r * 64 + lane < m ? buf[r * 64 + lane] : 0;
+#pragma unroll 1
+    for (int k = 2; k <= 64 * R; k <<= 1) {
+#pragma unroll
+        for (int d = R / 2; d > 0; d >>= 1) {
+            if (d * 128 > k) continue;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (r & d) continue;
+                const u64 a = x[r], b = x[r | d];
+                const bool swap = (a < b) == ((r * 64 & k) == 0);
+                x[r] = swap ? b : a;
+                x[r | d] = swap ? a : b;
+            }
+        }
+#pragma unroll 1
+        for (int j = min(k / 2, 32); j > 0; j >>= 1) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const u64 other = __shfl_xor(x[r], j);
+                const bool larger = (((r * 64 + lane) & k) == 0) == ((lane & j) == 0);
+                x[r] = (other > x[r]) == larger ? other : x[r];
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) buf[r * 64 + lane] = x[r];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// The same in LDS, for any number that the buffer holds (padded to a power of two): twice the time, and no registers
+__device__ __forceinline__ void sort_in_place(u64 *buf, int m, int lane) {
+    int p2 = 2;
+    while (p2 < m) p2 <<= 1;
+    for (int k = m + lane; k < p2; k += 64) buf[k] = 0;
     for (int k = 2; k <= p2; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            if (BLOCK && (j > 64 || (j == 64 && k > 128) || k == 2)) __syncthreads();
-            for (int t = thread; t < p2 / 2; t += threads) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            for (int t = lane; t < p2 / 2; t += 64) {
                 const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1)), l = i + j;
                 const u64 a = buf[i], b = buf[l];
                 if ((a < b) == ((i & k) == 0)) { buf[i] = b; buf[l] = a; }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
         }
-    if (BLOCK) __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+__device__ __forceinline__ void sort_keys(u64 *buf, int m, int lane) {
+    if (m <= 64) sort_in_registers<1>(buf, m, lane);
+    else if (m <= 128) sort_in_registers<2>(buf, m, lane);
+    else if (m <= 256) sort_in_registers<4>(buf, m, lane);
+    else if (m <= 512) sort_in_registers<8>(buf, m, lane);
+    else sort_in_place(buf, m, lane);
 }
 
 // what a row's lists name, when they are short: a hash table of the items with their counts and last bias entries, and a bit per item of a window
@@ -364,9 +415,9 @@ __device__ __forceinline__ void window_bits(Listed &m, int first) {
 // One workgroup per (row, segment of the row): ONE pass over the scores.  Scores at or above the running threshold become keys in the wavefront's
 // own part of LDS -- no barrier in the loop; when it is full, it is sorted and the threshold becomes the n-th best.  The first threshold comes
 // from the first 8192 scores (4096 under rules): each group of eight holds its maximum in a register, a wavefront finds by bisection over ballots the
-// value that ceil(n / 4) of its group maxima reach, and the least of the four wavefronts' values is reached by at least n scores.  So the final
-// sort sees a few times n keys, not the row.  Under rules, items that the row's lists name are left out of the pass (a bit per item in LDS) and
-// looked at by themselves afterwards.  FROM_KEYS: the "scores" are the sorted keys that the segments of a row left behind.
+// value that its share of n of its group maxima reach, and the least of the four wavefronts' values is reached by at least n scores.  So the final
+// sort sees a few times n keys, not the row (1837 rows of 640 items, the best two: 60 us when the empty wavefronts leave it none, 16 with it).  Under
+// rules, items that the row's lists name are left out of the pass (a bit per item in LDS) and looked at by themselves afterwards.  FROM_KEYS: the "scores" are the sorted keys that the segments of a row left behind.
 template <typename T, bool RULED, bool FROM_KEYS>
 __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score_rules u, long long row0, int segments, int segment, int n_items,
                                                               const T *__restrict__ scores, long long stride, const u64 *__restrict__ keys_in, int n_keys,
@@ -401,12 +452,7 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
             const unsigned long long who = __ballot(pass);
             if (!who) return;
             if (m > kBuf - 64) {
-                int p2 = 2;
-                while (p2 < m) p2 <<= 1;
-                for (int k = m + lane; k < p2; k += 64) mine[k] = 0;
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                sort_keys<false>(mine, p2, lane);
+                sort_in_place(mine, m, lane);
                 m = want;                                        // (m > kBuf - 64 >= want)
                 thr = max(thr, mine[want - 1]);
                 reach = key_score(thr);
@@ -475,11 +521,21 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
                     for (int k = 0; k < kPer; ++k) high = fmaxf(high, base == 0 || x[q * kPer + k] < taken ? x[q * kPer + k] : -INFINITY);
                     g[q] = score_key(high);
                 }
-                const int need = (want + kWaves - 1) / kWaves;
-                if (need <= 32) {                                // few are wanted: one group per lane
+                // Every wavefront's share of the wanted is that of the groups it holds scores of: the vectors of a short row do not reach them all.
+                const int vectors = (min(end - t0, kSuper * kTile) + ve - 1) / ve;
+                int groups = min(max(vectors - wave * 64, 0), 64), of = min(vectors, kThreads);
+                if (2 * want <= of) {                            // few are wanted: one group per lane
 #pragma unroll
                     for (int q = 1; q < kSuper; ++q) { g[0] = max(g[0], g[q]); g[q] = 0; }
+                } else {
+#pragma unroll
+                    for (int q = 1; q < kSuper; ++q) {
+                        const int left = vectors - q * (kPer / ve) * kThreads;
+                        groups += min(max(left - wave * 64, 0), 64);
+                        of += min(max(left, 0), kThreads);
+                    }
                 }
+                const int need = (want * groups + of - 1) / of;
                 unsigned t = 0;
                 for (int bit = 31; bit >= 12; --bit) {             // (cut to 20 bits: a little below the exact value)
                     const unsigned c = t | (1u << bit);
@@ -522,56 +578,62 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
                 }
             }
         }
-        // The candidates in order: put side by side and sorted.  Where rows are few and one workgroup's way to the end is what counts, up to 256 of them
-        // are placed by counting instead -- a key's place is the number of larger ones (keys are unique): no barriers, but the square of the work
-        // (one row of 200 k: 23.5 -> 17.6 us; at 4096 rows of 50 k it would be 196 -> 309).
+        // The candidates in order.  Few are placed by counting: a key's place is the number of larger ones (keys are unique).  Otherwise every wavefront
+        // sorts its own, and a key's place is its place there and the number of larger keys of the other three, each found by bisection.  (Sorting all
+        // of them together takes a barrier for each of its steps: 4096 rows of 50 k, 64 wanted, 194 -> 165 us.)  Counting is the square of the work; 256
+        // are few where rows are and one workgroup's way to the end is what counts.
         if (lane == 0) wave_m[wave] = m;
         if (threadIdx.x == 0) last_key = 0;
         __syncthreads();
-        int total = 0, at = 0;
+        int count[kWaves - 1], most = 0, total = m;              // of the other wavefronts
+        const u64 *other[kWaves - 1];
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-            at = k == wave ? total : at;
-            total += wave_m[k];
+        for (int v = 0; v < kWaves - 1; ++v) {
+            const int who = __builtin_amdgcn_readfirstlane((wave + 1 + v) & (kWaves - 1));
+            other[v] = buf + who * kBuf;
+            count[v] = __builtin_amdgcn_readfirstlane(wave_m[who]);
+            total += count[v];
+            most = max(most, count[v]);
         }
         const int got = total < want ? total : want;
         const size_t row_out = FROM_KEYS || segments == 1 ? (size_t)r * n : ((size_t)(r - row0) * segments + seg) * n;
         auto put = [&](int place, u64 key) {
+            if (place == want - 1) last_key = key;
             if (!FROM_KEYS && segments > 1) keys_out[row_out + base + place] = key;
             else {
                 items[row_out + base + place] = key ? key_item(key) : -1;
                 values[row_out + base + place] = key ? key_score(key) : -INFINITY;
             }
         };
-        if ((FROM_KEYS || segments > 1) && total <= 256) {
+        if (total <= (FROM_KEYS || segments > 1 ? 256 : 64)) {
             for (int k = lane; k < m; k += 64) {
                 const u64 key = mine[k];
                 int place = 0;
-#pragma unroll
-                for (int v = 0; v < kWaves; ++v) {
-                    const u64 *other = buf + v * kBuf;
-                    const int count = wave_m[v];
 #pragma unroll 4
-                    for (int q = 0; q < count; ++q) place += other[q] > key;
-                }
+                for (int q = 0; q < m; ++q) place += mine[q] > key;
+#pragma unroll
+                for (int v = 0; v < kWaves - 1; ++v)
+#pragma unroll 4
+                    for (int q = 0; q < count[v]; ++q) place += other[v][q] > key;
                 if (place < want) put(place, key);
-                if (place == want - 1) last_key = key;
             }
         } else {
-            u64 held[kBuf / 64];
-#pragma unroll
-            for (int k = 0; k < kBuf / 64; ++k)
-                if (k * 64 < m) held[k] = mine[k * 64 + lane];   // (what is read behind m is not written)
+            if (m > 1) sort_keys(mine, m, lane);
             __syncthreads();
+            for (int k = lane; k < min(m, want); k += 64) {
+                const u64 key = mine[k];
+                int above[kWaves - 1] = {0};
+                for (int step = most > 0 ? 1 << (31 - __clz(most)) : 0; step > 0; step >>= 1)
 #pragma unroll
-            for (int k = 0; k < kBuf / 64; ++k)
-                if (k * 64 + lane < m) buf[at + k * 64 + lane] = held[k];
-            int p2 = 2;
-            while (p2 < total) p2 <<= 1;
-            for (int k = total + threadIdx.x; k < p2; k += kThreads) buf[k] = 0;
-            sort_keys<true>(buf, p2, threadIdx.x);
-            for (int k = threadIdx.x; k < got; k += kThreads) put(k, buf[k]);
-            if (threadIdx.x == 0 && got == want) last_key = buf[want - 1];
+                    for (int v = 0; v < kWaves - 1; ++v) {
+                        const int next = above[v] + step;
+                        above[v] = next <= count[v] && other[v][next - 1] > key ? next : above[v];
+                    }
+                int place = k;
+#pragma unroll
+                for (int v = 0; v < kWaves - 1; ++v) place += above[v];
+                if (place < want) put(place, key);
+            }
         }
         for (int k = got + threadIdx.x; k < want; k += kThreads) put(k, 0);
         __syncthreads();

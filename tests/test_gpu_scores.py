@@ -237,6 +237,17 @@ def test_top_scores_of_half_width_rows(dtype):
     assert np.array_equal(got.items.cpu().numpy(), want_items) and np.array_equal(got.scores.cpu().numpy(), want_values)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows, items, n", [(700, 3, 1), (700, 5, 4), (700, 130, 128), (700, 655, 2), (700, 655, 600), (600, 900, 100), (6, 3204, 365), (6, 3204, 3), (3, 17_421, 3),
+                                            (3, 17_421, 500), (2, 1030, 1029)])
+def test_short_rows_and_short_ends(rows, items, n, dtype):
+    """rows, or last segments of rows, whose vectors do not reach every wavefront"""
+    s = torch.from_numpy(np.random.default_rng(items + n).standard_normal((rows, items)).astype(np.float32)).to(dtype)
+    got = top_scores(s.cuda(), n)
+    want_items, want_values = plain_top(s.float().numpy(), n)
+    assert np.array_equal(got.items.cpu().numpy(), want_items) and np.array_equal(got.scores.cpu().numpy(), want_values)
+
+
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%dx%d" % (s["rows"], s["items"]))
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_top_scores_under_rules_are_those_of_the_adjusted_rows(shape, dtype):
