@@ -62,8 +62,8 @@ __device__ __forceinline__ Four load_four(const float *row, int k, int factors) 
 // One wavefront per row: the teacher's distribution over the usable entries, and its part of the loss.
 //   part[r] = sum_j p_j (log p_j - z[r, t_j] / tau)     mass[r] = 1, 0 without a usable entry, NaN where the row's mask does not exist
 // For the gradients the list is left with the usable entries' p (-1, 0 elsewhere).  MERGE: merged too -- an item's first entry holds the sum of
-// its entries' p, the others are off, so that no two entries of a row meet in one element of dz.  ACC > 0 (quarters of 64 factors, rounded up):
-// acc [rows, kp] = sum_j p_j items[t_j].  s_dyn: per wavefront ids [n] and p [n].  No barrier: a wavefront works by itself.
+// its entries' p, the others are off, so that no two entries of a row meet in one element of dz.  ACC > 0: 64 ACC factors at most, in registers;
+// acc [rows, kp] = sum_j p_j items[t_j] where it is asked for.  s_dyn: per wavefront ids [n] and p [n].  No barrier: a wavefront works by itself.
 template <bool MERGE, int ACC>
 __device__ void teacher_row(const rfm_distill_args &a, long long r, int kp, int *s_dyn, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ merged_item,
                             float *__restrict__ merged_p, float *__restrict__ acc_out) {
@@ -97,90 +97,110 @@ __device__ void teacher_row(const rfm_distill_args &a, long long r, int kp, int 
     }
     sum = wave_sum(sum);
     const float log_sum = logf(sum), inv = 1.0f / sum;
+    // sum_j p_j (log p_j - bias / tau) here, the products of factors below: sum_j p_j < u, v_j > = < u, sum_j p_j v_j >
+    float acc = 0.0f;
+    for (int j = lane; j < n; j += 64) {
+        const float e = pr[j];
+        const int i = id[j];
+        if (!(e == 0.0f)) acc += e * inv * ((ts[j] - top) * inv_tau - log_sum - (a.bias ? a.bias[i] * inv_tau : 0.0f));
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    // the student's scores of the entries: 16 lanes per entry, two entries of each group of lanes at a time so that their loads overlap
+    // 16 lanes per entry, the loads of several entries of each group of lanes in flight
     const float *u = a.users + (size_t)r * a.user_stride;
     const int sub = lane & 15, grp = lane >> 4;
-    float acc = 0.0f;
-    Four mine[ACC > 0 ? ACC : 1], wsum[ACC > 0 ? ACC : 1];
+    float dot = 0.0f;
     if constexpr (ACC > 0) {
+        constexpr int AHEAD = ACC == 1 ? 8 : 5;
+        Four mine[ACC], wsum[ACC];
 #pragma unroll
         for (int q = 0; q < ACC; ++q) {
             mine[q] = load_four(u, 64 * q + 4 * sub, a.n_factors);
             wsum[q] = Four{{0.0f, 0.0f, 0.0f, 0.0f}};
         }
-    }
-    for (int j0 = 0; j0 < n; j0 += 8) {
-        float d[2] = {0.0f, 0.0f};
-        int item[2];
+        for (int j0 = 0; j0 < n; j0 += 4 * AHEAD) {
+            Four x[AHEAD][ACC];
+            float e[AHEAD];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int j = j0 + 4 * h + grp;
-            item[h] = j < n ? id[j] : -1;
-            if (item[h] < 0) continue;
-            const float *v = a.items + (size_t)item[h] * a.item_stride;
-            if constexpr (ACC > 0) {
-                const float e = pr[j];
+            for (int h = 0; h < AHEAD; ++h) {
+                const int j = j0 + 4 * h + grp, item = j < n ? id[j] : -1;
+                e[h] = item >= 0 ? pr[j] : 0.0f;
 #pragma unroll
                 for (int q = 0; q < ACC; ++q) {
-                    const Four x = load_four(v, 64 * q + 4 * sub, a.n_factors);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        d[h] = fmaf(mine[q].v[k], x.v[k], d[h]);
-                        wsum[q].v[k] = fmaf(e, x.v[k], wsum[q].v[k]);
-                    }
-                }
-            } else {
-                for (int f = 4 * sub; f < a.n_factors; f += 64) {
-                    const Four x = load_four(v, f, a.n_factors), y = load_four(u, f, a.n_factors);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) d[h] = fmaf(y.v[k], x.v[k], d[h]);
+                    x[h][q] = Four{{0.0f, 0.0f, 0.0f, 0.0f}};
+                    if (item >= 0) x[h][q] = load_four(a.items + (size_t)item * a.item_stride, 64 * q + 4 * sub, a.n_factors);
                 }
             }
-        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < AHEAD; ++h)
 #pragma unroll
-            for (int m = 8; m > 0; m >>= 1) d[h] += __shfl_xor(d[h], m);
-            if (item[h] >= 0 && sub == 0) {
-                const int j = j0 + 4 * h + grp;
-                const float e = pr[j], z = d[h] + (a.bias ? a.bias[item[h]] : 0.0f);
-                if (!(e == 0.0f)) acc += e * inv * ((ts[j] - top) * inv_tau - log_sum - z * inv_tau);
-            }
+                for (int q = 0; q < ACC; ++q)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) wsum[q].v[k] = fmaf(e[h], x[h][q].v[k], wsum[q].v[k]);
         }
-    }
-    acc = wave_sum(acc);
-    if (lane == 0) {
-        part[r] = some ? acc : 0.0f;
-        mass[r] = bad ? __uint_as_float(0x7fc00000u) : some ? 1.0f : 0.0f;
-    }
-    if constexpr (ACC > 0) {
 #pragma unroll
         for (int q = 0; q < ACC; ++q)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
+                dot = fmaf(mine[q].v[k], wsum[q].v[k], dot);
                 float x = wsum[q].v[k];
                 x += __shfl_xor(x, 16);
                 x += __shfl_xor(x, 32);
                 const int at = 64 * q + 4 * sub + k;
-                if (grp == 0 && at < kp) acc_out[(size_t)r * kp + at] = some ? x * inv : 0.0f;
+                if (acc_out && grp == 0 && at < kp) acc_out[(size_t)r * kp + at] = some ? x * inv : 0.0f;
             }
+    } else {
+        for (int j = grp; j < n; j += 4) {
+            const int item = id[j];
+            if (item < 0) continue;
+            float d = 0.0f;
+            for (int f = 4 * sub; f < a.n_factors; f += 64) {
+                const Four x = load_four(a.items + (size_t)item * a.item_stride, f, a.n_factors), y = load_four(u, f, a.n_factors);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d = fmaf(y.v[k], x.v[k], d);
+            }
+            dot = fmaf(pr[j], d, dot);
+        }
+    }
+    acc = wave_sum(acc) - wave_sum(dot) * inv * inv_tau;
+    if (lane == 0) {
+        part[r] = some ? acc : 0.0f;
+        mass[r] = bad ? __uint_as_float(0x7fc00000u) : some ? 1.0f : 0.0f;
     }
     if (!merged_item) return;
-    for (int j = lane; j < n; j += 64) {
-        int i = id[j];
-        float p = i >= 0 ? pr[j] * inv : 0.0f;
-        if (MERGE && i >= 0) {
-            bool first = true;
-            for (int k = 0; k < j; ++k) first &= id[k] != i;
-            if (first) {
-                for (int k = j + 1; k < n; ++k)
-                    if (id[k] == i) p += pr[k] * inv;
-            } else { i = -1; p = 0.0f; }
+    for (int j0 = 0; j0 < n; j0 += 256) {                        // four entries per lane against all of them
+        int i[4];
+        float p[4];
+        bool first[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int j = j0 + 64 * q + lane;
+            i[q] = j < n ? id[j] : -1;
+            p[q] = MERGE || i[q] < 0 ? 0.0f : pr[j];
+            first[q] = true;
         }
-        merged_item[(size_t)r * n + j] = bad ? -1 : i;
-        merged_p[(size_t)r * n + j] = p;
+        if constexpr (MERGE) {
+#pragma unroll 4
+            for (int k = 0; k < n; ++k) {
+                const int at = id[k];
+                const float more = pr[k];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const bool twin = at == i[q];
+                    first[q] &= !twin || k >= j0 + 64 * q + lane;
+                    p[q] += twin ? more : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int j = j0 + 64 * q + lane;
+            const bool on = i[q] >= 0 && first[q] && !bad;
+            if (j < n) {
+                merged_item[(size_t)r * n + j] = on ? i[q] : -1;
+                merged_p[(size_t)r * n + j] = on ? p[q] * inv : 0.0f;
+            }
+        }
     }
 }
 __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ merged_item,

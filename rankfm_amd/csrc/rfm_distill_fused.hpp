@@ -90,21 +90,33 @@ __device__ __forceinline__ float block_max(float x, float *s_max) {
 // multiply, so does a factor that is not finite: where it counts the score and with it the row's sum is NaN already, where a mask has taken it out its
 // weight is 0.
 template <int KP>
-__device__ void write_frags(const float *__restrict__ x, long long stride, int tile, long long rows, int factors, float by, const float *__restrict__ live,
-                            const float *__restrict__ weight, float all_weight, char *frag, char *frag_t, float *lds, float *s_max, int *e_out, int *e_t_out) {
+__device__ void write_frags(const float *__restrict__ x, long long stride, int tile, long long rows, int factors, float by, const float *live,
+                            const float *__restrict__ weight, float all_weight, char *frag, char *frag_t, float *lds, float *s_weight, float *s_max, int *e_out, int *e_t_out) {
     constexpr int ld = KP + 1;
     float big = 0.0f, big_t = 0.0f;
-    for (int e = threadIdx.x; e < 32 * KP; e += 256) {
-        const int row = e / KP, k = e % KP;
+    if (threadIdx.x < 32) {
+        const long long r = (long long)tile * 32 + threadIdx.x;
+        s_weight[threadIdx.x] = weight && r < rows ? weight[r] * all_weight : all_weight;
+    }
+    Four v[KP / 32];                                             // all of a thread's loads first
+#pragma unroll
+    for (int q = 0; q < KP / 32; ++q) {
+        const int e = q * 256 + (int)threadIdx.x, row = e / (KP / 4), k = e % (KP / 4) * 4;
         const long long r = (long long)tile * 32 + row;
-        float v = 0.0f;
-        if (r < rows && k < factors && (!live || live[row] > 0.0f)) {
-            v = x[r * stride + k];
-            const float a = fabsf(v * by), b = fabsf(v * (weight ? weight[r] * all_weight : all_weight));
+        v[q] = Four{{0.0f, 0.0f, 0.0f, 0.0f}};
+        if (r < rows && k < factors && (!live || live[row] > 0.0f)) v[q] = load_four(x + r * stride, k, factors);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < KP / 32; ++q) {
+        const int e = q * 256 + (int)threadIdx.x, row = e / (KP / 4), k = e % (KP / 4) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = fabsf(v[q].v[j] * by), b = fabsf(v[q].v[j] * s_weight[row]);
             if (a < INFINITY) big = fmaxf(big, a);
             if (b < INFINITY) big_t = fmaxf(big_t, b);
+            lds[row * ld + k + j] = v[q].v[j];
         }
-        lds[row * ld + k] = v;
     }
     const int ex = tile_exponent(block_max(big, s_max)), ex_t = tile_exponent(block_max(big_t, s_max));
     *e_out = ex;
@@ -128,8 +140,7 @@ __device__ void write_frags(const float *__restrict__ x, long long stride, int t
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int row = 16 * (ct & 1) + (j & 3) + 8 * (j >> 2) + 4 * half;
-            const long long r = (long long)tile * 32 + row;
-            const float v = lds[row * ld + 32 * (ct >> 1) + (lane & 31)], g = weight && r < rows ? weight[r] * all_weight : all_weight;
+            const float v = lds[row * ld + 32 * (ct >> 1) + (lane & 31)], g = s_weight[row];
             _Float16 a, b;
             split2(v == 0.0f || !(fabsf(v) < INFINITY) ? 0.0f : ldexpf(v * g, ex_t), a, b);
             h[j] = a; m[j] = b;
@@ -139,16 +150,18 @@ __device__ void write_frags(const float *__restrict__ x, long long stride, int t
     }
 }
 
-// One launch: the users' tiles, the items' tiles, and (workgroups behind them) the teacher's rows, four per workgroup.
+// One launch: the teacher's rows, four per workgroup (first: a row is a chain of loads, the tiles are bandwidth), the users' tiles and the items' tiles.
 template <int KP, bool GRAD>
 __global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ ids,
                                                       float *__restrict__ ps, float *__restrict__ acc) {
     extern __shared__ int s_dyn[];
-    __shared__ float lds[32 * (KP + 1)], s_max[4], live[32];
+    __shared__ float lds[32 * (KP + 1)], s_max[4], live[32], s_weight[32];
     const rfm_distill_args &a = f.a;
-    const int b = blockIdx.x;
+    const int teachers = (int)((a.n_rows + 3) / 4), b = (int)blockIdx.x - teachers;
     int e, e_t;
-    if (b < f.user_tiles) {
+    if (b < 0) {
+        teacher_row<GRAD, (KP + 63) / 64>(a, (long long)blockIdx.x * 4 + (threadIdx.x >> 6), KP, s_dyn, part, mass, ids, ps, acc);
+    } else if (b < f.user_tiles) {
         // a row is live when its list has a usable entry (and its mask exists): 8 threads look through each
         {
             const int row = threadIdx.x >> 3, sub = threadIdx.x & 7;
@@ -162,7 +175,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c
             if (sub == 0) live[row] = (any >> ((threadIdx.x & 63) & ~7)) & 0xff ? 1.0f : 0.0f;
         }
         __syncthreads();
-        write_frags<KP>(a.users, a.user_stride, b, a.n_rows, a.n_factors, c, live, GRAD ? a.row_weight : nullptr, a.temperature, f.user_frag, GRAD ? f.user_frag_t : nullptr, lds, s_max, &e, &e_t);
+        write_frags<KP>(a.users, a.user_stride, b, a.n_rows, a.n_factors, c, live, GRAD ? a.row_weight : nullptr, a.temperature, f.user_frag, GRAD ? f.user_frag_t : nullptr, lds, s_weight, s_max, &e, &e_t);
         if (threadIdx.x == 0) {
             f.user_data[(size_t)b * kUserData + 32] = ldexpf(1.0f, -e);
             f.user_data[(size_t)b * kUserData + 33] = (float)e_t;
@@ -174,17 +187,15 @@ __global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c
             if (live[threadIdx.x] > 0.0f) m = max(a.allowed_rows ? (long long)a.allowed_rows[r] : (a.n_allowed == 1 ? 0 : r), -1ll);
             f.mask_row[r] = (int32_t)m;                          // (below n_allowed: the row would not be live)
         }
-    } else if (b < f.user_tiles + f.item_tiles) {
+    } else {
         const int t = b - f.user_tiles;
-        write_frags<KP>(a.items, a.item_stride, t, a.n_items, a.n_factors, 1.0f, nullptr, nullptr, 1.0f, f.item_frag, GRAD ? f.item_frag_t : nullptr, lds, s_max, &e, &e_t);
+        write_frags<KP>(a.items, a.item_stride, t, a.n_items, a.n_factors, 1.0f, nullptr, nullptr, 1.0f, f.item_frag, GRAD ? f.item_frag_t : nullptr, lds, s_weight, s_max, &e, &e_t);
         float *data = f.item_data + (size_t)t * kItemData;
         if (threadIdx.x < 32) {
             const long long i = (long long)t * 32 + threadIdx.x;
             data[threadIdx.x] = i < a.n_items ? (a.bias ? a.bias[i] * c : 0.0f) : -INFINITY;
         }
         if (threadIdx.x == 32) { data[32] = ldexpf(1.0f, -e); data[33] = (float)e_t; data[34] = ldexpf(1.0f, e_t); }
-    } else {
-        teacher_row<GRAD, GRAD ? KP / 64 + (KP % 64 != 0) : 0>(a, (long long)(b - f.user_tiles - f.item_tiles) * 4 + (threadIdx.x >> 6), KP, s_dyn, part, mass, ids, ps, acc);
     }
 }
 
@@ -377,6 +388,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (GRAD ? kPerSimd<KP, NC>
             }
         }
         stage(t + 2, i == 0 ? 2 : i - 1);
+        if (tile >= f.user_tiles) continue;                      // (a wavefront without users only fetches)
         f32x16 s[NC];
         tile_scores<KP, NC>(buf[i], lane, x, s);
         const f32x4 *data = reinterpret_cast<const f32x4 *>(buf[i] + kBuf - kItemData * 4);
@@ -451,7 +463,11 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
     float top = kLowest;
     for (int s = lane; s < f.splits; s += 64) top = fmaxf(top, f.part_m[(size_t)s * padded + r]);
     top = wave_max(top);
-    float total = 0.0f, o[(KP + 63) / 64] = {0.0f};
+    // KP / 4 lanes take four factors each of one split, the lanes behind them of the next ones
+    constexpr int at_once = 64 / (KP / 4);
+    const int mine = lane / (KP / 4), k4 = lane % (KP / 4) * 4;
+    float total = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < f.splits; s0 += 64) {
         const int s = s0 + lane;
         const float w = s < f.splits ? __builtin_amdgcn_exp2f(f.part_m[(size_t)s * padded + r] - top) : 0.0f;
@@ -461,12 +477,14 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         const int count = min(64, f.splits - s0);
-        const float *from = f.part_o + ((size_t)s0 * padded + r) * KP;
-#pragma unroll 16                                                // (loads in flight: they are far apart)
-        for (int q = 0; q < count; ++q) {
+        const float *from = f.part_o + ((size_t)s0 * padded + r) * KP + k4;
+        if (mine < at_once) {
+#pragma unroll 8                                                 // (loads in flight: they are far apart)
+            for (int q = mine; q < count; q += at_once) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (size_t)q * padded * KP);
 #pragma unroll
-            for (int k = 0; k < (KP + 63) / 64; ++k)
-                if (KP % 64 == 0 || k * 64 + lane < KP) o[k] = fmaf(from[(size_t)q * padded * KP + k * 64 + lane], weight[q], o[k]);
+                for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], weight[q], o[j]);
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -478,8 +496,12 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
     const float coef = f.a.temperature * (f.a.row_weight ? f.a.row_weight[r] : 1.0f);
     if (lane == 0) { f.user_data[at] = lse2; f.user_data_t[at] = coef; }
 #pragma unroll
-    for (int k = 0; k < (KP + 63) / 64; ++k)
-        if (k * 64 + lane < f.a.n_factors) f.a.d_users[(size_t)r * f.a.n_factors + k * 64 + lane] = coef * (o[k] / total - acc[(size_t)r * KP + k * 64 + lane]);
+    for (int j = 0; j < 4; ++j) {
+        float sum = o[j];
+        for (int d = 1; d < at_once; ++d) sum += __shfl(o[j], lane + d * (KP / 4));
+        const int k = k4 + j;
+        if (mine == 0 && k < f.a.n_factors) f.a.d_users[(size_t)r * f.a.n_factors + k] = coef * (sum / total - acc[(size_t)r * KP + k]);
+    }
 }
 
 // One workgroup per tile of 32 rows: the tile's teacher entries by the block of items_kernel that they fall into, modulo kBuckets (a block skips what
