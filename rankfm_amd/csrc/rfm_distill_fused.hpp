@@ -479,11 +479,18 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
         const int count = min(64, f.splits - s0);
         const float *from = f.part_o + ((size_t)s0 * padded + r) * KP + k4;
         if (mine < at_once) {
-#pragma unroll 8                                                 // (loads in flight: they are far apart)
-            for (int q = mine; q < count; q += at_once) {
-                const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (size_t)q * padded * KP);
+            constexpr int ahead = 8;                             // loads in flight: they are far apart
+            for (int q0 = mine; q0 < count; q0 += ahead * at_once) {
+                f32x4 x[ahead];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], weight[q], o[j]);
+                for (int h = 0; h < ahead; ++h) x[h] = *reinterpret_cast<const f32x4 *>(from + (size_t)min(q0 + h * at_once, count - 1) * padded * KP);
+#pragma unroll
+                for (int h = 0; h < ahead; ++h) {
+                    const int q = q0 + h * at_once;
+                    const float by = q < count ? weight[q] : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = q < count ? fmaf(x[h][j], by, o[j]) : o[j];
+                }
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
