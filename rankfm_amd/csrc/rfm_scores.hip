@@ -90,6 +90,11 @@ __device__ __forceinline__ int element(int slot) {               // position ins
 template <typename T, int P>
 __device__ __forceinline__ void load_tile(const T *row, int first, int n_items, float *s) {
     constexpr int ve = Vec<T>::n;
+    if (first + P * kThreads <= n_items) {                       // (the same for all: no branch between the loads)
+#pragma unroll
+        for (int j = 0; j < P / ve; ++j) load_vec(row + first + (j * kThreads + (int)threadIdx.x) * ve, s + j * ve);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < P / ve; ++j) {
         const int i = first + (j * kThreads + (int)threadIdx.x) * ve;
@@ -114,15 +119,10 @@ __device__ __forceinline__ float pick(const float (&x)[N], int k) {
     }
 }
 
-// where the row's lists name an item of the tile: count[item] of the history, and 1 + the position of the last bias entry.  False (and nothing
-// written): they name none.
+// what the row's lists name of a tile: count[item] of the history, and 1 + the position of the last bias entry
 template <int P>
-__device__ __forceinline__ bool scan_lists(const RowRules &w, int first, int *count, int *last) {
+__device__ __forceinline__ void scan_lists(const RowRules &w, int first, int *count, int *last) {
     constexpr int tile = P * kThreads;
-    int here = 0;
-    for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) here |= (unsigned)(w.hist[k] - first) < (unsigned)tile;
-    for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) here |= (unsigned)(w.bias_item[k] - first) < (unsigned)tile;
-    if (!__syncthreads_or(here)) return false;
     for (int k = threadIdx.x; k < tile; k += kThreads) { count[k] = 0; last[k] = 0; }
     __syncthreads();
     for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) {
@@ -134,7 +134,6 @@ __device__ __forceinline__ bool scan_lists(const RowRules &w, int first, int *co
         if (at < (unsigned)tile) atomicMax(last + at, (int)k + 1);
     }
     __syncthreads();
-    return true;
 }
 
 // the rules of an item that the row's lists name (an allowed one)
@@ -149,37 +148,62 @@ __device__ __forceinline__ float listed_score(const rfm_score_rules &u, const Ro
     return x;
 }
 
-template <typename T, int P, bool LISTS>
-__device__ __forceinline__ void apply_rules(const rfm_score_rules &u, const RowRules &w, int first, int n_items, const int *count, const int *last, float *s) {
+// What the rules say of every item, for the scores of a tile: biases, and a bit per score that is allowed.  Asked for all at once, next to the scores:
+// one after the other they are a chain of loads (1024 rows of 50 k items, the best ten under every rule: 82.6 us like that, 65.8 like this).  A tile
+// starts at a multiple of 32 items, so a vector's bits lie in one word.
+template <int P> struct Everyones { float bias[P]; unsigned allowed; };
+template <typename T, int P>
+__device__ __forceinline__ void load_everyones(const rfm_score_rules &u, const RowRules &w, int first, int n_items, Everyones<P> &e) {
+    constexpr int ve = Vec<T>::n;
+    const bool whole = first + P * kThreads <= n_items;          // (the same for all)
+    unsigned word[P / ve];
+    if (w.mask) {
+#pragma unroll
+        for (int j = 0; j < P / ve; ++j) word[j] = w.mask[min(first + (j * kThreads + (int)threadIdx.x) * ve, n_items - 1) >> 5];
+    }
+    if (u.item_bias) {
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < P / ve; ++j)
+#pragma unroll
+                for (int k = 0; k < ve; k += 4) load_vec(u.item_bias + first + (j * kThreads + (int)threadIdx.x) * ve + k, e.bias + j * ve + k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < P; ++k) e.bias[k] = u.item_bias[min(first + element<T>(k), n_items - 1)];
+        }
+    }
+    e.allowed = 0xffffffffu;
+    if (w.mask) {
+        e.allowed = 0;
+#pragma unroll
+        for (int j = 0; j < P / ve; ++j) e.allowed |= ((word[j] >> ((first + (j * kThreads + (int)threadIdx.x) * ve) & 31)) & ((1u << ve) - 1)) << (j * ve);
+    }
+}
+template <int P>
+__device__ __forceinline__ void apply_everyones(const rfm_score_rules &u, const Everyones<P> &e, float *s) {
+    if (u.item_bias) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) s[k] = s[k] + e.bias[k];
+    }
+    if (__any(e.allowed != 0xffffffffu)) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) s[k] = (e.allowed >> k) & 1u ? s[k] : -INFINITY;
+    }
+}
+
+// ... and with a row's lists: what they count for a tile
+template <typename T, int P>
+__device__ __forceinline__ void apply_counts(const rfm_score_rules &u, const RowRules &w, int first, int n_items, const int *count, const int *last, float *s) {
     constexpr int ve = Vec<T>::n;
 #pragma unroll
     for (int j = 0; j < P / ve; ++j) {
         const int at = (j * kThreads + (int)threadIdx.x) * ve, i = first + at;
         if (i >= n_items) continue;
-        unsigned bits = 0xffffffffu;
-        if (w.mask) {                                            // the ve items may lie in two words
-            const int word = i >> 5, words = (n_items + 31) >> 5;
-            const unsigned long long both = ((unsigned long long)w.mask[word + 1 < words ? word + 1 : word] << 32) | w.mask[word];
-            bits = (unsigned)(both >> (i & 31));
-        }
-        float bias[ve];
-        if (!LISTS && u.item_bias) {
-            if (i + ve <= n_items) {
-#pragma unroll
-                for (int k = 0; k < ve; k += 4) load_vec(u.item_bias + i + k, bias + k);
-            } else {
-#pragma unroll
-                for (int k = 0; k < ve; ++k) bias[k] = i + k < n_items ? u.item_bias[i + k] : 0.0f;
-            }
-        }
+        const unsigned bits = w.mask ? w.mask[i >> 5] >> (i & 31) : 0xffffffffu;
 #pragma unroll
         for (int k = 0; k < ve; ++k) {
             float x = s[j * ve + k];
-            if constexpr (LISTS) {
-                if (i + k < n_items) x = listed_score(u, w, i + k, count[at + k], last[at + k], x);
-            } else {
-                if (u.item_bias) x = x + bias[k];
-            }
+            if (i + k < n_items) x = listed_score(u, w, i + k, count[at + k], last[at + k], x);
             s[j * ve + k] = (bits >> k) & 1u ? x : -INFINITY;
         }
     }
@@ -210,6 +234,8 @@ __global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score
     int hits = 0, mine = -1;                                     // the item that the lists name and this thread sees to, and what becomes of its score
     load_tile<T, P>(scores + r * stride, first, n_items, s);
     const RowRules w = row_rules(u, r, n_items);
+    Everyones<P> all;
+    load_everyones<T, P>(u, w, first, n_items, all);
     if (w.bad) {
 #pragma unroll
         for (int k = 0; k < P; ++k) s[k] = __uint_as_float(0x7fc00000u);
@@ -248,16 +274,15 @@ __global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score
             asm volatile("" : "+v"(value));                      // (no instruction: it is read by now)
             __syncthreads();                                     // `out` may be `scores`: no store before these reads
         }
-        if (!many) apply_rules<T, P, false>(u, w, first, n_items, nullptr, nullptr, s);
+        if (!many) apply_everyones<P>(u, all, s);
         else {
             constexpr int per = kCounted / kThreads;             // (tiles of P scores per thread lie in tiles of `per`: vectors of a tile come in order)
 #pragma unroll
             for (int q = 0; q < P / per; ++q) {
                 __syncthreads();
                 const int from = first + q * kCounted;
-                if (scan_lists<per>(w, from, lists.counted.count, lists.counted.last))
-                    apply_rules<T, per, true>(u, w, from, n_items, lists.counted.count, lists.counted.last, s + q * per);
-                else apply_rules<T, per, false>(u, w, from, n_items, nullptr, nullptr, s + q * per);
+                scan_lists<per>(w, from, lists.counted.count, lists.counted.last);
+                apply_counts<T, per>(u, w, from, n_items, lists.counted.count, lists.counted.last, s + q * per);
             }
         }
     }
@@ -473,12 +498,12 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
                     x[k] = key && key < ceiling ? key_score(key) : -INFINITY;
                 }
             } else {
-#pragma unroll
-                for (int q = 0; q < kSuper; ++q) load_tile<T, kPer>(row, t0 + q * kTile, end, x + q * kPer);
+                load_tile<T, kAll>(row, t0, end, x);
                 if constexpr (RULED) {
                     if (!listed || hashed) {
-#pragma unroll
-                        for (int q = 0; q < kSuper; ++q) apply_rules<T, kPer, false>(u, w, t0 + q * kTile, n_items, nullptr, nullptr, x + q * kPer);
+                        Everyones<kAll> all;
+                        load_everyones<T, kAll>(u, w, t0, n_items, all);
+                        apply_everyones<kAll>(u, all, x);
                         if (hashed) {
                             if (t0 / kWindow != window) { window = t0 / kWindow; window_bits(lists_memory.listed, window * kWindow); }
 #pragma unroll
@@ -493,9 +518,8 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
 #pragma unroll
                         for (int q = 0; q < kSuper; ++q) {
                             if (t0 + q * kTile >= end) break;    // (the same for all)
-                            if (scan_lists<kPer>(w, t0 + q * kTile, lists_memory.tiled.count, lists_memory.tiled.last))
-                                apply_rules<T, kPer, true>(u, w, t0 + q * kTile, n_items, lists_memory.tiled.count, lists_memory.tiled.last, x + q * kPer);
-                            else apply_rules<T, kPer, false>(u, w, t0 + q * kTile, n_items, nullptr, nullptr, x + q * kPer);
+                            scan_lists<kPer>(w, t0 + q * kTile, lists_memory.tiled.count, lists_memory.tiled.last);
+                            apply_counts<T, kPer>(u, w, t0 + q * kTile, n_items, lists_memory.tiled.count, lists_memory.tiled.last, x + q * kPer);
                             __syncthreads();                     // (the next tile's scan clears the counts)
                         }
                     }
