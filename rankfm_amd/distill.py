@@ -7,7 +7,12 @@ allowed, score not -inf; an item that stands there twice counts twice.
     loss[r] = temperature^2 * sum_j p_j (log p_j - log q[item_j])                   a row without a usable entry: 0
     gradients of sum_r row_weight[r] * loss[r]:  dz = temperature * row_weight * (q - p),  dz . items,  dz^T . users,  column sums
 
-All float32, like the model's weights; the device's current stream; no host synchronisation.  The gradients are returned, not recorded by
+All float32, like the model's weights.  Up to 128 factors the products are made of two half-precision parts per factor, scaled by a power of two per
+tile of 32 consecutive rows of [users] or [items]: as exact as float32 products for factors down to 2^-16 of the largest finite one of
+their tile; below that a factor is off by up to 2^-40 of the largest.  A factor that is not finite spoils the rows it counts in, and nothing
+where a mask takes it out.  At most 2^24 rows, 2^25 items, 1024 factors and 1024 entries per list.
+
+The device's current stream; no host synchronisation.  The gradients are returned, not recorded by
 autograd.  Sums have a fixed order: the same call gives the same bits.
 """
 import ctypes as C

@@ -12,7 +12,7 @@ import torch
 
 from . import _hip
 from .distill import distill_gradients
-from .scores import ScoreRules, TopScores, adjust_scores, top_scores
+from .scores import ScoreRules, TopScores, adjust_scores, check_rules, top_scores
 
 WEIGHT_NAMES = ("w_i", "w_if", "v_u", "v_i", "v_uf", "v_if")
 
@@ -260,8 +260,10 @@ class DeviceSession:
         if n_items < 1 or n_items > self.n_items:
             raise ValueError("[n_items] must be between 1 and the number of training items")
         rows_d = torch.where(torch.isnan(users_d), -1.0, users_d).to(torch.int32)
-        if rules is not None and rules.penalises() and rules.history is None:
-            rules = replace(rules, history=(self.csr_offsets, self.csr_items), history_rows=rows_d)
+        if rules is not None:
+            if isinstance(rules, ScoreRules) and rules.penalises() and rules.history is None:
+                rules = replace(rules, history=(self.csr_offsets, self.csr_items), history_rows=rows_d)
+            check_rules(rules, n, self.n_items, self.device)      # (all of the call's rows: below they are cut to what is held at a time)
         gone = None
         if filter_previous:
             gone = ScoreRules(history=(self.csr_offsets, self.csr_items), history_rows=rows_d,

@@ -144,6 +144,7 @@ def allowed_fields(u, allowed, allowed_rows, rows, items, device):
 
 
 def _rules_struct(rules, rows, items, device):
+    """rfm_score_rules of a call of `rows` rows, or ValueError"""
     if not isinstance(rules, ScoreRules):
         raise ValueError("[rules] must be a rankfm_amd.ScoreRules")
     u = _hip.ScoreRulesStruct(repetition_all=1.0)
@@ -172,6 +173,11 @@ def _rules_struct(rules, rows, items, device):
         u.n_bias_items = listed.shape[0]
     allowed_fields(u, rules.allowed, rules.allowed_rows, rows, items, device)
     return u
+
+
+def check_rules(rules, rows, items, device):
+    """ValueError unless the rules are those of a call of `rows` rows"""
+    _rules_struct(rules, rows, items, device)
 
 
 def _byte_range(t):

@@ -326,3 +326,22 @@ def test_large_problems(rows, items, factors, n, given):
         assert off <= 1, (name, off)
     again = distill_gradients(*args, row_weight=torch.from_numpy(p.g).cuda() if given else None, **kw)
     assert all(torch.equal(x, y) for x, y in zip(got, again) if x is not None)
+
+
+@pytest.mark.parametrize("factors", [24, 64, 128])
+def test_rows_of_very_different_size_share_a_tile(factors):
+    """users from 1e-2 to 1e2 of the others' size, every size in every tile of 32.  A row's bound counts its own scores, and what a factor may be off by next to
+    the largest of its tile: 2^-40 of that, against the item's factors (and the other way round), summed over the factors"""
+    p = Problem(rows=100, items=700, factors=factors, n=8, tau=1.0, seed=14)
+    p.u *= (10.0 ** (np.arange(100) % 5 - 2.0))[:, None].astype(np.float32)
+    want, _ = p.exact()
+    args, kw = p.given()
+    u, v = np.abs(p.u).astype(np.float64), np.abs(p.v).astype(np.float64)
+    s = (u @ v.T + np.abs(p.b)).max(1)
+    ez = (factors + 6) * E * s + 2.0 ** -40 * factors * (u.max() * v.max() + u.max(1) * v.max())
+    t = np.abs(np.where(np.isinf(p.t), 0, p.t)).max(1)
+    eq, ep = 2 * ez + (700 / 32 + 80) * E, (8 + 80 + 8 * t) * E
+    big = 2 * t + np.log(8) + 2 * s + np.log(700)                                 # |log p| <= 2 max |t| + log n;  |z|, |lse| <= s, s + log I
+    tol = 2 * ez + eq + ep + 88 * E * big
+    for got in (distill_loss(*args, **kw), distill_gradients(*args, **kw).loss):
+        assert (np.abs(got.cpu().numpy() - want[0]) <= tol).all()

@@ -147,3 +147,16 @@ def test_a_student_learns_from_a_teacher(P, Q):
         kw = dict(dict(users=users, learning_rate=None), **bad)
         with pytest.raises(ValueError):
             student.distill(np.array(kw["users"]), answers.items, answers.scores, learning_rate=kw["learning_rate"])
+
+
+def test_rules_of_other_rows_than_the_users_are_refused():
+    s, _ = session(seed=4)
+    users = np.arange(5, dtype=np.float32)
+    masks = pack_allowed(torch.ones((6, 130), dtype=torch.bool).cuda())
+    for rules in (ScoreRules(allowed=masks), ScoreRules(allowed=masks, allowed_rows=torch.zeros(6, dtype=torch.int32).cuda()), ScoreRules(presence=torch.ones(6).cuda()),
+                  ScoreRules(row_bias=(torch.zeros(7, dtype=torch.int64).cuda(), torch.zeros(0, dtype=torch.int32).cuda(), torch.zeros(0).cuda())),
+                  ScoreRules(item_bias=torch.zeros(131).cuda()), "none"):
+        with pytest.raises(ValueError):
+            s.top_scores(users, 3, rules)
+        with pytest.raises(ValueError):
+            s.recommend(users, 3, rules=rules)

@@ -159,3 +159,14 @@ def test_the_c_entries_refuse_bad_arguments(lib):
     assert lib.rfm_scores_workspace_bytes(C.byref(mv), 3) == 0 and lib.rfm_effective_factors(C.byref(mv)) == 0
     assert lib.rfm_scores_device(C.byref(mv), 1, one, one, one, 1 << 30, None) == _hip.ERR_BAD_ARG
     assert lib.rfm_effective_factors_device(C.byref(mv), 1, one, one, one, one, None) == _hip.ERR_BAD_ARG
+
+
+def test_sizes_that_distillation_does_not_take(lib):
+    base = dict(n_rows=2, n_items=8, n_factors=4, n_teacher=2, temperature=1.0, users=64, items=64, user_stride=4, item_stride=4, teacher_items=64, teacher_scores=64,
+                loss=64, d_users=64, d_items=64)
+    for kw in (dict(n_items=(1 << 25) + 1), dict(n_rows=(1 << 24) + 1), dict(n_factors=1025, user_stride=1025, item_stride=1025), dict(n_teacher=1025)):
+        a = _hip.DistillArgs(**dict(base, **kw))
+        assert lib.rfm_distill_workspace_bytes(C.byref(a)) == 0
+        assert lib.rfm_distill_device(C.byref(a), C.c_void_p(64), 1 << 60, None) == -5, kw
+    for kw in (dict(n_items=1 << 25), dict(n_rows=1 << 24), dict(n_factors=1024, user_stride=1024, item_stride=1024), dict(n_teacher=1024)):
+        assert lib.rfm_distill_workspace_bytes(C.byref(_hip.DistillArgs(**dict(base, **kw)))) > 0, kw
