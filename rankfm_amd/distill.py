@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _hip
-from .scores import allowed_fields, check_device, check_tensor
+from .scores import allowed_fields, check_device, check_tensor, current_stream, on_device
 
 
 class DistillGradients(NamedTuple):
@@ -64,24 +64,24 @@ def _call(users, items, bias, teacher_items, teacher_scores, temperature, allowe
     allowed_fields(a, allowed, allowed_rows, rows, a.n_items, device)
     if row_weight is not None:
         a.row_weight = check_tensor(row_weight, "row_weight", torch.float32, (rows,), device)
-    loss = torch.empty(rows, dtype=torch.float32, device=device)
+    loss = users.new_empty(rows)
     a.loss = loss.data_ptr()
     d_users = d_items = d_bias = None
     if gradients:
-        d_users = torch.empty((rows, factors), dtype=torch.float32, device=device)
-        d_items = torch.empty((a.n_items, factors), dtype=torch.float32, device=device)
+        d_users = users.new_empty((rows, factors))
+        d_items = users.new_empty((a.n_items, factors))
         if rows == 0:
             return DistillGradients(loss, d_users, d_items.zero_(), None if bias is None else torch.zeros_like(bias))
         a.d_users, a.d_items = d_users.data_ptr(), d_items.data_ptr()
         if bias is not None:
-            d_bias = torch.empty(a.n_items, dtype=torch.float32, device=device)
+            d_bias = users.new_empty(a.n_items)
             a.d_bias = d_bias.data_ptr()
     elif rows == 0:
         return loss
     lib = _hip.lib()
-    with torch.cuda.device(device):
+    with on_device(device):
         ws = torch.empty(lib.rfm_distill_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=device)
-        rc = lib.rfm_distill_device(C.byref(a), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(device).cuda_stream)
+        rc = lib.rfm_distill_device(C.byref(a), ws.data_ptr(), ws.numel(), current_stream(device))
     _hip.raise_for_status(rc)
     return DistillGradients(loss, d_users, d_items, d_bias) if gradients else loss
 

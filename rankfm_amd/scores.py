@@ -5,6 +5,7 @@ else holds: penalties for what a user has already had, biases, and masks of what
 MI355X; work is enqueued on that device's current stream and nothing synchronises, so the calls may be captured into a graph.
 """
 import ctypes as C
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -82,17 +83,28 @@ def pack_allowed(mask):
 
 def check_tensor(t, name, dtype, shape, device):
     """a contiguous tensor of this type and shape (None: any size) on this device, or ValueError"""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.is_contiguous() and (
+            t.shape == shape or None in shape and t.dim() == len(shape) and all(w is None or g == w for g, w in zip(t.shape, shape))):
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise ValueError("[%s] must be a torch tensor" % name)
     if t.dtype != dtype:
         raise ValueError("[%s] must be %s, got %s" % (name, str(dtype).replace("torch.", ""), str(t.dtype).replace("torch.", "")))
-    if t.dim() != len(shape) or any(w is not None and g != w for g, w in zip(t.shape, shape)):
-        raise ValueError("[%s] must have shape %s, got %s" % (name, list(shape), list(t.shape)))
     if t.device != device:
         raise ValueError("[%s] is on %s, the call on %s" % (name, t.device, device))
     if not t.is_contiguous():
         raise ValueError("[%s] must be contiguous" % name)
-    return t.data_ptr()
+    raise ValueError("[%s] must have shape %s, got %s" % (name, list(shape), list(t.shape)))
+
+
+def on_device(device):
+    """the context in which kernels of `device` are launched: nothing where it is the current one (a small call's time is the host's)"""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def current_stream(device):
+    """the device's current stream as the C entries take it (`torch.cuda.current_stream(device).cuda_stream` without the object)"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check_device(t, name):
@@ -193,7 +205,7 @@ def adjust_scores(scores, rules, out=None):
     device = _check_scores(scores)
     rows, items = scores.shape
     if out is None:
-        out = torch.empty((rows, items), dtype=scores.dtype, device=device)
+        out = scores.new_empty((rows, items))
     elif out is not scores:
         if not isinstance(out, torch.Tensor) or out.dtype != scores.dtype or out.shape != scores.shape or out.device != device:
             raise ValueError("[out] must be a tensor of the scores' type, shape and device")
@@ -206,9 +218,9 @@ def adjust_scores(scores, rules, out=None):
     u = _rules_struct(rules, rows, items, device)
     if rows == 0:
         return out
-    with torch.cuda.device(device):
+    with on_device(device):
         rc = _hip.lib().rfm_adjust_scores_device(C.byref(u), _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), out.data_ptr(),
-                                                 _row_stride(out), torch.cuda.current_stream(device).cuda_stream)
+                                                 _row_stride(out), current_stream(device))
     _hip.raise_for_status(rc)
     return out
 
@@ -229,9 +241,9 @@ def top_scores(scores, n, rules=None):
     if rows == 0:
         return TopScores(best, value)
     lib = _hip.lib()
-    with torch.cuda.device(device):
+    with on_device(device):
         ws = torch.empty(lib.rfm_top_scores_workspace_bytes(rows, items, n), dtype=torch.uint8, device=device)
         rc = lib.rfm_top_scores_device(C.byref(u) if u is not None else None, _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), n,
-                                       best.data_ptr(), value.data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(device).cuda_stream)
+                                       best.data_ptr(), value.data_ptr(), ws.data_ptr(), ws.numel(), current_stream(device))
     _hip.raise_for_status(rc)
     return TopScores(best, value)
