@@ -19,11 +19,12 @@
 //                    in-lane; weighted sums O^T += items^T . exp2(z^T - max).
 //   items_kernel     columns: 32 or 64 items per wavefront, fixed; streams user tiles.  z = users . items^T, dz from the row's lse, O^T += users^T . dz.
 //
-// What bounds them: the matrix instructions, at the clock that their power leaves.  8192 rows x 50 k items at k = 64, gradients: 0.69 ms in all, of which
-// forward_kernel 318 us, items_kernel 385, prepare 34; 2 x 6 x 8192 x 50 k x 64 x 2 operations are 0.63 TFLOP and 393 us at the 1.6 PFLOP/s that a
-// loop of nothing but these instructions reaches.  The rest are LDS reads of the streamed tiles (-18 .. -27 % in a copy without them), the exponentials
-// and the cuts into parts, which do not overlap with them where power is the limit.  The loss alone, k = 64: 187 us.  2048 rows x 200 k items at k = 128:
-// 1.28 ms, of which 564 + 659.
+// What bounds them: 8192 rows x 50 k items at k = 64, lists of 32, gradients: 0.69 ms in all, of which forward_kernel 313 us, items_kernel 382, prepare 25, the joins 14 and
+// 12 (under a profiler, which adds a few percent).  2 x 6 x 8192 x 50 k x 64 x 2 operations are 0.63 TFLOP: 393 us at
+// the 1.6 PFLOP/s that a loop of nothing but these instructions holds (its power sets its clock).  The matrix cores are busy in 55 % of the
+// cycles of forward_kernel and 43 % of items_kernel; vector instructions issue in 50 % of both.  In copies: no LDS reads of the streamed tiles -18 .. -27 %,
+// no teacher's entries -5 %, no test for a larger maximum -2 .. -4 %, no exponentials or a higher wave priority next to nothing.  The loss alone:
+// 175 us.  2048 rows x 200 k items at k = 128: 1.25 ms, of which 558 + 658; 63 % and 49 %.
 #pragma once
 
 namespace rfm {
@@ -48,7 +49,7 @@ template <int KP> struct Frag {
 };
 // Wavefronts per SIMD that the registers are kept to.  Up to 64 factors a wavefront may have two tiles of 32 columns, NC = 2: what it reads of a streamed
 // tile from LDS then serves both, at two wavefronts per SIMD instead of three and half as many workgroups (8192 rows x 50 k items at k = 64: 728 -> 689 us;
-// at k = 128, where it would leave one, 12 % slower).
+// at k = 128, where it would leave one wavefront per SIMD, 12 % slower).
 template <int KP, int NC> constexpr int kPerSimd = KP <= 64 && NC == 1 ? 3 : 2;
 
 struct FusedArgs {

@@ -223,6 +223,9 @@ struct Counted {
 // their way through three dependent loads passes meanwhile.  A tile's few list entries are gathered in LDS; a thread each counts those of its item, makes
 // that item's score and writes it over what the row's pass left there (read before anything of the tile is written: `out` may be `scores`).  Where
 // there are more than 256, counts per item are made, 2048 items at a time.
+// Bound by memory: 512 rows of 200 k items in bf16, 74 us = 5.5 TB/s read and written (a 4 GiB copy reaches 4.7); 1000 rows of 35 k in fp32 under every
+// rule, 61.6 us = 4.5 TB/s; one row of 3.7 k, 4.6 us of the device's and 16 of the host's time.  8 (fp32) or 16 scores per thread are 32 bytes of
+// a row either way: eight workgroups per CU, no loop.
 template <typename T, int P>
 __global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score_rules u, long long row0, int tiles, int n_items, const T *scores,
                                                                  long long stride, T *out, long long out_stride) {
@@ -330,13 +333,37 @@ template <bool RULED> struct Top {
 constexpr int kSlots = 1024, kShort = 512;       // hash slots for the items that a row's lists name; lists of more entries than kShort are scanned per tile
 constexpr int kWindow = 65536;                   // items whose membership bits are in LDS at a time
 
-// Descending bitonic sort of the `m` keys of a wavefront's buffer, in its registers: key r * 64 + lane is the r-th of its lane, so distances of 64 and
-// more stay inside a lane and shorter ones are a shuffle; nothing waits for another wavefront.
-template <int R>
-__device__ __forceinline__ void sort_in_registers(u64 *buf, int m, int lane) {
+// x of lane ^ J.  Inside a row of 16 lanes that is an operand's modifier (DPP), inside 32 a fixed pattern, beyond a shuffle
+template <int J>
+__device__ __forceinline__ unsigned from_lane_xor(unsigned x) {
+    if constexpr (J == 1) return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true);            // quad_perm 1 0 3 2
+    else if constexpr (J == 2) return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true);       // quad_perm 2 3 0 1
+    else if constexpr (J == 8) return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true);      // row_ror 8
+    else if constexpr (J < 32) return (unsigned)__builtin_amdgcn_ds_swizzle((int)x, J << 10 | 0x1f);
+    else return __shfl_xor(x, J);
+}
+// the step of distance J of the stage of 2 * k's merges (nothing where the stage has no such step)
+template <int R, int J>
+__device__ __forceinline__ void exchange(u64 (&x)[R], int k, int lane) {
+    if (J >= k) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const u64 other = (u64)from_lane_xor<J>((unsigned)(x[r] >> 32)) << 32 | from_lane_xor<J>((unsigned)x[r]);
+        const bool larger = (((r * 64 + lane) & k) == 0) == ((lane & J) == 0);
+        x[r] = (other > x[r]) == larger ? other : x[r];
+    }
+}
+// Descending bitonic sort of `m` keys by a wavefront, in its registers: key r * 64 + lane is the r-th of its lane, so distances of 64 and more stay inside
+// a lane and shorter ones are a shuffle; nothing waits for another wavefront but the writing back: key k is key `first` + k of the four buffers one
+// behind the other, whose ends are s[].
+template <int R, int BUF>
+__device__ __forceinline__ void sort_in_registers(u64 *all, const int (&s)[kWaves - 1], int first, int m, int wave, int lane) {
     u64 x[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) x[r] = r * 64 + lane < m ? buf[r * 64 + lane] : 0;
+    for (int r = 0; r < R; ++r) {
+        const int k = r * 64 + lane, g = first + k, at = g < s[0] ? g : g < s[1] ? BUF + g - s[0] : g < s[2] ? 2 * BUF + g - s[1] : 3 * BUF + g - s[2];
+        x[r] = k < m ? all[at] : 0;
+    }
 #pragma unroll 1
     for (int k = 2; k <= 64 * R; k <<= 1) {
 #pragma unroll
@@ -351,20 +378,16 @@ __device__ __forceinline__ void sort_in_registers(u64 *buf, int m, int lane) {
                 x[r | d] = swap ? a : b;
             }
         }
-#pragma unroll 1
-        for (int j = min(k / 2, 32); j > 0; j >>= 1) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const u64 other = __shfl_xor(x[r], j);
-                const bool larger = (((r * 64 + lane) & k) == 0) == ((lane & j) == 0);
-                x[r] = (other > x[r]) == larger ? other : x[r];
-            }
-        }
+        exchange<R, 32>(x, k, lane);
+        exchange<R, 16>(x, k, lane);
+        exchange<R, 8>(x, k, lane);
+        exchange<R, 4>(x, k, lane);
+        exchange<R, 2>(x, k, lane);
+        exchange<R, 1>(x, k, lane);
     }
+    __syncthreads();                                             // the keys of all wavefronts are in registers
 #pragma unroll
-    for (int r = 0; r < R; ++r) buf[r * 64 + lane] = x[r];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    for (int r = 0; r < R; ++r) all[wave * BUF + r * 64 + lane] = x[r];
 }
 // The same in LDS, for any number that the buffer holds (padded to a power of two): twice the time, and no registers
 __device__ __forceinline__ void sort_in_place(u64 *buf, int m, int lane) {
@@ -384,14 +407,6 @@ __device__ __forceinline__ void sort_in_place(u64 *buf, int m, int lane) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-__device__ __forceinline__ void sort_keys(u64 *buf, int m, int lane) {
-    if (m <= 64) sort_in_registers<1>(buf, m, lane);
-    else if (m <= 128) sort_in_registers<2>(buf, m, lane);
-    else if (m <= 256) sort_in_registers<4>(buf, m, lane);
-    else if (m <= 512) sort_in_registers<8>(buf, m, lane);
-    else sort_in_place(buf, m, lane);
-}
-
 // what a row's lists name, when they are short: a hash table of the items with their counts and last bias entries, and a bit per item of a window
 struct Listed {
     int id[kSlots], count[kSlots], last[kSlots];
@@ -442,7 +457,11 @@ __device__ __forceinline__ void window_bits(Listed &m, int first) {
 // from the first 8192 scores (4096 under rules): each group of eight holds its maximum in a register, a wavefront finds by bisection over ballots the
 // value that its share of n of its group maxima reach, and the least of the four wavefronts' values is reached by at least n scores.  So the final
 // sort sees a few times n keys, not the row (1837 rows of 640 items, the best two: 60 us when the empty wavefronts leave it none, 16 with it).  Under
-// rules, items that the row's lists name are left out of the pass (a bit per item in LDS) and looked at by themselves afterwards.  FROM_KEYS: the "scores" are the sorted keys that the segments of a row left behind.
+// rules, items that the row's lists name are left out of the pass (a bit per item in LDS) and looked at by themselves afterwards.  FROM_KEYS: the "scores"
+// are the sorted keys that the segments of a row left behind.
+// Bound by memory without rules: 4096 rows of 50 k items, the best 64, 160 us = 5.1 TB/s read (a plain sum of as much reaches 4.0 - 4.7); under every
+// rule 1024 rows take 63 us = 3.3 TB/s: the biases are as many loads again (54 us with them alone, 46 with nothing), from the L2, and so are the masks.  One
+// row of 200 k: 17.5 us, two launches of which neither has enough work for the chip.
 template <typename T, bool RULED, bool FROM_KEYS>
 __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score_rules u, long long row0, int segments, int segment, int n_items,
                                                               const T *__restrict__ scores, long long stride, const u64 *__restrict__ keys_in, int n_keys,
@@ -454,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
     __shared__ unsigned wave_t[kWaves];
     __shared__ int wave_m[kWaves];
     __shared__ u64 last_key;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const long long r = row0 + blockIdx.x / segments;
     const int seg = (int)(blockIdx.x % segments);
     const int begin = FROM_KEYS ? 0 : seg * segment, end = FROM_KEYS ? n_keys : min(n_items - begin, segment) + begin;
@@ -603,21 +622,18 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
             }
         }
         // The candidates in order.  Few are placed by counting: a key's place is the number of larger ones (keys are unique).  Otherwise every wavefront
-        // sorts its own, and a key's place is its place there and the number of larger keys of the other three, each found by bisection.  (Sorting all
-        // of them together takes a barrier for each of its steps: 4096 rows of 50 k, 64 wanted, 194 -> 165 us.)  Counting is the square of the work; 256
-        // are few where rows are and one workgroup's way to the end is what counts.
+        // sorts an equal share of them (the vectors of a short row go to the first wavefronts), and a key's place is its place there and the number of
+        // larger keys of the other three, each found by bisection.  (Sorting all of them together takes a barrier for each of its steps: 4096 rows of
+        // 50 k, 64 wanted, 194 -> 165 us.  The shares: 2377 rows of 1039, 390 wanted, 200 -> 152; 6 of 3204, 365 wanted, 31 -> 22.)  Counting is the
+        // square of the work; 256 are few where rows are and one workgroup's way to the end is what counts.
         if (lane == 0) wave_m[wave] = m;
         if (threadIdx.x == 0) last_key = 0;
         __syncthreads();
-        int count[kWaves - 1], most = 0, total = m;              // of the other wavefronts
-        const u64 *other[kWaves - 1];
+        int in_wave[kWaves], total = 0;
 #pragma unroll
-        for (int v = 0; v < kWaves - 1; ++v) {
-            const int who = __builtin_amdgcn_readfirstlane((wave + 1 + v) & (kWaves - 1));
-            other[v] = buf + who * kBuf;
-            count[v] = __builtin_amdgcn_readfirstlane(wave_m[who]);
-            total += count[v];
-            most = max(most, count[v]);
+        for (int v = 0; v < kWaves; ++v) {
+            in_wave[v] = __builtin_amdgcn_readfirstlane(wave_m[v]);
+            total += in_wave[v];
         }
         const int got = total < want ? total : want;
         const size_t row_out = FROM_KEYS || segments == 1 ? (size_t)r * n : ((size_t)(r - row0) * segments + seg) * n;
@@ -633,31 +649,66 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
             for (int k = lane; k < m; k += 64) {
                 const u64 key = mine[k];
                 int place = 0;
-#pragma unroll 4
-                for (int q = 0; q < m; ++q) place += mine[q] > key;
 #pragma unroll
-                for (int v = 0; v < kWaves - 1; ++v)
+                for (int v = 0; v < kWaves; ++v)
 #pragma unroll 4
-                    for (int q = 0; q < count[v]; ++q) place += other[v][q] > key;
+                    for (int q = 0; q < in_wave[v]; ++q) place += buf[v * kBuf + q] > key;
                 if (place < want) put(place, key);
             }
         } else {
-            if (m > 1) sort_keys(mine, m, lane);
+            const int share = (total + kWaves - 1) / kWaves;
+            if (share <= 512) {
+                const int ends[kWaves - 1] = {in_wave[0], in_wave[0] + in_wave[1], in_wave[0] + in_wave[1] + in_wave[2]}, first = wave * share;
+                m = min(max(total - first, 0), share);
+                if (share <= 64) sort_in_registers<1, kBuf>(buf, ends, first, m, wave, lane);
+                else if (share <= 128) sort_in_registers<2, kBuf>(buf, ends, first, m, wave, lane);
+                else if (share <= 256) sort_in_registers<4, kBuf>(buf, ends, first, m, wave, lane);
+                else sort_in_registers<8, kBuf>(buf, ends, first, m, wave, lane);
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v) in_wave[v] = min(max(total - v * share, 0), share);
+            } else sort_in_place(mine, m, lane);
             __syncthreads();
-            for (int k = lane; k < min(m, want); k += 64) {
-                const u64 key = mine[k];
-                int above[kWaves - 1] = {0};
-                for (int step = most > 0 ? 1 << (31 - __clz(most)) : 0; step > 0; step >>= 1)
+            int count[kWaves - 1], most = 0;                     // of the other wavefronts
+            const u64 *other[kWaves - 1];
 #pragma unroll
-                    for (int v = 0; v < kWaves - 1; ++v) {
-                        const int next = above[v] + step;
-                        above[v] = next <= count[v] && other[v][next - 1] > key ? next : above[v];
-                    }
-                int place = k;
-#pragma unroll
-                for (int v = 0; v < kWaves - 1; ++v) place += above[v];
-                if (place < want) put(place, key);
+            for (int v = 0; v < kWaves - 1; ++v) {
+                const int who = (wave + 1 + v) & (kWaves - 1);
+                other[v] = buf + who * kBuf;
+                count[v] = who == 0 ? in_wave[0] : who == 1 ? in_wave[1] : who == 2 ? in_wave[2] : in_wave[3];
+                most = max(most, count[v]);
             }
+            const int steps = most > 0 ? 1 << (31 - __clz(most)) : 0;
+            auto place_keys = [&](auto keys) {                   // `keys` of a lane at a time: their reads follow each other, not their bisections
+                constexpr int at_once = decltype(keys)::value;
+                for (int k0 = 0; k0 < min(m, want); k0 += 64 * at_once) {
+                    u64 key[at_once];
+                    int above[at_once][kWaves - 1];
+#pragma unroll
+                    for (int h = 0; h < at_once; ++h) {
+                        key[h] = k0 + h * 64 + lane < m ? mine[k0 + h * 64 + lane] : 0;
+#pragma unroll
+                        for (int v = 0; v < kWaves - 1; ++v) above[h][v] = 0;
+                    }
+                    for (int step = steps; step > 0; step >>= 1)
+#pragma unroll
+                        for (int h = 0; h < at_once; ++h)
+#pragma unroll
+                            for (int v = 0; v < kWaves - 1; ++v) {
+                                const int next = above[h][v] + step;
+                                above[h][v] = next <= count[v] && other[v][min(next, kBuf) - 1] > key[h] ? next : above[h][v];
+                            }
+#pragma unroll
+                    for (int h = 0; h < at_once; ++h) {
+                        int place = k0 + h * 64 + lane;
+                        const bool on = place < m;
+#pragma unroll
+                        for (int v = 0; v < kWaves - 1; ++v) place += above[h][v];
+                        if (on && place < want) put(place, key[h]);
+                    }
+                }
+            };
+            if (min(m, want) <= 64) place_keys(std::integral_constant<int, 1>());
+            else place_keys(std::integral_constant<int, 2>());
         }
         for (int k = got + threadIdx.x; k < want; k += kThreads) put(k, 0);
         __syncthreads();
