@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _hip
-from .scores import allowed_fields, check_device, check_tensor, current_stream, on_device
+from .scores import allowed_fields, check_device, check_tensor, launch
 
 
 class DistillGradients(NamedTuple):
@@ -79,10 +79,8 @@ def _call(users, items, bias, teacher_items, teacher_scores, temperature, allowe
     elif rows == 0:
         return loss
     lib = _hip.lib()
-    with on_device(device):
-        ws = torch.empty(lib.rfm_distill_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=device)
-        rc = lib.rfm_distill_device(C.byref(a), ws.data_ptr(), ws.numel(), current_stream(device))
-    _hip.raise_for_status(rc)
+    ws = users.new_empty(lib.rfm_distill_workspace_bytes(C.byref(a)), dtype=torch.uint8)
+    launch(device, lib.rfm_distill_device, C.byref(a), ws.data_ptr(), ws.numel())
     return DistillGradients(loss, d_users, d_items, d_bias) if gradients else loss
 
 

@@ -5,7 +5,6 @@ else holds: penalties for what a user has already had, biases, and masks of what
 MI355X; work is enqueued on that device's current stream and nothing synchronises, so the calls may be captured into a graph.
 """
 import ctypes as C
-from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -61,7 +60,8 @@ class ScoreRules:
 
     def penalises(self):
         """whether the rules look at a history at all"""
-        return any(isinstance(v, torch.Tensor) or v != off for v, off in ((self.repetition, 1.0), (self.frequency, 0.0), (self.presence, 0.0)))
+        rho, phi, pi = self.repetition, self.frequency, self.presence
+        return isinstance(rho, torch.Tensor) or isinstance(phi, torch.Tensor) or isinstance(pi, torch.Tensor) or not rho == 1.0 or not phi == 0.0 == pi
 
 
 class TopScores(NamedTuple):
@@ -97,14 +97,17 @@ def check_tensor(t, name, dtype, shape, device):
     raise ValueError("[%s] must have shape %s, got %s" % (name, list(shape), list(t.shape)))
 
 
-def on_device(device):
-    """the context in which kernels of `device` are launched: nothing where it is the current one (a small call's time is the host's)"""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def current_stream(device):
-    """the device's current stream as the C entries take it (`torch.cuda.current_stream(device).cuda_stream` without the object)"""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def launch(device, entry, *args):
+    """entry(*args, the device's current stream) with `device` the current one; the exception of its status if it refuses.  (A small call's time is the
+    host's: no stream object is made, and no device switched that is the current one)"""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        rc = entry(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args, stream)
+    if rc != _hip.OK:
+        _hip.raise_for_status(rc)
 
 
 def check_device(t, name):
@@ -118,9 +121,10 @@ def check_device(t, name):
 def _check_scores(scores):
     if not isinstance(scores, torch.Tensor) or scores.dtype not in _DTYPES or scores.dim() != 2:
         raise ValueError("[scores] must be a float32, float16 or bfloat16 tensor [rows, items]")
-    if scores.shape[1] < 1:
+    rows, items = scores.shape
+    if items < 1:
         raise ValueError("[scores] must have at least one item")
-    if scores.shape[1] > 1 and scores.stride(1) != 1 or scores.shape[0] > 1 and scores.stride(0) < scores.shape[1]:
+    if not scores.is_contiguous() and (items > 1 and scores.stride(1) != 1 or rows > 1 and scores.stride(0) < items):
         raise ValueError("[scores] must have rows of consecutive items that do not overlap")
     return check_device(scores, "scores")
 
@@ -218,10 +222,8 @@ def adjust_scores(scores, rules, out=None):
     u = _rules_struct(rules, rows, items, device)
     if rows == 0:
         return out
-    with on_device(device):
-        rc = _hip.lib().rfm_adjust_scores_device(C.byref(u), _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), out.data_ptr(),
-                                                 _row_stride(out), current_stream(device))
-    _hip.raise_for_status(rc)
+    launch(device, _hip.lib().rfm_adjust_scores_device, C.byref(u), _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), out.data_ptr(),
+           _row_stride(out))
     return out
 
 
@@ -241,9 +243,7 @@ def top_scores(scores, n, rules=None):
     if rows == 0:
         return TopScores(best, value)
     lib = _hip.lib()
-    with on_device(device):
-        ws = torch.empty(lib.rfm_top_scores_workspace_bytes(rows, items, n), dtype=torch.uint8, device=device)
-        rc = lib.rfm_top_scores_device(C.byref(u) if u is not None else None, _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), n,
-                                       best.data_ptr(), value.data_ptr(), ws.data_ptr(), ws.numel(), current_stream(device))
-    _hip.raise_for_status(rc)
+    ws = scores.new_empty(lib.rfm_top_scores_workspace_bytes(rows, items, n), dtype=torch.uint8)
+    launch(device, lib.rfm_top_scores_device, C.byref(u) if u is not None else None, _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), n,
+           best.data_ptr(), value.data_ptr(), ws.data_ptr(), ws.numel())
     return TopScores(best, value)
