@@ -400,7 +400,7 @@ static int pick_splits(int blocks, int tiles, int slots) {
 }
 
 struct FusedLayout {
-    int kp, columns, block_tiles, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, groups_i, units_i;
+    int kp, columns, block_tiles, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, lanes_f, groups_i, units_i;
     size_t part, mass, ids, ps, acc, user_frag, user_frag_t, item_frag, item_frag_t, item_data, user_data, user_data_t, mask_row, part_m, part_l, part_o, entry, entry_at, part_items, part_bias, bytes;
 };
 static FusedLayout fused_layout(const rfm_distill_args *a) {
@@ -419,7 +419,12 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     w.item_blocks = (w.item_tiles + w.block_tiles - 1) / w.block_tiles;
     // workgroups that fit on the chip at once, by registers and LDS (the loss alone needs fewer of both)
     const int slots = kCus * (w.kp > 64 ? 1 : w.columns == 2 ? 2 : 3), slots_loss = kCus * (w.kp <= 64 && w.columns == 1 ? 4 : 2);
-    w.splits_f = pick_splits(w.user_blocks, w.item_tiles, grad ? slots : slots_loss);
+    const int slots_f = grad ? slots : slots_loss;
+    w.splits_f = pick_splits(w.user_blocks, w.item_tiles, slots_f);
+    // a multiple of the 8 XCDs, where that takes no more rounds
+    const int even = (w.splits_f + 7) / 8 * 8;
+    auto rounds = [&](int each) { return ((long long)w.user_blocks * each + slots_f - 1) / slots_f; };
+    w.lanes_f = rounds(even) == rounds(w.splits_f) ? even : w.splits_f;
     // items_kernel: equal ranges for the workgroups that fit on the chip at once, no shorter than 4 tiles (or a block, if that is less)
     const long long units = (long long)w.item_blocks * w.user_tiles;
     w.units_i = (int)std::max<long long>((units + slots - 1) / slots, std::min(w.user_tiles, 4));
@@ -462,7 +467,8 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     else prepare_kernel<KP, false><<<grid_p, dim3(256), lds, stream>>>(f, c, part, mass, nullptr, nullptr, nullptr);
     f.splits = w.splits_f;
     f.chunk = (w.item_tiles + w.splits_f - 1) / w.splits_f;
-    const dim3 grid_f((unsigned)(w.user_blocks * w.splits_f)), threads(Frag<KP>::waves * 64);
+    f.lanes = w.lanes_f;
+    const dim3 grid_f((unsigned)(w.user_blocks * w.lanes_f)), threads(Frag<KP>::waves * 64);
     if constexpr (NC == 1) {
         if (grad && a->allowed) forward_kernel<KP, NC, true, true><<<grid_f, threads, 0, stream>>>(f);
         if (!grad && a->allowed) forward_kernel<KP, NC, false, true><<<grid_f, threads, 0, stream>>>(f);
