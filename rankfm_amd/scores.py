@@ -2,7 +2,8 @@
 
 The reference hands out ranked items only and knows one rule, `filter_previous` (rankfm/_rankfm.pyx:450-451).  Here the caller says what
 else holds: penalties for what a user has already had, biases, and masks of what may be shown at all.  Tensors are torch tensors on one
-MI355X; work is enqueued on that device's current stream and nothing synchronises, so the calls may be captured into a graph.
+MI355X; work is enqueued on that device's current stream and nothing synchronises, so the calls may be captured into a graph.  Nothing is
+recorded by autograd.
 """
 import ctypes as C
 from dataclasses import dataclass

@@ -345,3 +345,42 @@ def test_rows_of_very_different_size_share_a_tile(factors):
     tol = 2 * ez + eq + ep + 88 * E * big
     for got in (distill_loss(*args, **kw), distill_gradients(*args, **kw).loss):
         assert (np.abs(got.cpu().numpy() - want[0]) <= tol).all()
+
+
+def test_calls_on_two_streams_at_once():
+    """every call has a workspace of its own: many in flight on two streams, with different inputs and sizes, give what they give alone"""
+    problems = [Problem(rows=600, items=9001, factors=48, n=12, mask="few", seed=21), Problem(rows=333, items=20_005, factors=100, n=30, seed=22)]
+    given = [p.given() for p in problems]
+    alone = [distill_gradients(*args, **kw) for args, kw in given]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for s, (args, kw), out in zip(streams, given, got):
+            with torch.cuda.stream(s):
+                out.append(distill_gradients(*args, **kw))
+    torch.cuda.synchronize()
+    for want, results in zip(alone, got):
+        assert all(torch.equal(a, b) for r in results for a, b in zip(r, want))
+
+
+def test_two_graphs_in_turn_and_at_once():
+    given = [Problem(rows=90, items=1500, factors=24, n=6, seed=s).given() for s in (31, 32)]
+    want = [distill_gradients(*args, **kw) for args, kw in given]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for args, kw in given:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(distill_gradients(*args, **kw))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for h, w in zip(held, want) for a, b in zip(h, w))
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for h, w in zip(held, want) for a, b in zip(h, w))

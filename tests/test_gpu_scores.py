@@ -314,3 +314,21 @@ def test_refusals_on_the_device():
     for out in (torch.zeros(2, 5).cuda(), torch.zeros(2, 6, dtype=F16).cuda(), torch.zeros(2, 6), torch.zeros(6, 2).cuda().t()):
         with pytest.raises(ValueError):
             adjust_scores(s, ScoreRules(), out=out)
+
+
+def test_calls_on_two_streams_at_once():
+    """rows cut into segments, whose keys go through a workspace: one per call"""
+    s = [torch.randn(3, 120_001).cuda(), torch.randn(40, 30_011).cuda()]
+    want = [top_scores(x, 50) for x in s]
+    adjusted = [adjust_scores(x, ScoreRules(item_bias=torch.arange(x.shape[1], dtype=torch.float32).cuda() / 1000)) for x in s]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for st, x, out in zip(streams, s, got):
+            with torch.cuda.stream(st):
+                bias = torch.arange(x.shape[1], dtype=torch.float32, device="cuda") / 1000
+                out.append((top_scores(x, 50), adjust_scores(x, ScoreRules(item_bias=bias))))
+    torch.cuda.synchronize()
+    for w, a, results in zip(want, adjusted, got):
+        for top, rows in results:
+            assert torch.equal(top.items, w.items) and torch.equal(top.scores, w.scores) and torch.equal(rows, a)
