@@ -131,7 +131,8 @@ def _check_scores(scores):
 
 
 def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, items = t.shape
+    return t.stride(0) if rows > 1 else items              # (the stride of a single row means nothing)
 
 
 def _number_or_rows(u, name, value, rows, device):
@@ -210,7 +211,7 @@ def adjust_scores(scores, rules, out=None):
     device = _check_scores(scores)
     rows, items = scores.shape
     if out is None:
-        out = scores.new_empty((rows, items))
+        out = torch.empty_like(scores) if scores.is_contiguous() else scores.new_empty((rows, items))
     elif out is not scores:
         if not isinstance(out, torch.Tensor) or out.dtype != scores.dtype or out.shape != scores.shape or out.device != device:
             raise ValueError("[out] must be a tensor of the scores' type, shape and device")
