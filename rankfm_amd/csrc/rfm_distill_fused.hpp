@@ -5,7 +5,8 @@
 // |x x'| at most and 2^-27 in the mean: an fp32 product rounds away as much.  Three v_mfma_f32_32x32x16_f16 take 3 / 16 of the time of the
 // fp32 matrix instructions (six with bf16 parts, which hold 8 bits: the step of 8192 rows x 50 k items at k = 64 took 1164 us with those, 794 with these).
 // fp16 has little range, so every tile of 32 rows is scaled by a power of two, its largest finite value to 2^14 .. 2^15: what is 2^-16 of that
-// or more keeps its 22 bits, what is less an absolute error of 2^-40 of it.  The scales are taken back exactly where the sums are used.
+// or more keeps its 22 bits, what is less an absolute error of 2^-40 of it (the scale is 2^40 at most: 2^-65 then).  The scales are taken back
+// exactly where the sums are used.
 //
 // Fragments.  A 32 x 16 operand of that instruction is, for both sides, 8 consecutive k of row (lane & 31), k block (lane >> 5).  The tables are
 // laid out once per call in exactly that order, [tile of 32 rows][k / 16][part][lane][8], so that a wavefront's operand is a contiguous

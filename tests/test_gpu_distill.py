@@ -384,3 +384,23 @@ def test_two_graphs_in_turn_and_at_once():
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for h, w in zip(held, want) for a, b in zip(h, w))
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128, 200])
+@pytest.mark.parametrize("what", ["zero users", "zero items", "zero both", "one tile of zeros", "small"])
+def test_factors_of_nothing(factors, what):
+    """zeros: a fresh model's.  small: everything 1e-7 of the usual size, the scores all but equal and the gradients as small as the factors"""
+    p = Problem(rows=70, items=333, factors=factors, n=6, seed=15)
+    if what in ("zero users", "zero both"):
+        p.u[:] = 0
+    if what in ("zero items", "zero both"):
+        p.v[:] = 0
+    if what == "one tile of zeros":
+        p.u[32:64], p.v[64:96] = 0, 0
+    if what == "small":
+        p.u, p.v = p.u * np.float32(1e-7), p.v * np.float32(1e-7)
+    want, tol = p.exact()
+    args, kw = p.given()
+    got = distill_gradients(*args, row_weight=torch.from_numpy(p.g).cuda(), **kw)
+    for x, w, t in zip((*got, distill_loss(*args, **kw)), (*want, want[0]), (*tol, tol[0])):
+        assert (np.abs(x.cpu().numpy() - w) <= t).all()
