@@ -59,6 +59,19 @@ __device__ __forceinline__ Four load_four(const float *row, int k, int factors) 
     return x;
 }
 
+// ... and written
+__device__ __forceinline__ void store_four(float *row, int k, int factors, float a, float b, float c, float d) {
+    if (k + 4 <= factors) {
+        const Four x = {{a, b, c, d}};
+        __builtin_memcpy(reinterpret_cast<Four *>(row + k), &x, sizeof(x));
+    } else {
+        const float x[4] = {a, b, c, d};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (k + j < factors) row[k + j] = x[j];
+    }
+}
+
 // One wavefront per row: the teacher's distribution over the usable entries, and its part of the loss.
 //   part[r] = sum_j p_j (log p_j - z[r, t_j] / tau)     mass[r] = 1, 0 without a usable entry, NaN where the row's mask does not exist
 // For the gradients the list is left with the usable entries' p (-1, 0 elsewhere).  MERGE: merged too -- an item's first entry holds the sum of

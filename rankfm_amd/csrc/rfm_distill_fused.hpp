@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
             weighted_sum<KP, NC>(now + kBytes, lane, p, by, o);
         }
         __syncthreads();                                         // the buffers are free for the next block
-        const bool whole = t0 == 0 && t1 == f.user_tiles, vector = (f.a.n_factors & 3) == 0 && ((uintptr_t)f.a.d_items & 15) == 0;
+        const bool whole = t0 == 0 && t1 == f.user_tiles;
         const int K = f.a.n_factors;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
@@ -764,13 +764,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
                     for (int q = 0; q < 4; ++q) {
                         const int k = 32 * c + 8 * q + 4 * half;
                         const f32x4 v = f32x4{o[n][c][4 * q], o[n][c][4 * q + 1], o[n][c][4 * q + 2], o[n][c][4 * q + 3]} * unit_of;
-                        if (vector) {
-                            if (k < K) *reinterpret_cast<f32x4 *>(out + k) = v;
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (k + j < K) out[k + j] = v[j];
-                        }
+                        store_four(out, k, K, v[0], v[1], v[2], v[3]);
                     }
             } else if (!whole) {
                 const size_t at = ((size_t)(blockIdx.x + block) * WAVES * NC + wave * NC + n) * 32 + col;
@@ -797,10 +791,7 @@ __global__ void __launch_bounds__(256) join_items_kernel(const FusedArgs f, int 
         if (i0 + row >= f.a.n_items || k >= K) continue;
         f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int g = first; g <= last; ++g) s += *reinterpret_cast<const f32x4 *>(f.part_items + ((size_t)(g + block) * tiles * 32 + in_block + row) * KP + k);
-        float *out = f.a.d_items + (size_t)(i0 + row) * K + k;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (k + j < K) out[j] = s[j];
+        store_four(f.a.d_items + (size_t)(i0 + row) * K, k, K, s[0], s[1], s[2], s[3]);
     }
     if (!f.a.d_bias || threadIdx.x >= 32 || i0 + (int)threadIdx.x >= f.a.n_items) return;
     float s = 0.0f;
