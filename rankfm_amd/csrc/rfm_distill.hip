@@ -13,6 +13,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/rankfm_hip.h"
 
@@ -181,12 +182,13 @@ __device__ void teacher_row(const rfm_distill_args &a, long long r, int kp, int 
         mass[r] = bad ? __uint_as_float(0x7fc00000u) : some ? 1.0f : 0.0f;
     }
     if (!merged_item) return;
-    for (int j0 = 0; j0 < n; j0 += 256) {                        // four entries per lane against all of them
-        int i[4];
-        float p[4];
-        bool first[4];
+    auto merge = [&](int j0, auto slots) {                       // some entries per lane against all of them
+        constexpr int S = decltype(slots)::value;
+        int i[S];
+        float p[S];
+        bool first[S];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < S; ++q) {
             const int j = j0 + 64 * q + lane;
             i[q] = j < n ? id[j] : -1;
             p[q] = MERGE || i[q] < 0 ? 0.0f : pr[j];
@@ -198,7 +200,7 @@ __device__ void teacher_row(const rfm_distill_args &a, long long r, int kp, int 
                 const int at = id[k];
                 const float more = pr[k];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int q = 0; q < S; ++q) {
                     const bool twin = at == i[q];
                     first[q] &= !twin || k >= j0 + 64 * q + lane;
                     p[q] += twin ? more : 0.0f;
@@ -206,7 +208,7 @@ __device__ void teacher_row(const rfm_distill_args &a, long long r, int kp, int 
             }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < S; ++q) {
             const int j = j0 + 64 * q + lane;
             const bool on = i[q] >= 0 && first[q] && !bad;
             if (j < n) {
@@ -214,7 +216,11 @@ __device__ void teacher_row(const rfm_distill_args &a, long long r, int kp, int 
                 merged_p[(size_t)r * n + j] = on ? p[q] * inv : 0.0f;
             }
         }
-    }
+    };
+    int j0 = 0;
+    for (; n - j0 > 128; j0 += 256) merge(j0, std::integral_constant<int, 4>());
+    if (n - j0 > 64) merge(j0, std::integral_constant<int, 2>());
+    else if (n > j0) merge(j0, std::integral_constant<int, 1>());
 }
 __global__ void __launch_bounds__(256) teacher_kernel(const rfm_distill_args a, float *__restrict__ part, float *__restrict__ mass, int32_t *__restrict__ merged_item,
                                                       float *__restrict__ merged_p) {

@@ -790,11 +790,21 @@ __global__ void __launch_bounds__(256) join_items_kernel(const FusedArgs f, int 
         const int row = e / (KP / 4), k = e % (KP / 4) * 4;
         if (i0 + row >= f.a.n_items || k >= K) continue;
         f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int g = first; g <= last; ++g) s += *reinterpret_cast<const f32x4 *>(f.part_items + ((size_t)(g + block) * tiles * 32 + in_block + row) * KP + k);
+        const float *from = f.part_items + ((size_t)block * tiles * 32 + in_block + row) * KP + k;
+        int g = first;
+        for (; g + 3 <= last; g += 4) {                          // (four loads in flight)
+            f32x4 x[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) x[h] = *reinterpret_cast<const f32x4 *>(from + (size_t)(g + h) * tiles * 32 * KP);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) s += x[h];
+        }
+        for (; g <= last; ++g) s += *reinterpret_cast<const f32x4 *>(from + (size_t)g * tiles * 32 * KP);
         store_four(f.a.d_items + (size_t)(i0 + row) * K, k, K, s[0], s[1], s[2], s[3]);
     }
     if (!f.a.d_bias || threadIdx.x >= 32 || i0 + (int)threadIdx.x >= f.a.n_items) return;
     float s = 0.0f;
+#pragma unroll 8
     for (int g = first; g <= last; ++g) s += f.part_bias[(size_t)(g + block) * tiles * 32 + in_block + threadIdx.x];
     f.a.d_bias[i0 + threadIdx.x] = s;
 }
