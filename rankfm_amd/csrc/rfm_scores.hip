@@ -330,7 +330,8 @@ template <bool RULED> struct Top {
     static constexpr int buf = RULED ? 512 : 1024;               // candidates a wavefront holds
     static constexpr int round = buf / 2;        // most entries kept at a time; a longer list is taken in rounds of this many
 };
-constexpr int kSlots = 1024, kShort = 512;       // hash slots for the items that a row's lists name; lists of more entries than kShort are scanned per tile
+constexpr int kSlots = 1024;                     // hash slots for the items that a row's lists name
+constexpr int kFull = kSlots - kThreads;         // lists that name more are scanned once per tile instead
 constexpr int kWindow = 65536;                   // items whose membership bits are in LDS at a time
 
 // x of lane ^ J.  Inside a row of 16 lanes that is an operand's modifier (DPP), inside 32 a fixed pattern, beyond a shuffle
@@ -407,9 +408,10 @@ __device__ __forceinline__ void sort_in_place(u64 *buf, int m, int lane) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
-// what a row's lists name, when they are short: a hash table of the items with their counts and last bias entries, and a bit per item of a window
+// what a row's lists name of a segment, when that is not much: a hash table of the items with their counts and last bias entries, and a bit per item of a
+// window
 struct Listed {
-    int id[kSlots], count[kSlots], last[kSlots];
+    int used, id[kSlots], count[kSlots], last[kSlots];
     unsigned bits[kWindow / 32];
 };
 struct Tiled {
@@ -420,26 +422,40 @@ union ListMemory {
     Tiled tiled;
 };
 
-__device__ __forceinline__ void hash_lists(const RowRules &w, int n_items, Listed &m) {
+// false: there are too many of them for the table
+__device__ __forceinline__ bool hash_lists(const RowRules &w, int begin, int end, Listed &m) {
     for (int k = threadIdx.x; k < kSlots; k += kThreads) { m.id[k] = -1; m.count[k] = 0; m.last[k] = 0; }
+    if (threadIdx.x == 0) m.used = 0;
     __syncthreads();
-    auto slot_of = [&](int item) {                               // (at most kShort of kSlots are taken: the walk ends)
+    // (the walk ends: a table of more than kFull items is given up, and the threads that had not seen that yet fit in)
+    auto slot_of = [&](int item) {
         unsigned at = (unsigned)item * 2654435761u >> 22;
-        for (;;) {
+        while (__hip_atomic_load(&m.used, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) <= kFull) {
             const int was = atomicCAS(m.id + at, -1, item);
-            if (was == -1 || was == item) return at;
+            if (was == -1) atomicAdd(&m.used, 1);
+            if (was == -1 || was == item) return (int)at;
             at = (at + 1) & (kSlots - 1);
         }
+        return -1;
     };
     for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) {
         const int i = w.hist[k];
-        if (i >= 0 && i < n_items) atomicAdd(m.count + slot_of(i), 1);
+        if (i >= begin && i < end) {
+            const int at = slot_of(i);
+            if (at < 0) break;
+            atomicAdd(m.count + at, 1);
+        }
     }
     for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) {
         const int i = w.bias_item[k];
-        if (i >= 0 && i < n_items) atomicMax(m.last + slot_of(i), (int)k + 1);
+        if (i >= begin && i < end) {
+            const int at = slot_of(i);
+            if (at < 0) break;
+            atomicMax(m.last + at, (int)k + 1);
+        }
     }
     __syncthreads();
+    return m.used <= kFull;
 }
 __device__ __forceinline__ void window_bits(Listed &m, int first) {
     __syncthreads();                                             // (nobody reads the last window's any more)
@@ -470,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
     constexpr int kAll = kSuper * kPer, ve = FROM_KEYS ? 1 : Vec<T>::n;
     __shared__ u64 buf[kWaves * kBuf];
     __shared__ typename std::conditional<RULED, ListMemory, int>::type lists_memory;
-    __shared__ unsigned wave_t[kWaves];
+    __shared__ unsigned wave_t[kWaves], wave_q[kWaves];
     __shared__ int wave_m[kWaves];
     __shared__ u64 last_key;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -479,27 +495,68 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
     const int begin = FROM_KEYS ? 0 : seg * segment, end = FROM_KEYS ? n_keys : min(n_items - begin, segment) + begin;
     RowRules w;
     if constexpr (RULED) w = row_rules(u, r, n_items);
-    const bool listed = RULED && (w.hist_n > 0 || w.bias_n > 0), hashed = listed && w.hist_n + w.bias_n <= kShort;
+    const bool listed = RULED && (w.hist_n > 0 || w.bias_n > 0);
+    bool hashed = false;
     const T *row = FROM_KEYS ? nullptr : scores + r * stride;
     const u64 *krow = FROM_KEYS ? keys_in + (size_t)(r - row0) * n_keys : nullptr;
     u64 *mine = buf + wave * kBuf;
     if constexpr (RULED)
-        if (hashed) hash_lists(w, n_items, lists_memory.listed);
+        if (listed && end - begin > kSuper * kTile) hashed = hash_lists(w, begin, end, lists_memory.listed);
     u64 ceiling = ~0ull;                                         // keys of earlier rounds are at or above it
     for (int base = 0; base < n; base += kRound) {
         const int want = min(n - base, kRound);
+        if (threadIdx.x < kWaves) wave_q[threadIdx.x] = 0;      // (a barrier comes before the first is looked at: the first threshold's)
         u64 thr = 0;                                             // a key passes when it is above; a score is looked at when it is `reach` or more
         float reach = -3.402823466e38f;
         int m = 0;
+        // The wavefront's part of LDS is full: the value that its n-th best reaches and the least of the four values that a quarter of n of each wavefront's
+        // reach (as far as they have come there) are thresholds for everyone; what is above stays.  Found by bisection over ballots, cut to 20 bits,
+        // a sort only where too many are equal.
+        auto make_room = [&]() {
+            unsigned v[kBuf / 64];
+#pragma unroll
+            for (int k = 0; k < kBuf / 64; ++k) v[k] = k * 64 + lane < m ? (unsigned)(mine[k * 64 + lane] >> 32) : 0u;
+            unsigned whole = 0, quarter = 0;
+            for (int bit = 31; bit >= 12; --bit) {
+                const unsigned cw = whole | (1u << bit), cq = quarter | (1u << bit);
+                int nw = 0, nq = 0;
+#pragma unroll
+                for (int k = 0; k < kBuf / 64; ++k) { nw += __popcll(__ballot(v[k] >= cw)); nq += __popcll(__ballot(v[k] >= cq)); }
+                if (nw >= want) whole = cw;
+                if (nq >= (want + kWaves - 1) / kWaves) quarter = cq;
+            }
+            if (lane == 0) __hip_atomic_store(wave_q + wave, quarter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            unsigned least = quarter;                            // (0 as long as one of them has not been full)
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+                if (w != wave) least = min(least, __hip_atomic_load(wave_q + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+            const unsigned t = max(whole, least);
+            thr = max(thr, ((u64)t << 32) - (t ? 1 : 0));
+            int kept = 0;
+#pragma unroll 1
+            for (int k = 0; k < m; k += 64) {
+                const u64 key = k + lane < m ? mine[k + lane] : 0;
+                const bool stays = key > thr;
+                const unsigned long long who = __ballot(stays);
+                if (stays) mine[kept + __popcll(who & ((1ull << lane) - 1))] = key;
+                kept += __popcll(who);
+            }
+            m = kept;
+            if (m > kBuf / 4 * 3) {                              // many of the same value: the first ones stay
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                sort_in_place(mine, m, lane);
+                m = want;                                        // (less than half of the buffer)
+                thr = max(thr, mine[want - 1]);
+            }
+            reach = key_score(thr);
+        };
         auto keep = [&](bool pass, u64 key) {                    // (by whole wavefronts)
             pass = pass && key > thr && key < ceiling;
             const unsigned long long who = __ballot(pass);
             if (!who) return;
             if (m > kBuf - 64) {
-                sort_in_place(mine, m, lane);
-                m = want;                                        // (m > kBuf - 64 >= want)
-                thr = max(thr, mine[want - 1]);
-                reach = key_score(thr);
+                make_room();
                 pass = pass && key > thr;
             }
             const unsigned long long still = __ballot(pass);

@@ -332,3 +332,43 @@ def test_calls_on_two_streams_at_once():
     for w, a, results in zip(want, adjusted, got):
         for top, rows in results:
             assert torch.equal(top.items, w.items) and torch.equal(top.scores, w.scores) and torch.equal(rows, a)
+
+
+@pytest.mark.parametrize("listed, kinds", [(700, 1), (760, 760), (769, 769), (1024, 1024), (2000, 767), (2000, 770), (5000, 40), (5000, 5000)])
+@pytest.mark.parametrize("rows, items", [(2, 9000), (3, 60_007)], ids=["one segment or two", "many segments"])
+def test_top_scores_under_long_lists(rows, items, listed, kinds):
+    """lists of `listed` entries that name `kinds` different items: few enough for the table of items, just too many, far too many"""
+    rng = np.random.default_rng(listed + kinds)
+    p = Problem(rows, items, seed=listed, history=4, row_bias=3, item_bias=True, masks=rows)
+    p.hist = [rng.choice(items, kinds, replace=False)[rng.permutation(np.arange(listed) % kinds)] for _ in range(rows)]
+    p.hist_rows = np.arange(rows, dtype=np.int32)[::-1].copy()
+    p.mask[0] = True
+    adjusted = p.plain(np.float32)[0]
+    for n in (5, 300):
+        got = top_scores(p.s.cuda(), n, p.rules())
+        want_items, want_values = plain_top(adjusted, n)
+        assert np.array_equal(got.items.cpu().numpy(), want_items) and np.array_equal(got.scores.cpu().numpy(), want_values)
+    assert same(adjust_scores(p.s.cuda(), p.rules()).cpu(), torch.from_numpy(adjusted))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["normal", "few values", "ascending", "late"])
+def test_long_lists_of_long_rows(dtype, kind):
+    """more candidates than a wavefront holds, again and again: thresholds from what it has, shared among the four"""
+    rng = np.random.default_rng(8)
+    if kind == "normal":
+        s = rng.standard_normal((600, 40_003))
+    elif kind == "few values":
+        s = rng.integers(0, 5, (600, 40_003)) - 2.0
+    elif kind == "ascending":
+        s = np.sort(rng.standard_normal((600, 40_003)))
+    else:                                                                        # all that counts stands in what one wavefront reads
+        s = rng.standard_normal((600, 40_003)) * 0.01
+        s[:, 20_000:20_256] += 3.0
+    s = torch.from_numpy(s.astype(np.float32)).to(dtype)
+    for n in (200, 500, 513):
+        got = top_scores(s.cuda(), n)
+        want_items, want_values = plain_top(s[:5].float().numpy(), n)
+        assert np.array_equal(got.items[:5].cpu().numpy(), want_items) and np.array_equal(got.scores[:5].cpu().numpy(), want_values)
+        value, _ = torch.sort(s.cuda().float(), dim=1, descending=True)
+        assert torch.equal(got.scores, value[:, :n])
