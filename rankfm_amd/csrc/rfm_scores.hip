@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
         int m = 0;
         // The wavefront's part of LDS is full: the value that its n-th best reaches and the least of the four values that a quarter of n of each wavefront's
         // reach (as far as they have come there) are thresholds for everyone; what is above stays.  Found by bisection over ballots, cut to 20 bits,
-        // a sort only where too many are equal.
+        // a sort only where too many are equal.  (Sorting, and each wavefront its own n-th best alone: 500 rows of 190 k, 500 wanted, 305 us; 179 so.)
         auto make_room = [&]() {
             unsigned v[kBuf / 64];
 #pragma unroll
