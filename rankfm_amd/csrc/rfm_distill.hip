@@ -405,6 +405,7 @@ static int run_matrix(const rfm_distill_args *a, char *base, hipStream_t stream)
 // How often the streamed tiles are split: workgroups run `slots` at a time, a workgroup costs its tiles and about four more to start and end,
 // a split costs its partial sums.  The cheapest count wins; the sums of a count are always joined in the same order.
 constexpr int kCus = 256;
+constexpr int kThinItems = 256;                  // tiles of items from which few users are taken without copies
 static int pick_splits(int blocks, int tiles, int slots) {
     int best = 1;
     double least = 1e30;
@@ -419,7 +420,7 @@ static int pick_splits(int blocks, int tiles, int slots) {
 }
 
 struct FusedLayout {
-    int kp, columns, block_tiles, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, lanes_f, groups_i, units_i;
+    int kp, few, columns, block_tiles, user_tiles, item_tiles, user_blocks, item_blocks, splits_f, lanes_f, groups_i, units_i;
     size_t part, mass, ids, ps, acc, user_frag, user_frag_t, item_frag, item_frag_t, item_data, user_data, user_data_t, mask_row, part_m, part_l, part_o, entry, entry_at, part_items, part_bias, bytes;
 };
 static FusedLayout fused_layout(const rfm_distill_args *a) {
@@ -429,10 +430,13 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     const size_t R = (size_t)a->n_rows, n = (size_t)a->n_teacher, kp = (size_t)w.kp;
     w.user_tiles = (int)((a->n_rows + 31) / 32);
     w.item_tiles = (a->n_items + 31) / 32;
+    // Few users: no copies of the items' table are made (thin_forward_kernel).
+    const bool thin = w.user_tiles <= 2 && w.item_tiles >= kThinItems;
+    w.few = thin ? w.user_tiles : 0;
     // Column tiles per wavefront: two read LDS half as often, one leaves more workgroups to spread.  Measured with two against one, k = 64, gradients / loss
     // alone: 512 rows x 50 k items 1.10 / 1.13, 2048 x 50 k 1.01 / 0.96, 4096 x 20 k 1.00 / 0.95, 4096 x 50 k 0.95 / 0.93, 2048 x 200 k 0.96 / 0.93; k = 20
     // crosses at the same place; with masks one is the faster throughout (2048 x 50 k 1.06).
-    w.columns = w.kp <= 64 && !a->allowed && (long long)w.user_tiles * w.item_tiles >= (1 << 17) ? 2 : 1;
+    w.columns = !thin && w.kp <= 64 && !a->allowed && (long long)w.user_tiles * w.item_tiles >= (1 << 17) ? 2 : 1;
     w.block_tiles = (w.kp <= 64 ? 4 : 8) * w.columns;
     w.user_blocks = (w.user_tiles + w.block_tiles - 1) / w.block_tiles;
     w.item_blocks = (w.item_tiles + w.block_tiles - 1) / w.block_tiles;
@@ -444,6 +448,10 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     const int even = (w.splits_f + 7) / 8 * 8;
     auto rounds = [&](int each) { return ((long long)w.user_blocks * each + slots_f - 1) / slots_f; };
     w.lanes_f = rounds(even) == rounds(w.splits_f) ? even : w.splits_f;
+    if (w.few) {                                 // workgroups, each with 8 / few tiles of items at a time
+        const int at_once = kThinWaves / w.few;
+        w.splits_f = w.lanes_f = std::min(kCus, (w.item_tiles + at_once - 1) / at_once);
+    }
     // items_kernel: equal ranges for the workgroups that fit on the chip at once, no shorter than 4 tiles (or a block, if that is less)
     const long long units = (long long)w.item_blocks * w.user_tiles;
     w.units_i = (int)std::max<long long>((units + slots - 1) / slots, std::min(w.user_tiles, 4));
@@ -453,8 +461,8 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     auto take = [&](size_t bytes) { const size_t at = off; off += up(bytes ? bytes : 1); return at; };
     w.part = take(4 * R); w.mass = take(4 * R);
     w.ids = take(grad ? 4 * R * n : 0); w.ps = take(grad ? 4 * R * n : 0); w.acc = take(grad ? 4 * R * kp : 0);
-    w.user_frag = take(4 * ur * kp); w.item_frag = take(4 * ir * kp);
-    w.user_frag_t = take(grad ? 4 * ur * kp : 0); w.item_frag_t = take(grad ? 4 * ir * kp : 0);
+    w.user_frag = take(4 * ur * kp); w.item_frag = take(w.few ? 0 : 4 * ir * kp);
+    w.user_frag_t = take(grad ? 4 * ur * kp : 0); w.item_frag_t = take(grad && !w.few ? 4 * ir * kp : 0);
     w.item_data = take((size_t)w.item_tiles * kItemData * 4); w.user_data = take((size_t)w.user_tiles * kUserData * 4); w.user_data_t = take((size_t)w.user_tiles * kUserData * 4);
     w.mask_row = take(a->allowed ? 4 * ur : 0);
     w.part_m = take(4 * w.splits_f * ur); w.part_l = take(4 * w.splits_f * ur); w.part_o = take(grad ? 4 * w.splits_f * ur * kp : 0);
@@ -480,28 +488,46 @@ static int run_fused(const rfm_distill_args *a, const FusedLayout &w, char *base
     f.entry = (uint2 *)at(w.entry); f.entry_at = (int32_t *)at(w.entry_at);
     f.part_items = (float *)at(w.part_items); f.part_bias = (float *)at(w.part_bias);
     const float c = 1.4426950408889634f / a->temperature;
+    f.c = c;
+    f.few = w.few;
     const size_t lds = (size_t)a->n_teacher * 2 * 4 * 4;
-    const dim3 grid_p((unsigned)(w.user_tiles + w.item_tiles + (a->n_rows + 3) / 4));
+    const dim3 grid_p((unsigned)(w.user_tiles + (w.few ? 0 : w.item_tiles) + (a->n_rows + 3) / 4));
     if (grad) prepare_kernel<KP, true><<<grid_p, dim3(256), lds, stream>>>(f, c, part, mass, ids, ps, acc);
     else prepare_kernel<KP, false><<<grid_p, dim3(256), lds, stream>>>(f, c, part, mass, nullptr, nullptr, nullptr);
     f.splits = w.splits_f;
     f.chunk = (w.item_tiles + w.splits_f - 1) / w.splits_f;
     f.lanes = w.lanes_f;
     const dim3 grid_f((unsigned)(w.user_blocks * w.lanes_f)), threads(Frag<KP>::waves * 64);
-    if constexpr (NC == 1) {
-        if (grad && a->allowed) forward_kernel<KP, NC, true, true><<<grid_f, threads, 0, stream>>>(f);
-        if (!grad && a->allowed) forward_kernel<KP, NC, false, true><<<grid_f, threads, 0, stream>>>(f);
+    if (w.few) {
+        if constexpr (NC == 1) {
+            const dim3 grid_t((unsigned)w.splits_f), threads_t(kThinWaves * 64);
+            if (grad && a->allowed) thin_forward_kernel<KP, true, true><<<grid_t, threads_t, 0, stream>>>(f);
+            if (!grad && a->allowed) thin_forward_kernel<KP, false, true><<<grid_t, threads_t, 0, stream>>>(f);
+            if (grad && !a->allowed) thin_forward_kernel<KP, true, false><<<grid_t, threads_t, 0, stream>>>(f);
+            if (!grad && !a->allowed) thin_forward_kernel<KP, false, false><<<grid_t, threads_t, 0, stream>>>(f);
+        }
+    } else {
+        if constexpr (NC == 1) {
+            if (grad && a->allowed) forward_kernel<KP, NC, true, true><<<grid_f, threads, 0, stream>>>(f);
+            if (!grad && a->allowed) forward_kernel<KP, NC, false, true><<<grid_f, threads, 0, stream>>>(f);
+        }
+        if (grad && !a->allowed) forward_kernel<KP, NC, true, false><<<grid_f, threads, 0, stream>>>(f);
+        if (!grad && !a->allowed) forward_kernel<KP, NC, false, false><<<grid_f, threads, 0, stream>>>(f);
     }
-    if (grad && !a->allowed) forward_kernel<KP, NC, true, false><<<grid_f, threads, 0, stream>>>(f);
-    if (!grad && !a->allowed) forward_kernel<KP, NC, false, false><<<grid_f, threads, 0, stream>>>(f);
-    const int row_blocks = w.user_tiles * 4;
-    join_rows_kernel<KP><<<dim3((unsigned)(row_blocks + (grad ? w.user_tiles : 0))), dim3(512), 0, stream>>>(f, row_blocks, w.block_tiles * 32, part, mass, acc, ids, ps);
+    const bool wide = w.user_tiles <= 8 && w.splits_f > 64;      // (few rows, many splits)
+    const int row_blocks = w.user_tiles * (wide ? 32 : 4);
+    const dim3 grid_j((unsigned)(row_blocks + (grad ? w.user_tiles : 0)));
+    if (wide) join_rows_kernel<KP, 8><<<grid_j, dim3(512), 0, stream>>>(f, row_blocks, w.block_tiles * 32, part, mass, acc, ids, ps);
+    else join_rows_kernel<KP, 1><<<grid_j, dim3(512), 0, stream>>>(f, row_blocks, w.block_tiles * 32, part, mass, acc, ids, ps);
     if (!grad) return RFM_OK;
     f.units = w.units_i;
     const dim3 grid_i((unsigned)w.groups_i);
-    if constexpr (NC == 1)
-        if (a->allowed) items_kernel<KP, NC, true><<<grid_i, threads, 0, stream>>>(f);
-    if (!a->allowed) items_kernel<KP, NC, false><<<grid_i, threads, 0, stream>>>(f);
+    if constexpr (NC == 1) {
+        if (w.few && a->allowed) items_kernel<KP, NC, true, true><<<grid_i, threads, 0, stream>>>(f);
+        if (w.few && !a->allowed) items_kernel<KP, NC, false, true><<<grid_i, threads, 0, stream>>>(f);
+        if (!w.few && a->allowed) items_kernel<KP, NC, true><<<grid_i, threads, 0, stream>>>(f);
+    }
+    if (!w.few && !a->allowed) items_kernel<KP, NC, false><<<grid_i, threads, 0, stream>>>(f);
     // (a block is cut where a range ends inside it)
     if (w.groups_i > 1 && w.units_i % w.user_tiles != 0) join_items_kernel<KP><<<dim3((unsigned)(w.item_blocks * w.block_tiles)), dim3(256), 0, stream>>>(f, w.block_tiles);
     return RFM_OK;

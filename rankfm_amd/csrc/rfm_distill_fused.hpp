@@ -58,6 +58,8 @@ struct FusedArgs {
     int user_tiles, item_tiles, item_blocks;     // tiles of 32 rows; blocks of items_kernel's workgroups
     int splits, chunk, lanes;                    // forward: how the item tiles are split; workgroups that a block of users is given (`splits`, or a few more)
     int units;                                   // items: (block, user tile) pairs per workgroup
+    int few;                                     // user tiles, rounded up to a power of two, where they are few (thin_forward_kernel); else 0
+    float c;                                     // log2 e / temperature
     char *user_frag, *user_frag_t, *item_frag, *item_frag_t;
     float *item_data, *user_data, *user_data_t;  // [item_tiles, kItemData], [user_tiles, kUserData] twice
     int32_t *mask_row;                           // [user_tiles * 32] mask of each row, -1 = none, -2 = a row that counts nowhere
@@ -447,15 +449,210 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (GRAD ? kPerSimd<KP, NC>
     }
 }
 
-// One wavefront per row: the splits joined; loss, the users' gradient, and what items_kernel needs of the row.  weight: 64 floats of LDS
+// ---- Few users -----------------------------------------------------------------------------------------------------------------------------
+// With one or two tiles of users the items' two copies cost more than what is done with them: 4 x the table's bytes written and read again.  Here they
+// are not made.  A wavefront takes a tile of 32 items from the table itself -- its rows are the lanes, 8 factors each per step, as the operand wants
+// them -- cuts it into parts in its registers, and passes the parts through LDS (a word per factor: both parts) for the second product, where the lanes
+// are the factors.  Nothing is shared and nobody waits; the wavefronts of a workgroup that have the same users join their sums at the end.
+//
+// A tile of a table, the lane's factors of its row in operand order; the exponent of its scale is returned.  odd: something in it is not finite.
 template <int KP>
-__device__ void join_row(const FusedArgs &f, long long r, const float *__restrict__ part, const float *__restrict__ mass, const float *__restrict__ acc, float *weight) {
+__device__ __forceinline__ int raw_tile(const float *__restrict__ table, long long stride, int tile, int rows, int factors, int lane, Four (*raw)[2], bool &odd) {
+    const int half = lane >> 5, row = tile * 32 + (lane & 31);
+    const float *from = table + (size_t)min(row, rows - 1) * stride;
+#pragma unroll
+    for (int s = 0; s < Frag<KP>::steps; ++s)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) raw[s][q] = load_four(from, 16 * s + 8 * half + 4 * q, factors);
+    if (tile * 32 + 32 > rows) {                                 // (the same for all)
+#pragma unroll
+        for (int s = 0; s < Frag<KP>::steps; ++s)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[s][q].v[j] = row < rows ? raw[s][q].v[j] : 0.0f;
+    }
+    unsigned most = 0;                                           // |x| orders like its bits; what is not finite lies above all that is
+#pragma unroll
+    for (int s = 0; s < Frag<KP>::steps; ++s)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = max(most, __float_as_uint(raw[s][q].v[j]) & 0x7fffffffu);
+    odd = __any(most >= 0x7f800000u);
+    if (odd) {
+        most = 0;
+#pragma unroll
+        for (int s = 0; s < Frag<KP>::steps; ++s)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned b = __float_as_uint(raw[s][q].v[j]) & 0x7fffffffu;
+                    most = b < 0x7f800000u ? max(most, b) : most;
+                }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, d));
+    return tile_exponent(__uint_as_float(most));
+}
+// ... and one step of it as an operand, by = 2^e
+__device__ __forceinline__ void raw_step(const Four *raw, float by, f16x8 *x) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        _Float16 h, m;
+        split2(raw[j >> 2].v[j & 3] * by, h, m);
+        x[0][j] = h; x[1][j] = m;
+    }
+}
+
+constexpr int kThinWaves = 8;
+template <int KP, bool GRAD> constexpr int kThinPerSimd = KP <= (GRAD ? 32 : 64) ? 4 : 2;
+// Workgroup b: its wavefronts are f.few tiles of users times 8 / f.few tiles of items, which go round all workgroups.
+template <int KP, bool GRAD, bool MASK>
+__global__ void __launch_bounds__(kThinWaves * 64, (kThinPerSimd<KP, GRAD>)) thin_forward_kernel(const FusedArgs f) {
+    constexpr int ld = KP + 4;
+    __shared__ __attribute__((aligned(16))) unsigned words[GRAD ? kThinWaves : 1][GRAD ? 32 * ld : 4];
+    __shared__ __attribute__((aligned(16))) float row_bias[kThinWaves][32];
+    __shared__ float tops[kThinWaves][32], totals[kThinWaves][32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int user = wave & (f.few - 1), group = wave / f.few, groups = kThinWaves / f.few, mine = min(user, f.user_tiles - 1);
+    f16x8 x[Frag<KP>::steps][2];
+    load_columns<KP>(f.user_frag, mine, lane, x);
+    const float unscale = f.user_data[(size_t)mine * kUserData + 32];
+    const uint32_t *mask = nullptr;
+    if constexpr (MASK) {
+        const int m = f.mask_row[mine * 32 + col];
+        if (m >= 0) mask = f.a.allowed + (size_t)m * (size_t)f.item_tiles;
+    }
+    float top = kLowest, total = 0.0f;
+    f32x16 o[GRAD ? Frag<KP>::cols : 1];
+    for (int c = 0; c < (GRAD ? Frag<KP>::cols : 1); ++c) o[c] = f32x16{0};
+    const int last_tile = user < f.user_tiles ? f.item_tiles : 0;
+    for (int tile = (int)blockIdx.x * groups + group; tile < last_tile; tile += (int)gridDim.x * groups) {
+        const int item = tile * 32 + col;
+        const float b_of = item < f.a.n_items ? (f.a.bias ? f.a.bias[item] * f.c : 0.0f) : -INFINITY;
+        unsigned word = 0xffffffffu;
+        if constexpr (MASK)
+            if (mask) word = mask[tile];
+        Four raw[Frag<KP>::steps][2];
+        bool odd;
+        const int e_tile = raw_tile<KP>(f.a.items, f.a.item_stride, tile, f.a.n_items, f.a.n_factors, lane, raw, odd);
+        const float e = (float)e_tile, unit = ldexpf(unscale, -e_tile), scale = ldexpf(1.0f, e_tile);
+        if (half == 0) row_bias[wave][col] = b_of;
+        f32x16 s = f32x16{0};
+#pragma unroll
+        for (int k = 0; k < Frag<KP>::steps; ++k) {
+            f16x8 a[2];
+            raw_step(raw[k], scale, a);
+            s = mfma3(a, x[k], s);
+            if constexpr (GRAD) {
+                const u32x4 h = __builtin_bit_cast(u32x4, a[0]), m = __builtin_bit_cast(u32x4, a[1]);
+                u32x4 w[2];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j >> 2][j & 3] = __builtin_amdgcn_perm(m[j >> 1], h[j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+                if (odd) {                                       // (a part h that is not finite is one whose factor is not)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j >> 2][j & 3] = (w[j >> 2][j & 3] & 0x7c00u) == 0x7c00u ? 0u : w[j >> 2][j & 3];
+                }
+                u32x4 *to = reinterpret_cast<u32x4 *>(words[wave] + col * ld + 16 * k + 8 * half);
+                to[0] = w[0];
+                to[1] = w[1];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const f32x4 *data = reinterpret_cast<const f32x4 *>(row_bias[wave]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {                            // z in log2 units
+            const f32x4 b = data[half + 2 * q];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(s[4 * q + k], unit, b[k]);
+        }
+        if constexpr (MASK) mask16(s, word >> (4 * half));
+        const float high = largest16(s) - e;
+        float by = 1.0f;
+        if (__any(high > top + (kLimit - kUnit))) {
+            const float to = fmaxf(top, ceilf(fmaxf(high, __shfl_xor(high, 32))));
+            by = __builtin_amdgcn_exp2f(top - to);
+            top = to;
+        }
+        const float off = top + (e - kUnit);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - off);
+        total = fmaf(sum16(s), scale, total * by);
+        if constexpr (GRAD) {
+            f16x8 p[2][2];
+            split_weights(s, p);
+#pragma unroll
+            for (int c = 0; c < Frag<KP>::cols; ++c) {
+                f32x16 sum = f32x16{0};
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    u32x4 h, m;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {                // rows 2 j and 2 j + 1 of this lane's eight
+                        const int r = 16 * t + ((2 * j) & 3) + 8 * (j >> 1) + 4 * half;
+                        const unsigned w0 = words[wave][r * ld + 32 * c + col], w1 = words[wave][(r + 1) * ld + 32 * c + col];
+                        h[j] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+                        m[j] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+                    }
+                    const f16x8 parts[2] = {__builtin_bit_cast(f16x8, h), __builtin_bit_cast(f16x8, m)};
+                    sum = mfma3(parts, p[t], sum);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[c][r] = fmaf(o[c][r], by, sum[r]);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // the wavefronts of the same users, in their order
+    const float sum = total + __shfl_xor(total, 32);
+    if (half == 0) { tops[wave][col] = top; totals[wave][col] = sum; }
+    __syncthreads();
+    float highest = kLowest;
+    for (int g = 0; g < groups; ++g) highest = fmaxf(highest, tops[g * f.few + user][col]);
+    const float part = __builtin_amdgcn_exp2f(top - highest);
+    const size_t at = (size_t)blockIdx.x * f.user_tiles * 32 + (size_t)user * 32 + col;
+    if (group == 0 && half == 0 && user < f.user_tiles) {
+        float all = 0.0f;
+        for (int g = 0; g < groups; ++g) all = fmaf(totals[g * f.few + user][col], __builtin_amdgcn_exp2f(tops[g * f.few + user][col] - highest), all);
+        f.part_m[at] = highest;
+        f.part_l[at] = all;
+    }
+    if constexpr (GRAD) {
+        float *joined = reinterpret_cast<float *>(words[user]);  // (nobody needs the words any more)
+        for (int g = 0; g < groups; ++g) {
+            if (g == group && user < f.user_tiles) {
+#pragma unroll
+                for (int c = 0; c < Frag<KP>::cols; ++c)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        f32x4 *cell = reinterpret_cast<f32x4 *>(joined + col * ld + 32 * c + 8 * q + 4 * half);
+                        f32x4 v = f32x4{o[c][4 * q], o[c][4 * q + 1], o[c][4 * q + 2], o[c][4 * q + 3]} * part;
+                        if (g > 0) v += *cell;
+                        if (g < groups - 1) *cell = v;
+                        else *reinterpret_cast<f32x4 *>(f.part_o + at * KP + 32 * c + 8 * q + 4 * half) = v;
+                    }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// The splits of a row joined: loss, the users' gradient, and what items_kernel needs of the row.  W: wavefronts per row, this one the `share`-th (more than
+// one where rows are few and splits are many: 29 rows, 256 splits, k = 96: 16.9 us by one, 8.5 by eight).  weight: 64 floats of LDS, sums: W x (KP + 1)
+template <int KP, int W>
+__device__ void join_row(const FusedArgs &f, long long r, int share, const float *__restrict__ part, const float *__restrict__ mass, const float *__restrict__ acc, float *weight,
+                         float *sums) {
     const int lane = threadIdx.x & 63;
     const long long padded = (long long)f.user_tiles * 32;
     const bool grad = f.a.d_users != nullptr;
     const size_t at = (size_t)(r >> 5) * kUserData + (r & 31);
     const float has = r < f.a.n_rows ? mass[r] : 0.0f;
-    if (!(has > 0.0f)) {                                         // no row, nothing to learn from, or a mask that does not exist
+    if (!(has > 0.0f)) {                                         // no row, nothing to learn from, or a mask that does not exist (the same for the W)
+        if (share > 0) return;
         if (r < f.a.n_rows) {
             if (lane == 0) f.a.loss[r] = has;                    // (0 or NaN)
             if (grad)
@@ -472,7 +669,7 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
     const int mine = lane / (KP / 4), k4 = lane % (KP / 4) * 4;
     float total = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = 0; s0 < f.splits; s0 += 64) {
+    for (int s0 = share * 64; s0 < f.splits; s0 += 64 * W) {
         const int s = s0 + lane;
         const float w = s < f.splits ? __builtin_amdgcn_exp2f(f.part_m[(size_t)s * padded + r] - top) : 0.0f;
         if (s < f.splits) total += f.part_l[(size_t)s * padded + r] * w;
@@ -501,6 +698,32 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
         __builtin_amdgcn_wave_barrier();
     }
     total = wave_sum(total);
+    if (grad) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float sum = o[j];
+            for (int d = 1; d < at_once; ++d) sum += __shfl(o[j], lane + d * (KP / 4));
+            o[j] = sum;                                          // (of the first KP / 4 lanes)
+        }
+    }
+    if constexpr (W > 1) {
+        float *own = sums + share * (KP + 1);
+        if (grad && mine == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) own[k4 + j] = o[j];
+        }
+        if (lane == 0) own[KP] = total;
+        __syncthreads();                                         // (all W are here: a row is theirs alone)
+        if (share > 0) return;
+        for (int v = 1; v < W; ++v) {
+            const float *other = sums + v * (KP + 1);
+            total += other[KP];
+            if (grad && mine == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] += other[k4 + j];
+            }
+        }
+    }
     const float lse2 = top - kUnit + log2f(total);
     if (lane == 0) f.a.loss[r] = f.a.temperature * f.a.temperature * (part[r] + lse2 * 0.693147180559945309f);
     if (!grad) return;
@@ -508,10 +731,8 @@ __device__ void join_row(const FusedArgs &f, long long r, const float *__restric
     if (lane == 0) { f.user_data[at] = lse2; f.user_data_t[at] = coef; }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        float sum = o[j];
-        for (int d = 1; d < at_once; ++d) sum += __shfl(o[j], lane + d * (KP / 4));
         const int k = k4 + j;
-        if (mine == 0 && k < f.a.n_factors) f.a.d_users[(size_t)r * f.a.n_factors + k] = coef * (sum / total - acc[(size_t)r * KP + k]);
+        if (mine == 0 && k < f.a.n_factors) f.a.d_users[(size_t)r * f.a.n_factors + k] = coef * (o[j] / total - acc[(size_t)r * KP + k]);
     }
 }
 
@@ -557,9 +778,9 @@ __device__ void bucket_entries(const FusedArgs &f, int tile, int block_items, co
     }
 }
 
-// Two things that wait for different kernels and for nothing of each other, in one launch: the rows joined (8 per workgroup), and the tiles' entries
+// Two things that wait for different kernels and for nothing of each other, in one launch: the rows joined (8 / W per workgroup), and the tiles' entries
 // (workgroups behind the rows').
-template <int KP>
+template <int KP, int W>
 __global__ void __launch_bounds__(512) join_rows_kernel(const FusedArgs f, int row_blocks, int block_items, const float *__restrict__ part, const float *__restrict__ mass,
                                                         const float *__restrict__ acc, const int32_t *__restrict__ item, const float *__restrict__ p) {
     __shared__ int lds[kBuckets + 8];
@@ -567,8 +788,10 @@ __global__ void __launch_bounds__(512) join_rows_kernel(const FusedArgs f, int r
         bucket_entries(f, (int)blockIdx.x - row_blocks, block_items, item, p, lds);
         return;
     }
+    __shared__ float sums[W > 1 ? W * (KP + 1) : 1];
     const int wave = threadIdx.x >> 6;
-    join_row<KP>(f, (long long)blockIdx.x * 8 + wave, part, mass, acc, reinterpret_cast<float *>(lds) + wave * 64);
+    static_assert(W == 1 || W == 8, "a barrier for the W wavefronts of a row is one for the workgroup");
+    join_row<KP, W>(f, (long long)blockIdx.x * (8 / W) + wave / W, wave % W, part, mass, acc, reinterpret_cast<float *>(lds) + wave * 64, sums);
 }
 
 // The items' gradient.  p of the teacher enters through a 32 x 32 patch of LDS per wavefront: the few entries that fall into the tile are written
@@ -577,7 +800,8 @@ constexpr int kPatch = 36;                       // floats per item of the patch
 // The work is cut into equal ranges of (block of items, user tile) pairs, one per workgroup that fits on the chip: no workgroup waits for a last
 // round.  A block that lies inside one range is written out as it is; the others' parts go to slot workgroup + block -- workgroups and blocks
 // both ascend along the ranges, so no two parts share one -- and are joined in that order.
-template <int KP, int NC, bool MASK>
+// RAW: the items' own operands are made from the table (few users: no copies)
+template <int KP, int NC, bool MASK, bool RAW = false>
 __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) items_kernel(const FusedArgs f) {
     constexpr int WAVES = Frag<KP>::waves;
     constexpr int kBytes = Frag<KP>::bytes, kBuf = 2 * kBytes + 2 * kUserData * 4;
@@ -607,9 +831,20 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const int mine = min(tile + n, f.item_tiles - 1);
-            load_columns<KP>(f.item_frag, mine, lane, x[n]);
-            bias[n] = f.item_data[(size_t)mine * kItemData + col];
-            unscale[n] = f.item_data[(size_t)mine * kItemData + 32];
+            if constexpr (RAW) {
+                bool odd;
+                const int item = mine * 32 + col;
+                Four raw[Frag<KP>::steps][2];
+                const int e_raw = raw_tile<KP>(f.a.items, f.a.item_stride, mine, f.a.n_items, f.a.n_factors, lane, raw, odd);
+                unscale[n] = ldexpf(1.0f, -e_raw);
+#pragma unroll
+                for (int k = 0; k < Frag<KP>::steps; ++k) raw_step(raw[k], ldexpf(1.0f, e_raw), x[n][k]);
+                bias[n] = item < f.a.n_items ? (f.a.bias ? f.a.bias[item] * f.c : 0.0f) : -INFINITY;
+            } else {
+                load_columns<KP>(f.item_frag, mine, lane, x[n]);
+                bias[n] = f.item_data[(size_t)mine * kItemData + col];
+                unscale[n] = f.item_data[(size_t)mine * kItemData + 32];
+            }
             top[n] = 0.0f;
             gate[n] = kLowest;
             d_bias[n] = 0.0f;

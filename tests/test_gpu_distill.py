@@ -404,3 +404,43 @@ def test_factors_of_nothing(factors, what):
     got = distill_gradients(*args, row_weight=torch.from_numpy(p.g).cuda(), **kw)
     for x, w, t in zip((*got, distill_loss(*args, **kw)), (*want, want[0]), (*tol, tol[0])):
         assert (np.abs(x.cpu().numpy() - w) <= t).all()
+
+
+@pytest.mark.parametrize("case", [dict(rows=r, items=i, factors=k, n=n, mask=m, tau=1.5) for r, i, k, n, m in (
+    (1, 1, 1, 1, None), (2, 31, 7, 3, "rows"), (31, 4097, 20, 9, "rows"), (32, 9001, 32, 5, None), (33, 5003, 33, 7, "few"), (64, 20_011, 64, 40, "one"), (63, 8192, 79, 12, "rows"),
+    (65, 7777, 96, 6, None), (96, 12_345, 101, 33, "few"), (97, 3001, 128, 10, "rows"), (128, 30_007, 50, 20, None), (128, 6007, 127, 20, "rows"), (129, 6007, 127, 20, "rows"),
+    (20, 70_001, 60, 200, "few"))], ids=ids)
+def test_few_rows(case):
+    """up to four tiles of rows, one more, and catalogues that reach every workgroup once, several times or not at all"""
+    p = Problem(seed=case["items"], **case)
+    want, tol = p.exact()
+    args, kw = p.given()
+    weight = torch.from_numpy(p.g).cuda()
+    got = distill_gradients(*args, row_weight=weight, **kw)
+    for x, w, t in zip((*got, distill_loss(*args, **kw)), (*want, want[0]), (*tol, tol[0])):
+        assert (np.abs(x.cpu().numpy() - w) <= t).all()
+    again = distill_gradients(*args, row_weight=weight, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    wide_u, wide_v = torch.full((case["rows"], 131), NAN).cuda(), torch.full((case["items"], 133), NAN).cuda()
+    k = case["factors"]
+    wide_u[:, 1:k + 1], wide_v[:, 3:k + 3] = args[0], args[1]
+    strided = distill_gradients(wide_u[:, 1:k + 1], wide_v[:, 3:k + 3], *args[2:], row_weight=weight, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, strided))
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128])
+def test_few_rows_and_masked_items_that_hold_anything(factors):
+    p = Problem(rows=40, items=3000, factors=factors, n=6, mask="one", seed=23)
+    p.ti = np.abs(p.ti) % 3000
+    p.mask[0, [0, 17, 64, 2999]] = False
+    args, kw = p.given()
+    want, tol = p.exact()
+    v = args[1].clone()
+    v[0], v[17], v[64, 3], v[2999] = NAN, INF, -INF, NAN
+    got = distill_gradients(args[0], v, *args[2:], row_weight=torch.from_numpy(p.g).cuda(), **kw)
+    for x, w, t in zip((*got, distill_loss(args[0], v, *args[2:], **kw)), (*want, want[0]), (*tol, tol[0])):
+        assert (np.abs(x.cpu().numpy() - w) <= t).all()
+    v[5, 2] = NAN                                                                 # and an item that may be had
+    if p.mask[0, 5]:
+        got = distill_gradients(args[0], v, *args[2:], **kw)
+        assert torch.isnan(got.loss[2:]).all() and torch.isnan(got.users[2:]).all()
