@@ -405,7 +405,6 @@ static int run_matrix(const rfm_distill_args *a, char *base, hipStream_t stream)
 // How often the streamed tiles are split: workgroups run `slots` at a time, a workgroup costs its tiles and about four more to start and end,
 // a split costs its partial sums.  The cheapest count wins; the sums of a count are always joined in the same order.
 constexpr int kCus = 256;
-constexpr int kThinItems = 256;                  // tiles of items from which few users are taken without copies
 static int pick_splits(int blocks, int tiles, int slots) {
     int best = 1;
     double least = 1e30;
@@ -430,8 +429,10 @@ static FusedLayout fused_layout(const rfm_distill_args *a) {
     const size_t R = (size_t)a->n_rows, n = (size_t)a->n_teacher, kp = (size_t)w.kp;
     w.user_tiles = (int)((a->n_rows + 31) / 32);
     w.item_tiles = (a->n_items + 31) / 32;
-    // Few users: no copies of the items' table are made (thin_forward_kernel).
-    const bool thin = w.user_tiles <= 2 && w.item_tiles >= kThinItems;
+    // Few users: no copies of the items' table are made (thin_forward_kernel).  Measured with copies / without, us, gradients of 29 rows: k = 20, 6 k items
+    // 25.7 / 26.4, 190 k 73 / 43; k = 64, 6 k 28.8 / 31.6, 10 k 35.7 / 33.6, 150 k 88 / 60; k = 128, 6 k 42.0 / 50.4, 20 k 59.5 / 57.7, 150 k 151 / 109; the loss
+    // alone, k = 64: 2 k 14.3 / 14.7, 3.7 k 14.8 / 14.8, 150 k 46 / 25.  With three or four tiles of users they come out even, at any size.
+    const bool thin = w.user_tiles <= 2 && w.item_tiles >= (grad ? 5 * w.kp : w.kp + 64);
     w.few = thin ? w.user_tiles : 0;
     // Column tiles per wavefront: two read LDS half as often, one leaves more workgroups to spread.  Measured with two against one, k = 64, gradients / loss
     // alone: 512 rows x 50 k items 1.10 / 1.13, 2048 x 50 k 1.01 / 0.96, 4096 x 20 k 1.00 / 0.95, 4096 x 50 k 0.95 / 0.93, 2048 x 200 k 0.96 / 0.93; k = 20

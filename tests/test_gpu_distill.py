@@ -409,9 +409,10 @@ def test_factors_of_nothing(factors, what):
 @pytest.mark.parametrize("case", [dict(rows=r, items=i, factors=k, n=n, mask=m, tau=1.5) for r, i, k, n, m in (
     (1, 1, 1, 1, None), (2, 31, 7, 3, "rows"), (31, 4097, 20, 9, "rows"), (32, 9001, 32, 5, None), (33, 5003, 33, 7, "few"), (64, 20_011, 64, 40, "one"), (63, 8192, 79, 12, "rows"),
     (65, 7777, 96, 6, None), (96, 12_345, 101, 33, "few"), (97, 3001, 128, 10, "rows"), (128, 30_007, 50, 20, None), (128, 6007, 127, 20, "rows"), (129, 6007, 127, 20, "rows"),
-    (20, 70_001, 60, 200, "few"))], ids=ids)
+    (20, 70_001, 60, 200, "few"), (29, 20_500, 128, 9, "rows"), (64, 20_511, 97, 9, None), (33, 5122, 32, 9, "rows"), (64, 10_250, 64, 9, "one"))], ids=ids)
 def test_few_rows(case):
-    """up to four tiles of rows, one more, and catalogues that reach every workgroup once, several times or not at all"""
+    """one or two tiles of rows, and more; catalogues on both sides of the sizes from which their tables are taken as they are, reaching every workgroup once,
+    several times or not at all"""
     p = Problem(seed=case["items"], **case)
     want, tol = p.exact()
     args, kw = p.given()
