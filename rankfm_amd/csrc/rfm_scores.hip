@@ -455,7 +455,9 @@ __device__ __forceinline__ bool hash_lists(const RowRules &w, int begin, int end
         }
     }
     __syncthreads();
-    return m.used <= kFull;
+    const bool fits = m.used <= kFull;
+    __syncthreads();                                             // (where it does not, counts of tiles take the table's place at once)
+    return fits;
 }
 __device__ __forceinline__ void window_bits(Listed &m, int first) {
     __syncthreads();                                             // (nobody reads the last window's any more)
