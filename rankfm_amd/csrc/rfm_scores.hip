@@ -328,7 +328,7 @@ constexpr int kPer = 8, kTile = kPer * kThreads; // scores per thread of a tile
 template <bool RULED> struct Top {
     static constexpr int super = RULED ? 2 : 4;  // tiles whose scores are in registers at once
     static constexpr int buf = RULED ? 512 : 1024;               // candidates a wavefront holds
-    static constexpr int round = buf / 2;        // most entries kept at a time; a longer list is taken in rounds of this many
+    static constexpr int round = buf / 4 * 3;    // most entries kept at a time; a longer list is taken in rounds of this many
 };
 constexpr int kSlots = 1024;                     // hash slots for the items that a row's lists name
 constexpr int kFull = kSlots - kThreads;         // lists that name more are scanned once per tile instead
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
                 sort_in_place(mine, m, lane);
-                m = want;                                        // (less than half of the buffer)
+                m = want;                                        // (three quarters of the buffer at most)
                 thr = max(thr, mine[want - 1]);
             }
             reach = key_score(thr);

@@ -344,7 +344,7 @@ def test_top_scores_under_long_lists(rows, items, listed, kinds):
     p.hist_rows = np.arange(rows, dtype=np.int32)[::-1].copy()
     p.mask[0] = True
     adjusted = p.plain(np.float32)[0]
-    for n in (5, 300):
+    for n in (5, 300, 384, 385, 800):
         got = top_scores(p.s.cuda(), n, p.rules())
         want_items, want_values = plain_top(adjusted, n)
         assert np.array_equal(got.items.cpu().numpy(), want_items) and np.array_equal(got.scores.cpu().numpy(), want_values)
@@ -366,7 +366,7 @@ def test_long_lists_of_long_rows(dtype, kind):
         s = rng.standard_normal((600, 40_003)) * 0.01
         s[:, 20_000:20_256] += 3.0
     s = torch.from_numpy(s.astype(np.float32)).to(dtype)
-    for n in (200, 500, 513):
+    for n in (200, 500, 768, 769, 1540):
         got = top_scores(s.cuda(), n)
         want_items, want_values = plain_top(s[:5].float().numpy(), n)
         assert np.array_equal(got.items[:5].cpu().numpy(), want_items) and np.array_equal(got.scores[:5].cpu().numpy(), want_values)
