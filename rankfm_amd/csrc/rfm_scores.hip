@@ -807,12 +807,14 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
     }
 }
 
-// how many segments a row is cut into: with few rows, enough to give every CU work, of at least one block of 8192 scores each.  Lists of more than 1024
-// are not cut: every segment would hand that many on.
+// How many segments a row is cut into: with few rows, enough to give every CU work, of at least one block of 8192 scores each.  Lists of more than 1024
+// are not cut: every segment would hand that many on.  From 256 rows on joining costs more than the second workgroup per CU gives (400 rows of 17 k, n = 10 / 100 /
+// 450, cut in two: 20.4 / 35.6 / 79.0 us, whole: 12.5 / 19.0 / 44.4; of 190 k: 71 / 129 / 191 and 61 / 129 / 157), but for long rows under rules
+// (500 of 190 k, n = 10: 91 and 118).
 constexpr int kBlock = 8192;
-static int top_segments(long long n_rows, int n_items, int n) {
-    if (n > 1024 || n_rows >= 512) return 1;
+static int top_segments(long long n_rows, int n_items, int n, bool ruled) {
     const long long blocks = ((long long)n_items + kBlock - 1) / kBlock;
+    if (n > 1024 || n_rows >= 512 || (n_rows >= 256 && !(ruled && blocks > 12))) return 1;
     return (int)std::max<long long>(1, std::min<long long>(blocks, (512 + n_rows - 1) / n_rows));
 }
 static int top_segment(int n_items, int segments) {
@@ -850,7 +852,7 @@ static void launch_adjust(const rfm_score_rules &u, long long n_rows, int n_item
 template <typename T, bool RULED>
 static void launch_top(const rfm_score_rules &u, long long n_rows, int n_items, const void *in, long long stride, int n, int32_t *items, float *values, u64 *keys,
                        hipStream_t stream) {
-    int segments = top_segments(n_rows, n_items, n);
+    int segments = top_segments(n_rows, n_items, n, RULED);
     const int segment = top_segment(n_items, segments);
     segments = (n_items + segment - 1) / segment;
     const long long step = std::max<long long>(1, kMaxBlocks / segments);
@@ -886,7 +888,7 @@ int rfm_adjust_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_
 
 size_t rfm_top_scores_workspace_bytes(int64_t n_rows, int32_t n_items, int32_t n) {
     if (n_rows < 0 || n_items < 1 || n < 1 || n > n_items) return 0;
-    const int segments = top_segments(n_rows, n_items, n);
+    const int segments = top_segments(n_rows, n_items, n, true);            // (with rules there are as many or more)
     return segments > 1 ? sizeof(u64) * (size_t)n_rows * (size_t)segments * (size_t)n : 8;
 }
 

@@ -372,3 +372,14 @@ def test_long_lists_of_long_rows(dtype, kind):
         assert np.array_equal(got.items[:5].cpu().numpy(), want_items) and np.array_equal(got.scores[:5].cpu().numpy(), want_values)
         value, _ = torch.sort(s.cuda().float(), dim=1, descending=True)
         assert torch.equal(got.scores, value[:, :n])
+
+
+@pytest.mark.parametrize("rows", [255, 256, 511, 512])
+@pytest.mark.parametrize("ruled", [False, True], ids=["plain", "ruled"])
+def test_rows_around_the_counts_that_are_cut(rows, ruled):
+    s = torch.from_numpy(np.random.default_rng(rows).standard_normal((rows, 110_003)).astype(np.float32)).to(F16).cuda()
+    bias = torch.linspace(-0.1, 0.1, 110_003).cuda()
+    got = top_scores(s, 70, ScoreRules(item_bias=bias) if ruled else None)
+    full = s.float() + bias if ruled else s.float()
+    value, _ = torch.sort(full, dim=1, descending=True)
+    assert torch.equal(got.scores, value[:, :70]) and torch.equal(full.gather(1, got.items.long()), got.scores)
