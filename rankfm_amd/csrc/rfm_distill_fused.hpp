@@ -41,8 +41,8 @@ constexpr int kItemData = 64;                    // floats that travel with an i
 constexpr int kUserData = 64;                    // ... with a user tile: 32 lse (log2 units), 2^-e of one copy, e and 2^e of the other; and 32 coefficients
 constexpr int kBuckets = 1024;                   // of a tile's teacher entries, by block of items
 constexpr float kLowest = -3.402823466e38f;
-constexpr float kUnit = 7.0f;                    // a column's largest weight is 2^7 when its maximum is set, and at most 2^15 (fp16 ends at 2^16)
-constexpr float kLimit = 15.0f;
+constexpr float kUnit = 15.0f;                   // a column's largest weight in a tile is 2^14 .. 2^15 (fp16 ends at 2^16)
+constexpr float kSlack = 8.0f;                   // how far a tile may be above a column's running unit before that is moved
 
 template <int KP> struct Frag {
     static constexpr int steps = KP / 16, cols = KP / 32;
@@ -264,10 +264,10 @@ __device__ __forceinline__ void split_weights(const f32x16 &w, f16x8 (*p)[2]) {
         p[t][1] = __builtin_bit_cast(f16x8, m);
     }
 }
-// o[n][c] = o[n][c] * by[n] + rows of the transposed tile . weights of column tile n.  A tile's 32 terms are summed by themselves first: the running sum
+// o[n][c] += unit[n] * rows of the transposed tile . weights of column tile n.  A tile's 32 terms are summed by themselves first: the running sum
 // sees one operation per tile
 template <int KP, int NC>
-__device__ __forceinline__ void weighted_sum(const char *tile_t, int lane, const f16x8 (*p)[2][2], const float *by, f32x16 (*o)[Frag<KP>::cols]) {
+__device__ __forceinline__ void weighted_sum(const char *tile_t, int lane, const f16x8 (*p)[2][2], const float *unit, f32x16 (*o)[Frag<KP>::cols]) {
 #pragma unroll
     for (int c = 0; c < Frag<KP>::cols; ++c) {
         f32x16 sum[NC];
@@ -283,7 +283,7 @@ __device__ __forceinline__ void weighted_sum(const char *tile_t, int lane, const
 #pragma unroll
         for (int n = 0; n < NC; ++n)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[n][c][r] = fmaf(o[n][c][r], by[n], sum[n][r]);
+            for (int r = 0; r < 16; ++r) o[n][c][r] = fmaf(sum[n][r], unit[n], o[n][c][r]);
     }
 }
 template <int KP, int NC>
@@ -330,6 +330,11 @@ __device__ __forceinline__ float largest16(const f32x16 &s) {
     for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
     return high;
 }
+// the larger of a column's two halves, for both (v_permlane32_swap_b32 exchanges one's upper with the other's lower lanes)
+__device__ __forceinline__ float both_halves(float x) {
+    const auto pair = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(pair[0]), __uint_as_float(pair[1]));
+}
 __device__ __forceinline__ float sum16(const f32x16 &s) {
     float sum[4];
 #pragma unroll
@@ -337,10 +342,45 @@ __device__ __forceinline__ float sum16(const f32x16 &s) {
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// Both kernels keep a column's sums in units of 2^(top - 7): a weight 2^x of a tile of scale 2^e enters as 2^(x - e - top + 7), against the tile's
-// values times 2^e.  `top` is moved only when that passes 2^15; it is the same in both halves of the wavefront, and a whole number, so that every scale
-// is an exact power of two (a fractional one rounds differently where it is put in and where it is taken out: up to 7e-7 of a column).
-//
+// A weight 2^x is cut into its two parts as 2^(x - high + 15), `high` being the least whole number that none of its column's in the tile is above: the parts
+// end at 2^-25, 2^-40 of the column's largest weight in the TILE.  (With one unit for all tiles, the column's largest so far, they ended at 2^-32 of that:
+// of 200 k items 16 nats below the first the users' gradient lost 1.4e-3, at 20 nats a tenth, and an item on a teacher's list the shares of all other users
+// below 2^-9 of its own.)  The running sums are in units of 2^(top - 15), top >= high - e - 8 for a tile whose values are scaled by 2^e: what a tile
+// gives is multiplied by 2^(high - e - top) where it is added, and `top` moved only when that would pass 2^8.  All of these are the same in both halves
+// of the wavefront, and whole numbers, so that every scale is an exact power of two (a fractional one rounds differently where it is put in and where it
+// is taken out: up to 7e-7 of a column).
+template <int COLS>
+__device__ __forceinline__ float tile_unit(float level, float &top, float &total, f32x16 (&o)[COLS]) {
+    if (__any(level > top + kSlack)) {                           // (kLowest + 8 is kLowest: a column's first weight moves it)
+        const float to = level > top + kSlack ? level : top, by = __builtin_amdgcn_exp2f(top - to);
+        top = to;
+        total *= by;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][r] *= by;
+    }
+    return __builtin_amdgcn_exp2f(level - top);
+}
+// the weights of exponents s, and their sum
+__device__ __forceinline__ float weigh(f32x16 &s, float high) {
+    const float off = high - kUnit;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - off);
+    return sum16(s);
+}
+// Where nothing but their sum is wanted they are not cut, and the unit is the column's largest so far (50 k items, k = 64, 8192 rows: 179 us; 185 with a unit
+// per tile)
+__device__ __forceinline__ void add_weights(f32x16 &s, float &top, float &total) {
+    const float high = largest16(s);
+    if (__any(high > top + kSlack)) {
+        const float to = fmaxf(top, ceilf(both_halves(high)));
+        total *= __builtin_amdgcn_exp2f(top - to);
+        top = to;
+    }
+    total += weigh(s, top);
+}
+
 // Workgroup b: split b % lanes of the items, columns block b / lanes.  Workgroups go round the XCDs: where `lanes` is a multiple of 8, those of one XCD stream
 // the same items, out of its L2 (512 rows x 50 k items, k = 20, gradients: 75.1 us without, 72.8 with; 1503 x 35 k, 61 splits: 141.3 with 61 lanes, 139.3 with 64).
 template <int KP, int NC, bool GRAD, bool MASK>
@@ -401,7 +441,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (GRAD ? kPerSimd<KP, NC>
         const f32x4 *data = reinterpret_cast<const f32x4 *>(buf[i] + kBuf - kItemData * 4);
         const f32x4 last = data[8];
         const float e = last[1], scale = last[2];
-        float by[NC];
+        float by[NC];                                            // (the gradients' alone, as the two above)
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const float unit = last[0] * unscale[n];
@@ -412,17 +452,11 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (GRAD ? kPerSimd<KP, NC>
                 for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unit, b[k]);
             }
             if constexpr (MASK) mask16(s[n], word[n] >> (4 * half));
-            const float high = largest16(s[n]) - e;
-            by[n] = 1.0f;
-            if (__any(high > top[n] + (kLimit - kUnit))) {
-                const float to = fmaxf(top[n], ceilf(fmaxf(high, __shfl_xor(high, 32))));
-                by[n] = __builtin_amdgcn_exp2f(top[n] - to);
-                top[n] = to;
-            }
-            const float off = top[n] + (e - kUnit);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - off);
-            total[n] = fmaf(sum16(s[n]), scale, total[n] * by[n]);
+            if constexpr (GRAD) {
+                const float high = fmaxf(ceilf(both_halves(largest16(s[n]))), kLowest);      // (kLowest: nothing is allowed, all weights are 0)
+                by[n] = tile_unit(high - e, top[n], total[n], o[n]);
+                total[n] = fmaf(weigh(s[n], high), by[n] * scale, total[n]);
+            } else add_weights(s[n], top[n], total[n]);
         }
         if constexpr (GRAD) {
             f16x8 p[NC][2][2];
@@ -571,17 +605,12 @@ __global__ void __launch_bounds__(kThinWaves * 64, (kThinPerSimd<KP, GRAD>)) thi
             for (int k = 0; k < 4; ++k) s[4 * q + k] = fmaf(s[4 * q + k], unit, b[k]);
         }
         if constexpr (MASK) mask16(s, word >> (4 * half));
-        const float high = largest16(s) - e;
         float by = 1.0f;
-        if (__any(high > top + (kLimit - kUnit))) {
-            const float to = fmaxf(top, ceilf(fmaxf(high, __shfl_xor(high, 32))));
-            by = __builtin_amdgcn_exp2f(top - to);
-            top = to;
-        }
-        const float off = top + (e - kUnit);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - off);
-        total = fmaf(sum16(s), scale, total * by);
+        if constexpr (GRAD) {
+            const float high = fmaxf(ceilf(both_halves(largest16(s))), kLowest);
+            by = tile_unit(high - e, top, total, o);
+            total = fmaf(weigh(s, high), by * scale, total);
+        } else add_weights(s, top, total);
         if constexpr (GRAD) {
             f16x8 p[2][2];
             split_weights(s, p);
@@ -602,7 +631,7 @@ __global__ void __launch_bounds__(kThinWaves * 64, (kThinPerSimd<KP, GRAD>)) thi
                     sum = mfma3(parts, p[t], sum);
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[c][r] = fmaf(o[c][r], by, sum[r]);
+                for (int r = 0; r < 16; ++r) o[c][r] = fmaf(sum[r], by, o[c][r]);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -820,8 +849,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
         const int tile = (block * WAVES + wave) * NC;
         const unsigned base = (unsigned)tile * 32u;
         f16x8 x[NC][Frag<KP>::steps][2];
-        // `gate`: what an exponent may reach before `top` is moved -- anything at first, so that the first weight of a column sets it
-        float bias[NC], unscale[NC], top[NC], gate[NC], d_bias[NC];
+        float bias[NC], unscale[NC], top[NC], d_bias[NC];
         unsigned next_word[NC];
         f32x16 o[NC][Frag<KP>::cols];
         auto mask_word = [&](int t, int n) {                     // of row `col` of the tile, the bits of this wavefront's items
@@ -846,8 +874,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
                 bias[n] = f.item_data[(size_t)mine * kItemData + col];
                 unscale[n] = f.item_data[(size_t)mine * kItemData + 32];
             }
-            top[n] = 0.0f;
-            gate[n] = kLowest;
+            top[n] = kLowest;
             d_bias[n] = 0.0f;
             next_word[n] = 0;
             if constexpr (MASK) next_word[n] = mask_word(t0, n);
@@ -899,30 +926,23 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
             const f32x4 *data = reinterpret_cast<const f32x4 *>(now + 2 * kBytes);
             const f32x4 last = data[8];
             const float e = last[1], scale = last[2];
-            float by[NC];
+            float high[NC];
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-                // the exponents of the weights, for `top` as it stands
-                const float unscaled = last[0] * unscale[n], shift = bias[n] - (top[n] + (e - kUnit));
+                // the exponents of the weights but for the column's bias
+                const float unscaled = last[0] * unscale[n];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const f32x4 lse = data[half + 2 * q];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unscaled, shift) - lse[k];
+                    for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unscaled, -lse[k]);
                 }
                 if constexpr (MASK) mask16_rows(s[n], word[n]);
-                const float high = largest16(s[n]);
-                by[n] = 1.0f;
-                if (__any(high > gate[n])) {
-                    const float h = fmaxf(high, __shfl_xor(high, 32)), more = h > gate[n] ? ceilf(h - kUnit) : 0.0f;
-                    by[n] = gate[n] == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);       // (1: there is nothing to scale yet)
-                    gate[n] = h > gate[n] ? kLimit : gate[n];
-                    top[n] += more;
+                const float most = both_halves(largest16(s[n])), b = most == -INFINITY ? 0.0f : bias[n];       // (no row has it: its bias may be anything)
+                high[n] = fmaxf(ceilf(most + b), kLowest);
+                const float off = b - (high[n] - kUnit);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[n][r] -= more;
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r]);
+                for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r] + off);
             }
             // the teacher's share
             unsigned any = 0;                                    // a bit per column tile that is hit
@@ -950,17 +970,14 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
 #pragma unroll
                         for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(p[q][k]));
                     }
-                    const float log_p = __builtin_amdgcn_logf(__uint_as_float(most)) - (top[n] + (e - kUnit));       // (-inf where there is none)
-                    if (__any(log_p > gate[n])) {
-                        const float h = fmaxf(log_p, __shfl_xor(log_p, 32)), more = h > gate[n] ? ceilf(h - kUnit) : 0.0f;
-                        const float by_p = gate[n] == kLowest ? 1.0f : __builtin_amdgcn_exp2f(-more);
+                    const float log_p = both_halves(__builtin_amdgcn_logf(__uint_as_float(most)));       // (-inf where there is none)
+                    if (__any(log_p > high[n])) {
+                        const float to = fmaxf(high[n], ceilf(log_p)), by_p = __builtin_amdgcn_exp2f(high[n] - to);
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[n][r] *= by_p;
-                        by[n] *= by_p;
-                        gate[n] = h > gate[n] ? kLimit : gate[n];
-                        top[n] += more;
+                        high[n] = to;
                     }
-                    const float unit = fminf(__builtin_amdgcn_exp2f(kUnit - e - top[n]), -kLowest);      // (finite where a column has no weight yet: 0 stays 0)
+                    const float unit = fminf(__builtin_amdgcn_exp2f(kUnit - high[n]), -kLowest);      // (finite where a column has no weight: 0 stays 0)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -970,8 +987,10 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
                 __builtin_amdgcn_wave_barrier();
             }
             f16x8 p[NC][2][2];
+            float by[NC];
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
+                by[n] = tile_unit(high[n] - e, top[n], d_bias[n], o[n]);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -979,7 +998,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
 #pragma unroll
                     for (int k = 0; k < 4; ++k) sum[k] = fmaf(s[n][4 * q + k], coef[k], sum[k]);
                 }
-                d_bias[n] = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), scale, d_bias[n] * by[n]);
+                d_bias[n] = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), by[n] * scale, d_bias[n]);
                 split_weights(s[n], p[n]);
             }
             weighted_sum<KP, NC>(now + kBytes, lane, p, by, o);
@@ -989,27 +1008,32 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
         const int K = f.a.n_factors;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const float sum = d_bias[n] + __shfl_xor(d_bias[n], 32), unit_of = __builtin_amdgcn_exp2f(top[n] - kUnit);
+            const float sum = d_bias[n] + __shfl_xor(d_bias[n], 32);
+            // out of their unit 2^(top - 15), which may be below float32's smallest where its sums are not: by the exponent, not by a factor
+            const int unit = (int)fminf(fmaxf(top[n] - kUnit, -1000.0f), 1000.0f);
+            auto out_of_unit = [&](int c, int q) {
+                return f32x4{ldexpf(o[n][c][4 * q], unit), ldexpf(o[n][c][4 * q + 1], unit), ldexpf(o[n][c][4 * q + 2], unit), ldexpf(o[n][c][4 * q + 3], unit)};
+            };
             const int item = (tile + n) * 32 + col;
             if (whole && item < f.a.n_items) {
                 float *out = f.a.d_items + (size_t)item * K;
-                if (half == 0 && f.a.d_bias) f.a.d_bias[item] = sum * unit_of;
+                if (half == 0 && f.a.d_bias) f.a.d_bias[item] = ldexpf(sum, unit);
 #pragma unroll
                 for (int c = 0; c < Frag<KP>::cols; ++c)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int k = 32 * c + 8 * q + 4 * half;
-                        const f32x4 v = f32x4{o[n][c][4 * q], o[n][c][4 * q + 1], o[n][c][4 * q + 2], o[n][c][4 * q + 3]} * unit_of;
+                        const f32x4 v = out_of_unit(c, q);
                         store_four(out, k, K, v[0], v[1], v[2], v[3]);
                     }
             } else if (!whole) {
                 const size_t at = ((size_t)(blockIdx.x + block) * WAVES * NC + wave * NC + n) * 32 + col;
-                if (half == 0) f.part_bias[at] = sum * unit_of;
+                if (half == 0) f.part_bias[at] = ldexpf(sum, unit);
 #pragma unroll
                 for (int c = 0; c < Frag<KP>::cols; ++c)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<f32x4 *>(f.part_items + at * KP + 32 * c + 8 * q + 4 * half) = f32x4{o[n][c][4 * q], o[n][c][4 * q + 1], o[n][c][4 * q + 2], o[n][c][4 * q + 3]} * unit_of;
+                        *reinterpret_cast<f32x4 *>(f.part_items + at * KP + 32 * c + 8 * q + 4 * half) = out_of_unit(c, q);
             }
         }
     }

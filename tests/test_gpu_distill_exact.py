@@ -1,0 +1,151 @@
+"""distill_loss / distill_gradients where the scores themselves carry no rounding: factors of 0 and +-1, whole biases, a temperature of log2(e), so that
+softmax weights are powers of two and their sums exact.  What is left are a handful of roundings, whatever the catalogue's length, and every tile of 32 rows
+or items has a factor of its own class: a tile left out or taken twice is off by percents of a gradient, against tolerances of 1e-5.
+
+Tolerances, with E = 2^-24 and D the largest |log2 q| + |lse| + |z| (log2 units; ln 2 < 0.7 turns them into relative ones):
+  eq   a weight q: the temperature's own rounding, the lse's, the exponent's and its parts', each at most E of D, one step of the logarithm and two
+       of exp2, 2^-23 for a weight's two half-precision parts:  E (0.7 * 5 D + 12).  Beyond 128 factors expf of natural units: the same count
+  ep   a teacher's p (equal scores):  E (n + 8)
+  a gradient is a sum of terms |dz| |factor| (exact factors): eq + ep of each, and the additions -- 100 in a tile of 32 rows, one per tile and split
+  a weight's parts are cut at 2^-40 of the largest weight that its column has in the tile:  2^-40 of that for each of the 32 terms
+  loss: tau^2 (p's part: (n + 8) E of its size; lse and z: 4 E D)"""
+import numpy as np
+import pytest
+import torch
+
+from rankfm_amd import distill_gradients, distill_loss, pack_allowed
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+TAU = float(np.float32(1.4426950408889634))
+NAN, INF = float("nan"), float("inf")
+
+
+def check(users, items, bias, ti, weight=None, mask=None, which=None, additions=None):
+    """both calls against float64; teacher scores are all equal.  mask: bool [masks, items] on the device"""
+    rows, catalogue, n = users.shape[0], items.shape[0], ti.shape[1]
+    t = torch.zeros(ti.shape, device="cuda")
+    kw = dict(temperature=TAU, allowed=None if mask is None else pack_allowed(mask), allowed_rows=which)
+    got = distill_gradients(users, items, bias, ti, t, row_weight=weight, **kw)
+    alone = distill_loss(users, items, bias, ti, t, **kw)
+    u, v = users.double(), items.double()
+    z2 = u @ v.T + bias.double()                                                  # log2 units but for the temperature's rounding
+    z = z2 / TAU
+    usable = (ti >= 0) & (ti < catalogue)
+    at = ti.long().clamp(0, catalogue - 1)
+    if mask is not None:
+        ok = mask.expand(rows, -1) if which is None else torch.where(which[:, None] >= 0, mask[which.long().clamp(min=0)], True)
+        z = torch.where(ok, z, -INF)
+        usable = usable & ok.gather(1, at)
+    live = usable.any(1)
+    lse = torch.where(live, torch.logsumexp(z, 1), 0.0)
+    count = usable.sum(1, keepdim=True).clamp(min=1)
+    p = usable.double() / count
+    log_q = torch.where(usable, z.gather(1, at) - lse[:, None], 0.0)
+    loss = torch.where(live, TAU * TAU * (p * (-torch.log(count.double()) - log_q)).sum(1), 0.0)
+    q = torch.where(live[:, None], torch.exp(z - lse[:, None]), 0.0)
+    teacher = torch.zeros_like(q).scatter_add_(1, at, p)
+    coef = (TAU * live * (weight.double() if weight is not None else 1.0))[:, None]
+    coef = torch.where(live[:, None], coef, 0.0)                                  # (a dead row's weight may be anything)
+    dz, size = (q - teacher) * coef, (q + teacher) * coef.abs()
+    finite = torch.where(z > -INF, z, 0.0)
+    D = float((finite - lse[:, None]).abs().max() + lse.abs().max() + finite.abs().max()) * 1.4427
+    eq, ep = E * (0.7 * 5 * D + 12), E * (n + 8)
+    # 2^-40 of a tile's largest weight per row, for each of its items; and per item, for each of a tile's rows
+    pad = (-catalogue) % 32
+    by_tile = torch.nn.functional.pad(q, (0, pad)).view(rows, -1, 32).amax(2).sum(1) * 32 * 2.0 ** -40
+    cut_u = (coef.abs()[:, 0] * by_tile)[:, None] * v.abs().amax(0)
+    pad = (-rows) % 32
+    by_tile = torch.nn.functional.pad(size, (0, 0, 0, pad)).view(-1, 32, catalogue).amax(1).sum(0) * 32 * 2.0 ** -40
+    cut_i = by_tile[:, None] * u.abs().amax(0)
+    deep_i = E * (rows / 32 + 160)
+    if u.shape[1] > 128:                                                         # a slice of the items is one chain of additions there, then the slices
+        slices = max(1, min(16, catalogue // 2048))
+        additions = catalogue / slices + slices + 32
+    deep_u = E * (additions or 100)
+    tol = TAU * TAU * ((n + 8) * E * float(np.log(n) + 1) + 4 * E * D) * torch.ones_like(loss)
+    for name, x, want, bound in (("loss", alone, loss, tol), ("loss", got.loss, loss, tol), ("users", got.users, dz @ v, (eq + ep + deep_u) * (size @ v.abs()) + cut_u),
+                                 ("items", got.items, dz.T @ u, (eq + ep + deep_i) * (size.T @ u.abs()) + cut_i), ("bias", got.bias, dz.sum(0), (eq + ep + deep_i) * size.sum(0) + by_tile)):
+        off = (x.double() - want).abs() / (bound + 1e-38)
+        assert float(off.max()) <= 1, (name, float(off.max()), int(off.argmax()))
+    return got
+
+
+SIZES = [(4129, 32_801, 20), (1030, 129_037, 64), (1000, 20_011, 96), (300, 60_007, 128), (29, 150_001, 60), (64, 200_003, 33), (5, 21_001, 128), (33, 9001, 20), (130, 3001, 50),
+         (1, 5, 3), (257, 20_011, 130), (70, 5003, 300)]
+
+
+@pytest.mark.parametrize("rows,items,factors", SIZES, ids=lambda x: str(x))
+@pytest.mark.parametrize("masks", [None, "one", "rows"])
+def test_every_tile_counts_once(rows, items, factors, masks):
+    """one column tile per wavefront and two, few rows, long splits, the path without registers; with masks that leave whole tiles out"""
+    if masks == "rows" and rows * items > 60_000_000:
+        pytest.skip("masks of that size take too long to make")
+    gen = torch.Generator(device="cuda").manual_seed(items)
+    classes = factors - 1
+    sign = lambda n: torch.randint(0, 2, (n,), generator=gen, device="cuda").float() * 2 - 1      # noqa: E731
+    users, table = torch.zeros(rows, factors, device="cuda"), torch.zeros(items, factors, device="cuda")
+    for t in (users, table):
+        n = t.shape[0]
+        if classes:
+            t[torch.arange(n, device="cuda"), torch.arange(n, device="cuda") // 32 % classes] = 1.0
+        t[:, factors - 1] = sign(n)
+    bias = torch.randint(0, 2, (items,), generator=gen, device="cuda").float()
+    ti = torch.randint(-1, items + 1, (rows, 8), generator=gen, device="cuda", dtype=torch.int32)
+    if rows > 40:
+        ti[37] = -1
+    mask = which = None
+    if masks == "one":
+        mask = torch.rand(1, items, generator=gen, device="cuda") < 0.7
+        mask[:, items // 3:items // 3 + 200] = False
+    elif masks == "rows":
+        mask = torch.rand(rows, items, generator=gen, device="cuda") < 0.7
+        mask[rows // 2, items // 2:] = False
+    check(users, table, bias, ti, torch.rand(rows, generator=gen, device="cuda") + 0.5, mask, which)
+
+
+@pytest.mark.parametrize("factors,items", [(20, 6001), (64, 11_003), (128, 21_003), (200, 3001)])
+@pytest.mark.parametrize("rows", [40, 300])
+@pytest.mark.parametrize("nats", [12, 16, 20, 26])
+@pytest.mark.parametrize("masked", [False, True], ids=["", "masked"])
+def test_a_long_tail_behind_a_peak(factors, items, rows, nats, masked):
+    """one item holds nearly all of a row's mass, is what the teacher says, and has no factors: the users' gradient is the tail's, thousands of items that are
+    `nats` down each.  (A weight cut at 2^-32 of the peak's: 1.4e-3 at 16 nats, a tenth at 20)"""
+    torch.manual_seed(factors)
+    users, table = torch.zeros(rows, factors, device="cuda"), torch.zeros(items, factors, device="cuda")
+    table[:, 0] = 1.0
+    users[:, factors - 1] = 1.0
+    bias = torch.full((items,), 0.4541, device="cuda")
+    peak = 1234
+    table[peak], bias[peak] = 0.0, 0.4541 + nats * 1.4427
+    ti = torch.full((rows, 2), -1, dtype=torch.int32, device="cuda")
+    ti[:, 1] = peak
+    mask = torch.rand(1, items, device="cuda") < 0.8 if masked else None
+    if masked:
+        mask[0, peak] = True
+    got = check(users, table, bias, ti, None, mask, additions=items / 32 + 160)
+    # (the head's own share of that gradient is 0: nothing but the tail's is in it)
+    assert (got.users[:, 0] > 0).all()
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128, 200])
+@pytest.mark.parametrize("rows", [60, 1500])
+@pytest.mark.parametrize("down", [8.3, 16.3])
+@pytest.mark.parametrize("masked", [False, True], ids=["", "masked"])
+def test_an_item_that_one_user_holds(factors, rows, down, masked):
+    """an item's column: one user gives it all, the others 2^-19 and 2^-27 of that; in a factor that the one lacks the items' gradient is theirs"""
+    torch.manual_seed(factors)
+    items, special = 3001, 777
+    if rows == 60:
+        items = {20: 6001, 64: 11_003, 128: 21_003, 200: 3001}[factors]
+    users, table = torch.zeros(rows, factors, device="cuda"), torch.zeros(items, factors, device="cuda")
+    users[:, 0], users[:, 1] = -down, 1.0
+    users[5, 0], users[5, 1] = 30.0, 0.0
+    table[special, 0] = 1.0
+    ti = torch.full((rows, 2), 50, dtype=torch.int32, device="cuda")
+    ti[5] = special                                                              # (what the one user's teacher says: its dz is next to nothing)
+    mask = torch.rand(1, items, device="cuda") < 0.8 if masked else None
+    if masked:
+        mask[0, [special, 50]] = True
+    got = check(users, table, torch.zeros(items, device="cuda"), ti, None, mask, additions=items / 32 + 160)
+    assert got.items[special, 1] > 0
