@@ -889,21 +889,22 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
         // the tile's teacher entries: where they are is known two steps ahead (scalar loads), the first 64 are asked for one step ahead
         const int bucket = block % kBuckets;
         typedef const __attribute__((address_space(4))) int32_t *scalar_ptr;
-        auto bounds = [&](int t, int &begin, int &end) {
-            const scalar_ptr at = (scalar_ptr)(f.entry_at + (size_t)min(t, t1 - 1) * (kBuckets + 1) + bucket);
-            begin = at[0];
-            end = at[1];
+        auto bounds = [&](int t, int &begin, int &end, int &all) {
+            const scalar_ptr at = (scalar_ptr)(f.entry_at + (size_t)min(t, t1 - 1) * (kBuckets + 1));
+            begin = at[bucket];
+            end = at[bucket + 1];
+            all = at[kBuckets];                                  // of all buckets: 0 where the tile has no live row
         };
         auto entry_of = [&](int t, int begin) { return f.entry[(size_t)min(t, t1 - 1) * n32 + min(begin + lane, n32 - 1)]; };
-        int begin, end, begin1, end1;
-        bounds(t0, begin, end);
-        bounds(t0 + 1, begin1, end1);
+        int begin, end, all, begin1, end1, all1;
+        bounds(t0, begin, end, all);
+        bounds(t0 + 1, begin1, end1, all1);
         uint2 next_entry = entry_of(t0, begin);
         stage(t0);
         for (int t = t0; t < t1; ++t) {
             staged<0>();
             const char *now = buf[t & 1];
-            const int from = begin, to = end;
+            const int from = begin, to = end, entries = all;
             uint2 entry = next_entry;
             unsigned word[NC];
             // (no instructions: what was asked for a step ago is here, and is taken before anything else is asked for)
@@ -918,7 +919,8 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
             }
             begin = begin1;
             end = end1;
-            bounds(t + 2, begin1, end1);
+            all = all1;
+            bounds(t + 2, begin1, end1, all1);
             next_entry = entry_of(t + 1, begin);
             if (t + 1 < t1) stage(t + 1);
             f32x16 s[NC];
@@ -926,6 +928,9 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
             const f32x4 *data = reinterpret_cast<const f32x4 *>(now + 2 * kBytes);
             const f32x4 last = data[8];
             const float e = last[1], scale = last[2];
+            // a tile without a live row gives nothing, whatever the items hold.  (Beside a live one no row is without all items: where those are not finite
+            // the live row's own share is not, either)
+            if (!entries) continue;
             float high[NC];
 #pragma unroll
             for (int n = 0; n < NC; ++n) {

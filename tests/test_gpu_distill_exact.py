@@ -149,3 +149,24 @@ def test_an_item_that_one_user_holds(factors, rows, down, masked):
         mask[0, [special, 50]] = True
     got = check(users, table, torch.zeros(items, device="cuda"), ti, None, mask, additions=items / 32 + 160)
     assert got.items[special, 1] > 0
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128, 200])
+@pytest.mark.parametrize("rows,items", [(40, 21_003), (300, 901)])
+def test_rows_with_nothing_to_learn_reach_nothing(factors, rows, items):
+    """a batch of empty lists: all gradients are 0, whatever the table and the biases hold"""
+    torch.manual_seed(factors)
+    users, table, bias = torch.randn(rows, factors, device="cuda"), torch.randn(items, factors, device="cuda"), torch.randn(items, device="cuda")
+    table[3, 1], table[40], bias[7], bias[8], bias[9] = NAN, INF, INF, NAN, -INF
+    ti = torch.full((rows, 3), -1, dtype=torch.int32, device="cuda")
+    got = distill_gradients(users, table, bias, ti, torch.zeros(rows, 3, device="cuda"), temperature=2.0)
+    for x in got:
+        assert (x == 0).all()
+    # and one tile of such rows among others: theirs alone
+    ti[:32, 0] = 11
+    table[3, 1], table[40], bias[7], bias[8], bias[9] = 0.5, 0.25, 1.0, 2.0, 3.0
+    both = distill_gradients(users, table, bias, ti, torch.zeros(rows, 3, device="cuda"), temperature=2.0)
+    alone = distill_gradients(users[:32], table, bias, ti[:32].contiguous(), torch.zeros(32, 3, device="cuda"), temperature=2.0)
+    assert (both.loss[32:] == 0).all() and (both.users[32:] == 0).all()
+    for a, b in ((both.items, alone.items), (both.bias, alone.bias)):            # (32 terms of products within 1e-5: other splits, another order of sums)
+        assert torch.allclose(a, b, rtol=0, atol=1e-4)
