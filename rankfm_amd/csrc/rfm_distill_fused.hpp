@@ -75,11 +75,14 @@ __device__ __forceinline__ void split2(float x, _Float16 &h, _Float16 &m) {
     m = (_Float16)(x - (float)h);
 }
 
+// the scales of two tiles taken back.  Where their largest values multiply beyond float32's range a score of them does, too, and one of 0 stays 0
+__device__ __forceinline__ float unscaled(float a, float b) { return fminf(a * b, -kLowest); }
+
 // the exponent that brings a tile's largest value to 2^14 .. 2^15.  A tile of zeros or nearly so is scaled as if it held 2^-26: its weights then
 // stay out of the way of the others' (the running maximum below is that of weight / scale).
 __device__ __forceinline__ int tile_exponent(float largest) {
     const int e = 14 - (largest > 0.0f ? ilogbf(largest) : -1000);
-    return min(max(e, -100), 40);
+    return min(max(e, -113), 40);                                // (-113: float32 ends there)
 }
 // largest of a value per thread; every thread gets it
 __device__ __forceinline__ float block_max(float x, float *s_max) {
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (GRAD ? kPerSimd<KP, NC>
         float by[NC];                                            // (the gradients' alone, as the two above)
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const float unit = last[0] * unscale[n];
+            const float unit = unscaled(last[0], unscale[n]);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {                        // z in log2 units
                 const f32x4 b = data[half + 2 * q];
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(kThinWaves * 64, (kThinPerSimd<KP, GRAD>)) thi
         Four raw[Frag<KP>::steps][2];
         bool odd;
         const int e_tile = raw_tile<KP>(f.a.items, f.a.item_stride, tile, f.a.n_items, f.a.n_factors, lane, raw, odd);
-        const float e = (float)e_tile, unit = ldexpf(unscale, -e_tile), scale = ldexpf(1.0f, e_tile);
+        const float e = (float)e_tile, unit = unscaled(unscale, ldexpf(1.0f, -e_tile)), scale = ldexpf(1.0f, e_tile);
         if (half == 0) row_bias[wave][col] = b_of;
         f32x16 s = f32x16{0};
 #pragma unroll
@@ -935,12 +938,12 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 // the exponents of the weights but for the column's bias
-                const float unscaled = last[0] * unscale[n];
+                const float unit = unscaled(last[0], unscale[n]);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const f32x4 lse = data[half + 2 * q];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unscaled, -lse[k]);
+                    for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unit, -lse[k]);
                 }
                 if constexpr (MASK) mask16_rows(s[n], word[n]);
                 const float most = both_halves(largest16(s[n])), b = most == -INFINITY ? 0.0f : bias[n];       // (no row has it: its bias may be anything)

@@ -170,3 +170,24 @@ def test_rows_with_nothing_to_learn_reach_nothing(factors, rows, items):
     assert (both.loss[32:] == 0).all() and (both.users[32:] == 0).all()
     for a, b in ((both.items, alone.items), (both.bias, alone.bias)):            # (32 terms of products within 1e-5: other splits, another order of sums)
         assert torch.allclose(a, b, rtol=0, atol=1e-4)
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128, 200])
+@pytest.mark.parametrize("rows,items", [(40, 21_003), (300, 901)])
+def test_the_largest_factors(factors, rows, items):
+    """2^120 in a table whose scores are finite, and 2^80 in both where no score has them"""
+    users, table = torch.zeros(rows, factors, device="cuda"), torch.zeros(items, factors, device="cuda")
+    users[:, 0] = 2.0 ** 120
+    table[::2, 0] = 1.0
+    ti = torch.zeros(rows, 2, dtype=torch.int32, device="cuda")
+    ti[:, 1] = 1                                                                 # half the teacher's mass on items that are 2^120 down
+    t, bias = torch.zeros(rows, 2, device="cuda"), torch.zeros(items, device="cuda")
+    want = TAU * TAU * 0.5 * 2.0 ** 120 / TAU
+    for loss in (distill_loss(users, table, bias, ti, t, temperature=TAU), distill_gradients(users, table, bias, ti, t, temperature=TAU).loss):
+        assert ((loss.double() - want).abs() <= 16 * E * want).all()
+    users, table = torch.zeros_like(users), torch.zeros_like(table)
+    users[:, 0], table[:, 1] = 2.0 ** 80, 2.0 ** 80
+    got = distill_gradients(users, table, bias, ti, t, temperature=TAU)
+    want = TAU * TAU * (np.log(items) - np.log(2))
+    assert ((got.loss.double() - want).abs() <= 40 * E * (np.log(items) * TAU * TAU)).all()
+    assert torch.isfinite(got.users).all() and torch.isfinite(got.items).all()
