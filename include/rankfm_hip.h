@@ -348,6 +348,8 @@ int rfm_top_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_t n
  *   gradients of sum_r row_weight[r] * loss[r]:  with dz = temperature * row_weight * (q - p) (a row without a usable entry: 0)
  *   d_users = dz . items    d_items = dz^T . users    d_bias = column sums of dz
  * All of it float32 in and out; no array of the size n_rows x n_items of scores is kept (a block of rows is, above 128 factors).
+ * Up to 128 factors a product of two factors is off by up to 2^-21 of its size, 2^-24.2 in the mean (two half-precision parts per factor, scaled by a
+ * power of two per 32 rows of users or items: a factor below 2^-16 of the largest of its 32 rows is off by up to 2^-40 of that); sums are float32.
  * d_users = d_items = d_bias = NULL: the loss alone.  A row that names a mask behind the last one has loss NaN.
  * RFM_ERR_UNSUPPORTED: more than 2^24 rows, 2^25 items, 1024 factors or 1024 entries per list. ---- */
 typedef struct rfm_distill_args {

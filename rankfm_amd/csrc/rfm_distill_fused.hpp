@@ -1,9 +1,12 @@
 // rfm_distill_fused.hpp -- the distillation loss and its gradients without the score matrix (included by rfm_distill.hip).
 //
 // fp32 products on the fp16 matrix cores.  Every fp32 factor is the sum of two fp16 parts, x = h + m: 11 bits of the significand each, rounded to
-// nearest at each cut, so that 2^-24 of x is left over -- half a step of fp32.  Of the four products of two such sums m m' is left out, 2^-24 of
-// |x x'| at most and 2^-27 in the mean: an fp32 product rounds away as much.  Three v_mfma_f32_32x32x16_f16 take 3 / 16 of the time of the
-// fp32 matrix instructions (six with bf16 parts, which hold 8 bits: the step of 8192 rows x 50 k items at k = 64 took 1164 us with those, 794 with these).
+// nearest at each cut.  The last of fp32's 24 bits is lost where m is large and the bit is set: 2^-23 of x at most, in a quarter of all values.  Of the
+// four products of two such sums m m' is left out, 2^-22 of |x x'| at most and 2^-25 in the mean.  So a product is off by up to 2^-21 (2^-24.2 in the
+// mean), where an fp32 product rounds away 2^-24 (2^-25.5): 8 times as much at worst, 2.4 times in the mean, and in a score as much as the additions of 8 terms
+// may round away.  With the fourth product it would be 2^-22 still, and 2^-24.6 in the mean (loss of 8192 rows x 50 k items at k = 64: 179 -> 198 us, gradients
+// 708 -> 823; 2048 x 200 k, k = 128: 1255 -> 1496).  Three v_mfma_f32_32x32x16_f16 take 3 / 16 of the time of the fp32 matrix instructions (six with
+// bf16 parts, which hold 8 bits: gradients at k = 64 took 1164 us with those, 794 with these).
 // fp16 has little range, so every tile of 32 rows is scaled by a power of two, its largest finite value to 2^14 .. 2^15: what is 2^-16 of that
 // or more keeps its 22 bits, what is less an absolute error of 2^-40 of it (the scale is 2^40 at most: 2^-65 then).  The scales are taken back
 // exactly where the sums are used.
@@ -94,7 +97,7 @@ __device__ __forceinline__ float block_max(float x, float *s_max) {
 }
 
 // One workgroup per tile of 32 rows of a table: its fragments.  One copy holds row * `by`, the transposed one row * weight[row] (1 without), each with
-// a scale of its own.  Rows without a usable teacher entry (live [32]) count as zeros: they may be padding.  In the transposed copy, which the weights
+// a scale of its own -- the transposed one that of the largest product, so a row of little weight is cut as one of small factors is.  Rows without a usable teacher entry (live [32]) count as zeros: they may be padding.  In the transposed copy, which the weights
 // multiply, so does a factor that is not finite: where it counts the score and with it the row's sum is NaN already, where a mask has taken it out its
 // weight is 0.
 template <int KP>

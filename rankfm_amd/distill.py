@@ -7,11 +7,13 @@ allowed, score not -inf; an item that stands there twice counts twice.
     loss[r] = temperature^2 * sum_j p_j (log p_j - log q[item_j])                   a row without a usable entry: 0
     gradients of sum_r row_weight[r] * loss[r]:  dz = temperature * row_weight * (q - p),  dz . items,  dz^T . users,  column sums
 
-All float32, like the model's weights.  Up to 128 factors the products are made of two half-precision parts per factor, scaled by a power of two per
-tile of 32 consecutive rows of [users] or [items]: as exact as float32 products for factors down to 2^-16 of the largest finite one of
-their tile; below that a factor is off by up to 2^-40 of the largest (or by 2^-65, in a tile that holds nothing above 2^-26).  The weights q and p
-of the gradients are cut likewise: at 2^-40 of the largest that a row has among a tile's 32 items, or an item among a tile's 32 rows.  A factor
-that is not finite spoils the rows it counts in, and nothing where a mask takes it out.  At most 2^24 rows, 2^25 items, 1024 factors and 1024 entries per list.
+All float32, like the model's weights; sums are float32.  Up to 128 factors the products are made of two half-precision parts per factor: a product of two
+factors is off by up to 2^-21 of its size and by 2^-24.2 in the mean (a float32 product: 2^-24, 2^-25.5).  The parts are scaled by a power of two
+per tile of 32 consecutive rows of [users] or [items].  That holds for factors down to 2^-16 of the largest finite one of their tile; below, a factor is off by
+up to 2^-40 of the largest (or by 2^-65, in a tile that holds nothing above 2^-26).  In the items' gradient it is a row's factor times
+its row_weight that counts so.  The weights q and p of the gradients are cut likewise: at 2^-40 of the largest that a row has among a tile's 32
+items, or an item among a tile's 32 rows.  A factor that is not finite spoils the rows it counts in, and nothing where a mask takes it out.  At most
+2^24 rows, 2^25 items, 1024 factors and 1024 entries per list.
 
 The device's current stream; no host synchronisation.  The gradients are returned, not recorded by
 autograd.  Sums have a fixed order: the same call gives the same bits.

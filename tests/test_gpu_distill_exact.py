@@ -191,3 +191,61 @@ def test_the_largest_factors(factors, rows, items):
     want = TAU * TAU * (np.log(items) - np.log(2))
     assert ((got.loss.double() - want).abs() <= 40 * E * (np.log(items) * TAU * TAU)).all()
     assert torch.isfinite(got.users).all() and torch.isfinite(got.items).all()
+
+
+@pytest.mark.parametrize("factors", [8, 64, 128, 256])
+@pytest.mark.parametrize("rows,items", [(40, 21_003), (300, 901)])
+def test_factors_whose_second_parts_are_largest(factors, rows, items):
+    """(1 + 2^-11) 2^j: what a product of two such factors loses (the product of their second parts, 2^-22 of it) has one sign in all of them.  Off by at most
+    2^-21 of the sum of the products' sizes, which enters the loss once (the teacher's scores are float32 products), and the float32 roundings of
+    the scores themselves"""
+    gen = torch.Generator(device="cuda").manual_seed(factors)
+    draw = lambda n: (1 + 2.0 ** -11) * 2.0 ** torch.randint(-1, 2, (n, factors), generator=gen, device="cuda").float() / factors ** 0.5      # noqa: E731
+    users, table = draw(rows), draw(items)
+    ti = torch.randint(0, items, (rows, 4), generator=gen, device="cuda", dtype=torch.int32)
+    t, bias = torch.zeros(rows, 4, device="cuda"), torch.zeros(items, device="cuda")
+    z = users.double() @ table.double().T / TAU
+    lse = torch.logsumexp(z, 1)
+    want = TAU * TAU * (-np.log(4) - z.gather(1, ti.long()).mean(1) + lse)
+    s = float(z.max()) * TAU
+    tol = TAU * TAU * (s * (2.0 ** -21 + 12 * E) + 24 * E * (float(lse.max()) + s) + 2 * factors ** 0.5 * E * s)
+    for loss in (distill_loss(users, table, bias, ti, t, temperature=TAU), distill_gradients(users, table, bias, ti, t, temperature=TAU).loss):
+        assert float((loss.double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128, 200])
+@pytest.mark.parametrize("rows,items", [(40, 21_003), (300, 901)])
+def test_rows_of_very_different_weight_share_a_tile(factors, rows, items):
+    """weights from 2^-12 to 2^12, both signs and 0, in every tile of 32 rows.  In the items' gradient a row's factors times its weight are cut at 2^-40 of the
+    tile's largest such product: 2^-40 of that, times the row's share of the item, comes to a term's bound; the users' gradient and the loss are a
+    row's own"""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    users, table = torch.zeros(rows, factors, device="cuda"), torch.zeros(items, factors, device="cuda")
+    users[torch.arange(rows), torch.arange(rows) % factors] = 1.0
+    table[torch.arange(items), torch.arange(items) // 7 % factors] = 1.0
+    weight = 2.0 ** (torch.arange(rows, device="cuda") % 25 - 12).float() * (1 + torch.rand(rows, generator=gen, device="cuda") / 2)
+    weight[3::5] *= -1
+    weight[4::9] = 0
+    ti = torch.randint(0, items, (rows, 6), generator=gen, device="cuda", dtype=torch.int32)
+    bias = torch.randint(0, 3, (items,), generator=gen, device="cuda").float()
+    t = torch.zeros(rows, 6, device="cuda")
+    z = (users.double() @ table.double().T + bias.double()) / TAU
+    lse = torch.logsumexp(z, 1)
+    q = torch.exp(z - lse[:, None])
+    teacher = torch.zeros_like(q).scatter_add_(1, ti.long(), torch.full(ti.shape, 1 / 6, dtype=torch.float64, device="cuda"))
+    coef = (TAU * weight.double())[:, None]
+    dz, size = (q - teacher) * coef, (q + teacher) * coef.abs()
+    D = float(2 * z.abs().max() + 2 * lse.max()) * 1.4427
+    rel = E * (0.7 * 5 * D + 12 + 14)
+    pad = (-rows) % 32
+    largest = torch.nn.functional.pad(coef.abs()[:, 0], (0, pad)).view(-1, 32).amax(1).repeat_interleave(32)[:rows, None]       # (factors are 1 at most)
+    cut = 2.0 ** -40 * ((q + teacher) * largest).sum(0)[:, None]
+    by_tile = torch.nn.functional.pad(size, (0, 0, 0, pad)).view(-1, 32, items).amax(1).sum(0) * 32 * 2.0 ** -40
+    got = distill_gradients(users, table, bias, ti, t, temperature=TAU, row_weight=weight)
+    per_user = items / max(1, min(16, items // 2048)) + 48 if factors > 128 else items / 32 + 160
+    per_item = rows / 32 + 160 if factors <= 128 else rows + 32
+    for name, x, want, tol in (("users", got.users, dz @ table.double(), (rel + E * per_user) * (size @ table.double())),
+                               ("items", got.items, dz.T @ users.double(), (rel + E * per_item) * (size.T @ users.double()) + cut + by_tile[:, None]),
+                               ("bias", got.bias, dz.sum(0), (rel + E * per_item) * size.sum(0) + by_tile)):
+        off = (x.double() - want).abs() / (tol + 1e-38)
+        assert float(off.max()) <= 1, (name, float(off.max()))
