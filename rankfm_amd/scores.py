@@ -202,6 +202,20 @@ def _byte_range(t):
     return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + (t.shape[1] - 1) * t.stride(1) + 1) * t.element_size()
 
 
+def _overlap(x, y):
+    """whether rows of one shape share an element.  Exact for rows equally far apart, which may lie between each other (halves of wider rows); others
+    overlap if their ranges do"""
+    (a, b), (c, d) = _byte_range(x), _byte_range(y)
+    if b <= c or d <= a:
+        return False
+    rows, items = x.shape
+    stride, size = _row_stride(x), x.element_size()
+    if rows == 1 or _row_stride(y) != stride:
+        return True
+    apart = (c - a) % (stride * size)                            # from a row of x to the next row of y
+    return apart < items * size or apart > (stride - items) * size
+
+
 def adjust_scores(scores, rules, out=None):
     """the score rows under the rules, rounded once to the scores' type
 
@@ -217,10 +231,8 @@ def adjust_scores(scores, rules, out=None):
             raise ValueError("[out] must be a tensor of the scores' type, shape and device")
         if items > 1 and out.stride(1) != 1 or rows > 1 and out.stride(0) < items:
             raise ValueError("[out] must have rows of consecutive items that do not overlap")
-        if rows and (out.data_ptr(), out.stride()) != (scores.data_ptr(), scores.stride()):
-            (a, b), (c, d) = _byte_range(scores), _byte_range(out)
-            if a < d and c < b:
-                raise ValueError("[out] must be [scores] itself or not overlap it")
+        if rows and (out.data_ptr(), _row_stride(out)) != (scores.data_ptr(), _row_stride(scores)) and _overlap(scores, out):
+            raise ValueError("[out] must be [scores] itself or not overlap it")
     u = _rules_struct(rules, rows, items, device)
     if rows == 0:
         return out
