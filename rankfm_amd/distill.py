@@ -24,7 +24,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _hip
-from .scores import allowed_fields, check_device, check_tensor, launch
+from .scores import allowed_fields, check_device, check_tensor, launch, warn_if_cut
 
 
 class DistillGradients(NamedTuple):
@@ -93,7 +93,10 @@ def distill_loss(users, items, bias, teacher_items, teacher_scores, *, temperatu
     users            float32 [rows, factors], items float32 [items, factors] (rows may be strided), bias float32 [items] or None
     teacher_items    int32 [rows, n], -1 for padding; teacher_scores float32 [rows, n]
     allowed, allowed_rows    masks of the items the student's distribution ranges over, as in `ScoreRules`
+
+    The loss cannot be differentiated (its gradients are `distill_gradients`'): with tensors that require a gradient the call warns.
     """
+    warn_if_cut("distill_loss", users, items, bias, teacher_scores)
     return _call(users, items, bias, teacher_items, teacher_scores, temperature, allowed, allowed_rows, None, False)
 
 

@@ -3,9 +3,10 @@
 The reference hands out ranked items only and knows one rule, `filter_previous` (rankfm/_rankfm.pyx:450-451).  Here the caller says what
 else holds: penalties for what a user has already had, biases, and masks of what may be shown at all.  Tensors are torch tensors on one
 MI355X; work is enqueued on that device's current stream and nothing synchronises, so the calls may be captured into a graph.  Nothing is
-recorded by autograd.
+recorded by autograd: a call whose result looks differentiable and is not warns (UserWarning).
 """
 import ctypes as C
+import warnings
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -119,6 +120,17 @@ def check_device(t, name):
     return t.device
 
 
+def warn_if_cut(call, *tensors):
+    """UserWarning where autograd would have followed these tensors into a call's result"""
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if getattr(t, "requires_grad", False):
+            warnings.warn("%s is not recorded by autograd: its result does not depend on tensors that require a gradient (detach them, or call it under "
+                          "torch.no_grad())" % call, UserWarning, stacklevel=3)
+            return
+
+
 def _check_scores(scores):
     if not isinstance(scores, torch.Tensor) or scores.dtype not in _DTYPES or scores.dim() != 2:
         raise ValueError("[scores] must be a float32, float16 or bfloat16 tensor [rows, items]")
@@ -222,6 +234,7 @@ def adjust_scores(scores, rules, out=None):
     scores   float32, float16 or bfloat16 [rows, items], rows of consecutive items (the rows themselves may be strided)
     out      None (a new tensor), `scores` itself (in place), or a tensor of the same type and shape that does not overlap it
     """
+    warn_if_cut("adjust_scores", scores)
     device = _check_scores(scores)
     rows, items = scores.shape
     if out is None:
@@ -246,6 +259,7 @@ def top_scores(scores, n, rules=None):
 
     By descending score, the lower index first among equals; NaN and -inf never rank.  The adjusted rows are not written anywhere.
     """
+    warn_if_cut("top_scores", scores)
     device = _check_scores(scores)
     rows, items = scores.shape
     n = int(n)

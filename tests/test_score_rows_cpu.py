@@ -1,9 +1,12 @@
 """Where score rows lie, and what a call says of tensors that it cannot take: no GPU."""
 import itertools
+import warnings
 
 import pytest
 import torch
 
+import rankfm_amd
+from rankfm_amd import ScoreRules, _hip
 from rankfm_amd.scores import _overlap
 
 
@@ -25,3 +28,17 @@ def test_halves_of_wider_rows_do_not_overlap():
     wide = torch.zeros(4, 10, dtype=torch.bfloat16)
     assert not _overlap(wide[:, :5], wide[:, 5:]) and not _overlap(wide[:, 6:], wide[:, :4])
     assert _overlap(wide[:, :6], wide[:, 4:]) and _overlap(wide[:3], wide[1:])
+
+
+def test_calls_that_cut_the_graph_say_so():
+    """before anything else is looked at: here the calls end for want of a GPU, with the warning given"""
+    scores, ti = torch.zeros(2, 3, requires_grad=True), torch.zeros(2, 1, dtype=torch.int32)
+    calls = [lambda s: rankfm_amd.adjust_scores(s, ScoreRules()), lambda s: rankfm_amd.top_scores(s, 1), lambda s: rankfm_amd.distill_loss(s, torch.zeros(4, 3), None, ti, torch.zeros(2, 1)),
+             lambda s: rankfm_amd.distill_loss(torch.zeros(2, 3), torch.zeros(4, 3), None, ti, s[:, :1].contiguous())]
+    for call in calls:
+        with pytest.warns(UserWarning, match="not recorded by autograd"), pytest.raises((_hip.EngineUnavailable, ValueError)):
+            call(scores)
+        for quiet in (scores.detach(), scores):
+            with warnings.catch_warnings(), torch.set_grad_enabled(quiet is not scores), pytest.raises((_hip.EngineUnavailable, ValueError)):
+                warnings.simplefilter("error")
+                call(quiet)
