@@ -237,6 +237,7 @@ def adjust_scores(scores, rules, out=None):
     warn_if_cut("adjust_scores", scores)
     device = _check_scores(scores)
     rows, items = scores.shape
+    given = out
     if out is None:
         out = torch.empty_like(scores) if scores.is_contiguous() else scores.new_empty((rows, items))
     elif out is not scores:
@@ -251,6 +252,8 @@ def adjust_scores(scores, rules, out=None):
         return out
     launch(device, _hip.lib().rfm_adjust_scores_device, C.byref(u), _DTYPES[scores.dtype], rows, items, scores.data_ptr(), _row_stride(scores), out.data_ptr(),
            _row_stride(out))
+    if given is not None and not given.is_inference():
+        torch.autograd.graph.increment_version(given)            # (a backward pass that has kept it says so instead of using what it is now)
     return out
 
 

@@ -49,6 +49,18 @@ def test_strided_rows_are_adjusted_as_contiguous_ones(dtype):
         assert torch.equal(adjust_scores(s.float(), r).to(dtype), want)          # (one rounding, at the end)
 
 
+def test_autograd_hears_of_a_row_that_changed():
+    x = torch.randn(3, 50, device="cuda", requires_grad=True)
+    y = x.exp()                                                                  # (keeps its result for the backward pass)
+    with torch.no_grad():
+        adjust_scores(y, ScoreRules(item_bias=torch.ones(50, device="cuda")), out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        z = torch.randn(3, 50, device="cuda")
+        adjust_scores(z, ScoreRules(item_bias=torch.ones(50, device="cuda")), out=z)
+
+
 def test_calls_that_cut_the_graph_say_so():
     x = torch.randn(3, 50, device="cuda", requires_grad=True)
     with pytest.warns(UserWarning, match="not recorded by autograd"):
