@@ -126,11 +126,11 @@ __device__ __forceinline__ void scan_lists(const RowRules &w, int first, int *co
     for (int k = threadIdx.x; k < tile; k += kThreads) { count[k] = 0; last[k] = 0; }
     __syncthreads();
     for (long long k = threadIdx.x; k < w.hist_n; k += kThreads) {
-        const unsigned at = (unsigned)(w.hist[k] - first);
+        const unsigned at = (unsigned)w.hist[k] - (unsigned)first;               // (an id may be any 32 bits)
         if (at < (unsigned)tile) atomicAdd(count + at, 1);
     }
     for (long long k = threadIdx.x; k < w.bias_n; k += kThreads) {
-        const unsigned at = (unsigned)(w.bias_item[k] - first);
+        const unsigned at = (unsigned)w.bias_item[k] - (unsigned)first;
         if (at < (unsigned)tile) atomicMax(last + at, (int)k + 1);
     }
     __syncthreads();
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads) adjust_scores_kernel(const rfm_score
         if (w.hist_n > 0 || w.bias_n > 0) {
             __syncthreads();
             auto note = [&](int item, int entry) {
-                if ((unsigned)(item - first) >= (unsigned)(P * kThreads) || item >= n_items) return;
+                if ((unsigned)item - (unsigned)first >= (unsigned)(P * kThreads) || item >= n_items) return;
                 const int at = atomicAdd(&lists.hits.n, 1);
                 if (at < kHits) lists.hits.at[at] = make_int2(item, entry);
             };

@@ -68,3 +68,20 @@ def test_calls_that_cut_the_graph_say_so():
     u, ti = torch.randn(4, 8, device="cuda", requires_grad=True), torch.zeros(4, 2, dtype=torch.int32, device="cuda")
     got = distill_gradients(u, torch.randn(20, 8, device="cuda"), None, ti, torch.zeros(4, 2, device="cuda"))     # (what it is for: no warning)
     assert not got.users.requires_grad and np.isfinite(got.users.cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("entries", [20, 3000], ids=["few", "many"])
+def test_ids_of_any_32_bits(entries):
+    """the smallest and largest ids among those of the catalogue: skipped, on every path that looks at lists"""
+    gen = torch.Generator(device="cuda").manual_seed(entries)
+    for items in (700, 9001):
+        good = torch.randint(0, items, (entries,), generator=gen, device="cuda", dtype=torch.int32)
+        edges = torch.tensor([-2 ** 31, 2 ** 31 - 1, -2 ** 31 + items - 1, -2 ** 31 + 4095, -1, items], dtype=torch.int64).int().cuda()
+        wild = torch.cat([edges, good, edges])
+        scores, value = torch.randn(1, items, device="cuda"), torch.randn(entries + 12, generator=gen, device="cuda")
+        lists = lambda x: (torch.tensor([0, x.numel()], device="cuda"), x)       # noqa: E731
+        a = ScoreRules(history=lists(good), presence=0.5, row_bias=(*lists(good), value[6:-6].contiguous()))
+        b = ScoreRules(history=lists(wild), presence=0.5, row_bias=(*lists(wild), value))
+        assert torch.equal(adjust_scores(scores, a), adjust_scores(scores, b))
+        for x, y in zip(top_scores(scores, 30, a), top_scores(scores, 30, b)):
+            assert torch.equal(x, y)
