@@ -7,6 +7,18 @@ import pytest
 from conftest import ROOT
 
 
+def test_build_compiles_also_where_a_library_is_there(monkeypatch):
+    import __graft_entry__ as entry
+    from rankfm_amd import _build
+    asked = []
+    monkeypatch.setattr(_build, "build", lambda force=False, verbose=False: asked.append(force) or _build.LIB)
+    monkeypatch.setenv("RANKFM_REFERENCE", os.path.join(ROOT, "no such folder"))
+    if not os.path.exists(_build.LIB):
+        pytest.skip("nothing is built")
+    entry.build()
+    assert asked == [True]
+
+
 @pytest.mark.gpu
 def test_the_counters_of_the_bench_line_are_there():
     """bench.py prints `traffic` and the atomic rates from them where it runs"""
