@@ -249,3 +249,23 @@ def test_rows_of_very_different_weight_share_a_tile(factors, rows, items):
                                ("bias", got.bias, dz.sum(0), (rel + E * per_item) * size.sum(0) + by_tile)):
         off = (x.double() - want).abs() / (tol + 1e-38)
         assert float(off.max()) <= 1, (name, float(off.max()))
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128, 200])
+@pytest.mark.parametrize("rows,items", [(40, 21_003), (300, 901)])
+def test_a_factor_that_counts_spoils_its_rows_alone(factors, rows, items):
+    """even rows may have the first half of the catalogue, odd ones the second: a NaN in an item of the first half is in the even rows' losses and gradients, in
+    all of the first half's items, and nowhere else"""
+    torch.manual_seed(factors)
+    half = items // 2
+    users, table, bias = torch.randn(rows, factors, device="cuda") / 4, torch.randn(items, factors, device="cuda") / 4, torch.randn(items, device="cuda")
+    mask = (torch.arange(items, device="cuda") < half)[None] ^ (torch.arange(rows, device="cuda") % 2 == 1)[:, None]
+    ti = torch.randint(0, half, (rows, 4), device="cuda", dtype=torch.int32) + half * (torch.arange(rows, device="cuda") % 2)[:, None].int()
+    t, kw = torch.randn(rows, 4, device="cuda"), dict(allowed=pack_allowed(mask), temperature=1.5)
+    clean = distill_gradients(users, table, bias, ti, t, **kw)
+    table[5, 2] = NAN
+    got, alone = distill_gradients(users, table, bias, ti, t, **kw), distill_loss(users, table, bias, ti, t, **kw)
+    assert torch.isnan(got.loss[::2]).all() and torch.isnan(alone[::2]).all() and torch.isnan(got.users[::2]).all()
+    assert torch.isnan(got.items[:half]).all() and torch.isnan(got.bias[:half]).all()
+    for a, b in ((got.loss[1::2], clean.loss[1::2]), (alone[1::2], clean.loss[1::2]), (got.users[1::2], clean.users[1::2]), (got.items[half:], clean.items[half:]), (got.bias[half:], clean.bias[half:])):
+        assert torch.isfinite(a).all() and torch.allclose(a, b, rtol=1e-4, atol=1e-5)        # (a tile's scale is that of what is finite in it)
