@@ -335,7 +335,8 @@ int rfm_adjust_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_
                              void *dev_out, int64_t out_stride, void *hip_stream);
 
 /* the n best items of every row under `rules` (NULL: none) by descending score, the lower index first among equals, and their scores:
- * int32 / float32 [n_rows, n].  NaN and -inf never rank; rows with fewer than n ranking items end in (-1, -inf). */
+ * int32 / float32 [n_rows, n].  NaN and -inf never rank; rows with fewer than n ranking items end in (-1, -inf).  A pass over the rows for every 768
+ * wanted (384 under rules). */
 size_t rfm_top_scores_workspace_bytes(int64_t n_rows, int32_t n_items, int32_t n);
 int rfm_top_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_t n_rows, int32_t n_items, const void *dev_scores, int64_t stride,
                           int32_t n, int32_t *dev_items, float *dev_values, void *workspace, size_t workspace_bytes, void *hip_stream);

@@ -810,7 +810,9 @@ __global__ void __launch_bounds__(kThreads, 4) top_scores_kernel(const rfm_score
 // How many segments a row is cut into: with few rows, enough to give every CU work, of at least one block of 8192 scores each.  Lists of more than 1024
 // are not cut: every segment would hand that many on.  From 256 rows on joining costs more than the second workgroup per CU gives (400 rows of 17 k, n = 10 / 100 /
 // 450, cut in two: 20.4 / 35.6 / 79.0 us, whole: 12.5 / 19.0 / 44.4; of 190 k: 71 / 129 / 191 and 61 / 129 / 157), but for long rows under rules
-// (500 of 190 k, n = 10: 91 and 118).
+// (500 of 190 k, n = 10: 91 and 118).  Below 256 rows the rule knows the row's length by its blocks alone, and cuts short rows that would be faster
+// whole (255 rows of 17 k, cut, with the call: 25 / 36 / 67 us; 256, whole: 21 / 27 / 50).  Uncut, a long list is walked by one workgroup: one row of
+// 200 k, n = 1024 / 1025 / 5000: 310 / 240 / 979 us.
 constexpr int kBlock = 8192;
 static int top_segments(long long n_rows, int n_items, int n, bool ruled) {
     const long long blocks = ((long long)n_items + kBlock - 1) / kBlock;

@@ -287,7 +287,8 @@ class DeviceSession:
         'v_if'; 'v_u' has one row per user of the call.  With `learning_rate` the weights are moved against them, in place.
 
         users: distinct indexes of the model's users; teacher_items int32 [n, k] (-1 = padding), teacher_scores float32 [n, k], on the device,
-        such as another session's `top_scores` returns them.  The gradients come back as device tensors."""
+        such as another session's `top_scores` returns them.  The gradients come back as device tensors.  The users are checked on the host: a
+        device tensor of them is waited for, and the call cannot be captured into a graph."""
         host = np.asarray(users.cpu() if isinstance(users, torch.Tensor) else users)
         index = np.asarray(host, dtype=np.float64)
         if index.ndim != 1 or not np.all((index >= 0) & (index < self.n_users) & (index == np.floor(index))):

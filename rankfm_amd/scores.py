@@ -261,6 +261,10 @@ def top_scores(scores, n, rules=None):
     """the `n` best items of every row and their scores under the rules: `TopScores(items, scores)`
 
     By descending score, the lower index first among equals; NaN and -inf never rank.  The adjusted rows are not written anywhere.
+
+    One pass over the rows up to 768 wanted (384 under rules); a longer list is taken in rounds of that many, each a pass of its own, and from 1025 on
+    by one workgroup per row: 0.3 ms for 1024 of one row of 200 k, 1.0 ms for 5000, 4.7 ms for 20,000 and 74 ms for all of it (116 under rules).  For a
+    ranking of everything a sort is the better tool.
     """
     warn_if_cut("top_scores", scores)
     device = _check_scores(scores)
