@@ -299,13 +299,13 @@ __global__ void __launch_bounds__(256) softmax_rows_kernel(const rfm_distill_arg
     m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     l = 0.0f;
     for (int w = 0; w < 4; ++w) l += sm[w] > -INFINITY || isnan(sl[w]) ? sl[w] * expf(sm[w] - m) : 0.0f;
-    const float lse = m + logf(l), has = mass[r];
-    if (threadIdx.x == 0) a.loss[r] = has == 0.0f ? 0.0f : a.temperature * a.temperature * (part[r] + has * lse);
+    const float log_l = logf(l), has = mass[r];                  // (m and log l apart: their sum would lose what m is rounded to)
+    if (threadIdx.x == 0) a.loss[r] = has == 0.0f ? 0.0f : a.temperature * (a.temperature * (part[r] + has * (m + log_l)));
     if (!a.d_users) return;
     const float coef = a.temperature * (a.row_weight ? a.row_weight[r] : 1.0f);
     for (int i = threadIdx.x; i < a.n_items; i += 256) {
         const bool ok = !mask || ((mask[i >> 5] >> (i & 31)) & 1u);
-        row[i] = has == 0.0f || bad || !ok ? 0.0f : coef * expf(row[i] * c - lse);
+        row[i] = has == 0.0f || bad || !ok ? 0.0f : coef * expf((row[i] * c - m) - log_l);
     }
     __syncthreads();
     for (int j = threadIdx.x; j < a.n_teacher; j += 256) {

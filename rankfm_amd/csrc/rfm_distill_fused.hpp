@@ -41,7 +41,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kItemData = 64;                    // floats that travel with an item tile: 32 biases (log2 units), 2^-e, e, 2^e, for its scale 2^e
-constexpr int kUserData = 64;                    // ... with a user tile: 32 lse (log2 units), 2^-e of one copy, e and 2^e of the other; and 32 coefficients
+constexpr int kUserData = 64;                    // ... with a user tile: 32 lse (log2 units, whole), 2^-e of one copy, e and 2^e of the other; 32 row weights, 32 rests of the lse
 constexpr int kBuckets = 1024;                   // of a tile's teacher entries, by block of items
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kUnit = 15.0f;                   // a column's largest weight in a tile is 2^14 .. 2^15 (fp16 ends at 2^16)
@@ -103,12 +103,12 @@ __device__ __forceinline__ float block_max(float x, float *s_max) {
 // weight is 0.
 template <int KP>
 __device__ void write_frags(const float *__restrict__ x, long long stride, int tile, long long rows, int factors, float by, const float *live,
-                            const float *__restrict__ weight, float all_weight, char *frag, char *frag_t, float *lds, float *s_weight, float *s_max, int *e_out, int *e_t_out) {
+                            const float *__restrict__ weight, char *frag, char *frag_t, float *lds, float *s_weight, float *s_max, int *e_out, int *e_t_out) {
     constexpr int ld = KP + 1;
     float big = 0.0f, big_t = 0.0f;
     if (threadIdx.x < 32) {
         const long long r = (long long)tile * 32 + threadIdx.x;
-        s_weight[threadIdx.x] = weight && r < rows ? weight[r] * all_weight : all_weight;
+        s_weight[threadIdx.x] = weight && r < rows ? weight[r] : 1.0f;
     }
     Four v[KP / 32];                                             // all of a thread's loads first
 #pragma unroll
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c
             if (sub == 0) live[row] = (any >> ((threadIdx.x & 63) & ~7)) & 0xff ? 1.0f : 0.0f;
         }
         __syncthreads();
-        write_frags<KP>(a.users, a.user_stride, b, a.n_rows, a.n_factors, c, live, GRAD ? a.row_weight : nullptr, a.temperature, f.user_frag, GRAD ? f.user_frag_t : nullptr, lds, s_weight, s_max, &e, &e_t);
+        write_frags<KP>(a.users, a.user_stride, b, a.n_rows, a.n_factors, c, live, GRAD ? a.row_weight : nullptr, f.user_frag, GRAD ? f.user_frag_t : nullptr, lds, s_weight, s_max, &e, &e_t);
         if (threadIdx.x == 0) {
             f.user_data[(size_t)b * kUserData + 32] = ldexpf(1.0f, -e);
             f.user_data[(size_t)b * kUserData + 33] = (float)e_t;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const FusedArgs f, float c
         }
     } else {
         const int t = b - f.user_tiles;
-        write_frags<KP>(a.items, a.item_stride, t, a.n_items, a.n_factors, 1.0f, nullptr, nullptr, 1.0f, f.item_frag, GRAD ? f.item_frag_t : nullptr, lds, s_weight, s_max, &e, &e_t);
+        write_frags<KP>(a.items, a.item_stride, t, a.n_items, a.n_factors, 1.0f, nullptr, nullptr, f.item_frag, GRAD ? f.item_frag_t : nullptr, lds, s_weight, s_max, &e, &e_t);
         float *data = f.item_data + (size_t)t * kItemData;
         if (threadIdx.x < 32) {
             const long long i = (long long)t * 32 + threadIdx.x;
@@ -245,10 +245,11 @@ __device__ __forceinline__ void staged() {
 }
 
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-// c + (ah + am) (bh + bm), the small products first
+// c + (ah + am) (bh + bm), the small products first; SWAP: those in the other order
+template <bool SWAP = false>
 __device__ __forceinline__ f32x16 mfma3(const f16x8 *a, const f16x8 *b, f32x16 c) {
-    c = mfma(a[1], b[0], c);
-    c = mfma(a[0], b[1], c);
+    c = SWAP ? mfma(a[0], b[1], c) : mfma(a[1], b[0], c);
+    c = SWAP ? mfma(a[1], b[0], c) : mfma(a[0], b[1], c);
     return mfma(a[0], b[0], c);
 }
 // the two parts of the 16 weights.  x - h in one instruction (v_fma_mix_f32 takes a half of a packed pair as a factor); the compiler makes three
@@ -293,7 +294,9 @@ __device__ __forceinline__ void weighted_sum(const char *tile_t, int lane, const
             for (int r = 0; r < 16; ++r) o[n][c][r] = fmaf(sum[n][r], unit[n], o[n][c][r]);
     }
 }
-template <int KP, int NC>
+// SWAP: the columns are the items (the same sums in the same order as where they are the rows: a score has the same bits in both kernels, so that the largest
+// share of a row is as exact as the row's sum, however large the scores are)
+template <int KP, int NC, bool SWAP = false>
 __device__ __forceinline__ void tile_scores(const char *tile, int lane, const f16x8 (*x)[Frag<KP>::steps][2], f32x16 *s) {
 #pragma unroll
     for (int n = 0; n < NC; ++n) s[n] = f32x16{0};
@@ -302,7 +305,7 @@ __device__ __forceinline__ void tile_scores(const char *tile, int lane, const f1
         const f16x8 *at = reinterpret_cast<const f16x8 *>(tile) + k * 128 + lane;
         const f16x8 a[2] = {at[0], at[64]};
 #pragma unroll
-        for (int n = 0; n < NC; ++n) s[n] = mfma3(a, x[n][k], s[n]);
+        for (int n = 0; n < NC; ++n) s[n] = mfma3<SWAP>(a, x[n][k], s[n]);
     }
 }
 template <int KP>
@@ -349,18 +352,23 @@ __device__ __forceinline__ float sum16(const f32x16 &s) {
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// A weight 2^x is cut into its two parts as 2^(x - high + 15), `high` being the least whole number that none of its column's in the tile is above: the parts
+// A weight 2^x is cut into its two parts as 2^(x - off), off = high - 15, `high` being the least whole number that none of its column's in the tile is above: the parts
 // end at 2^-25, 2^-40 of the column's largest weight in the TILE.  (With one unit for all tiles, the column's largest so far, they ended at 2^-32 of that:
 // of 200 k items 16 nats below the first the users' gradient lost 1.4e-3, at 20 nats a tenth, and an item on a teacher's list the shares of all other users
-// below 2^-9 of its own.)  The running sums are in units of 2^(top - 15), top >= high - e - 8 for a tile whose values are scaled by 2^e: what a tile
-// gives is multiplied by 2^(high - e - top) where it is added, and `top` moved only when that would pass 2^8 -- by 24 more than it has to be, so that a
+// below 2^-9 of its own.)  The running sums are in units of 2^top, top >= off - e - 8 for a tile whose values are scaled by 2^e: what a tile
+// gives is multiplied by 2^(off - e - top) where it is added, and `top` moved only when that would pass 2^8 -- by 24 more than it has to be, so that a
 // column is moved once and not at every larger tile (an item's first entry of a teacher's list is some 2^13 above its shares: gradients of 8192 rows x
 // 50 k items at k = 64, 702 us without, 691 with).  All of these are the same in both halves of the wavefront, and whole numbers, so that every scale is
 // an exact power of two (a fractional one rounds differently where it is put in and where it is taken out: up to 7e-7 of a column).
+__device__ __forceinline__ float below(float high) {
+    const float off = high - kUnit;
+    return high - off > kUnit ? high - 7.0f : off;               // (beyond 2^24 a step of float32 is 2 and more: 2^16 would be infinite in fp16)
+}
 template <int COLS>
-__device__ __forceinline__ float tile_unit(float level, float &top, float &total, f32x16 (&o)[COLS]) {
-    if (__any(level > top + kSlack)) {                           // (kLowest + 8 is kLowest: a column's first weight moves it)
-        const float to = level > top + kSlack ? level + kHead : top, by = __builtin_amdgcn_exp2f(top - to);
+__device__ __forceinline__ float tile_unit(float off, float e, float &top, float &total, f32x16 (&o)[COLS]) {
+    const float over = (off - top) - e;
+    if (__any(over > kSlack)) {                                  // (top is kLowest at first)
+        const float to = over > kSlack ? (off - e) + kHead : top, by = __builtin_amdgcn_exp2f(top - to);
         top = to;
         total *= by;
 #pragma unroll
@@ -368,11 +376,10 @@ __device__ __forceinline__ float tile_unit(float level, float &top, float &total
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[c][r] *= by;
     }
-    return __builtin_amdgcn_exp2f(level - top);
+    return __builtin_amdgcn_exp2f((off - top) - e);
 }
 // the weights of exponents s, and their sum
-__device__ __forceinline__ float weigh(f32x16 &s, float high) {
-    const float off = high - kUnit;
+__device__ __forceinline__ float weigh(f32x16 &s, float off) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - off);
     return sum16(s);
@@ -462,8 +469,9 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (GRAD ? kPerSimd<KP, NC>
             if constexpr (MASK) mask16(s[n], word[n] >> (4 * half));
             if constexpr (GRAD) {
                 const float high = fmaxf(ceilf(both_halves(largest16(s[n]))), kLowest);      // (kLowest: nothing is allowed, all weights are 0)
-                by[n] = tile_unit(high - e, top[n], total[n], o[n]);
-                total[n] = fmaf(weigh(s[n], high), by[n] * scale, total[n]);
+                const float off = below(high);
+                by[n] = tile_unit(off, e, top[n], total[n], o[n]);
+                total[n] = fmaf(weigh(s[n], off), by[n] * scale, total[n]);
             } else add_weights(s[n], top[n], total[n]);
         }
         if constexpr (GRAD) {
@@ -615,9 +623,9 @@ __global__ void __launch_bounds__(kThinWaves * 64, (kThinPerSimd<KP, GRAD>)) thi
         if constexpr (MASK) mask16(s, word >> (4 * half));
         float by = 1.0f;
         if constexpr (GRAD) {
-            const float high = fmaxf(ceilf(both_halves(largest16(s))), kLowest);
-            by = tile_unit(high - e, top, total, o);
-            total = fmaf(weigh(s, high), by * scale, total);
+            const float off = below(fmaxf(ceilf(both_halves(largest16(s))), kLowest));
+            by = tile_unit(off, e, top, total, o);
+            total = fmaf(weigh(s, off), by * scale, total);
         } else add_weights(s, top, total);
         if constexpr (GRAD) {
             f16x8 p[2][2];
@@ -696,7 +704,7 @@ __device__ void join_row(const FusedArgs &f, long long r, int share, const float
             if (grad)
                 for (int k = lane; k < f.a.n_factors; k += 64) f.a.d_users[(size_t)r * f.a.n_factors + k] = 0.0f;
         }
-        if (grad && lane == 0) { f.user_data[at] = INFINITY; f.user_data_t[at] = 0.0f; }
+        if (grad && lane == 0) { f.user_data[at] = INFINITY; f.user_data_t[at] = 0.0f; f.user_data_t[at + 32] = 0.0f; }
         return;
     }
     float top = kLowest;
@@ -762,11 +770,13 @@ __device__ void join_row(const FusedArgs &f, long long r, int share, const float
             }
         }
     }
-    const float lse2 = top - kUnit + log2f(total);
-    if (lane == 0) f.a.loss[r] = f.a.temperature * f.a.temperature * (part[r] + lse2 * 0.693147180559945309f);
+    // lse (log2 units) as a whole number and a rest, neither of which loses what the other is rounded to
+    const int power = total > 0.0f && total < INFINITY ? ilogbf(total) : 0;
+    const float lse2 = top + (float)power, rest = log2f(ldexpf(total, -power)) + ((top - lse2) + (float)power);
+    if (lane == 0) f.a.loss[r] = f.a.temperature * (f.a.temperature * (part[r] + (lse2 + rest) * 0.693147180559945309f));
     if (!grad) return;
-    const float coef = f.a.temperature * (f.a.row_weight ? f.a.row_weight[r] : 1.0f);
-    if (lane == 0) { f.user_data[at] = lse2; f.user_data_t[at] = coef; }
+    const float weight_of = f.a.row_weight ? f.a.row_weight[r] : 1.0f, coef = f.a.temperature * weight_of;
+    if (lane == 0) { f.user_data[at] = lse2; f.user_data_t[at] = weight_of; f.user_data_t[at + 32] = rest; }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int k = k4 + j;
@@ -932,30 +942,28 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
             next_entry = entry_of(t + 1, begin);
             if (t + 1 < t1) stage(t + 1);
             f32x16 s[NC];
-            tile_scores<KP, NC>(now, lane, x, s);
+            tile_scores<KP, NC, true>(now, lane, x, s);
             const f32x4 *data = reinterpret_cast<const f32x4 *>(now + 2 * kBytes);
             const f32x4 last = data[8];
             const float e = last[1], scale = last[2];
             // a tile without a live row gives nothing, whatever the items hold.  (Beside a live one no row is without all items: where those are not finite
             // the live row's own share is not, either)
             if (!entries) continue;
-            float high[NC];
+            float high[NC], off[NC];
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-                // the exponents of the weights but for the column's bias
                 const float unit = unscaled(last[0], unscale[n]);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 lse = data[half + 2 * q];
+                for (int q = 0; q < 4; ++q) {                    // log2 of the shares: z as forward_kernel has it, less the row's lse
+                    const f32x4 lse = data[half + 2 * q], rest = data[kUserData / 4 + 8 + half + 2 * q];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[n][4 * q + k] = fmaf(s[n][4 * q + k], unit, -lse[k]);
+                    for (int k = 0; k < 4; ++k) s[n][4 * q + k] = (fmaf(s[n][4 * q + k], unit, bias[n]) - lse[k]) - rest[k];
                 }
                 if constexpr (MASK) mask16_rows(s[n], word[n]);
-                const float most = both_halves(largest16(s[n])), b = most == -INFINITY ? 0.0f : bias[n];       // (no row has it: its bias may be anything)
-                high[n] = fmaxf(ceilf(most + b), kLowest);
-                const float off = b - (high[n] - kUnit);
+                high[n] = fmaxf(ceilf(both_halves(largest16(s[n]))), kLowest);
+                off[n] = below(high[n]);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r] + off);
+                for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - off[n]);
             }
             // the teacher's share
             unsigned any = 0;                                    // a bit per column tile that is hit
@@ -985,12 +993,12 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
                     }
                     const float log_p = both_halves(__builtin_amdgcn_logf(__uint_as_float(most)));       // (-inf where there is none)
                     if (__any(log_p > high[n])) {
-                        const float to = fmaxf(high[n], ceilf(log_p)), by_p = __builtin_amdgcn_exp2f(high[n] - to);
+                        const float to = below(fmaxf(high[n], ceilf(log_p))), by_p = __builtin_amdgcn_exp2f(off[n] - to);
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s[n][r] *= by_p;
-                        high[n] = to;
+                        off[n] = to;
                     }
-                    const float unit = fminf(__builtin_amdgcn_exp2f(kUnit - high[n]), -kLowest);      // (finite where a column has no weight: 0 stays 0)
+                    const float unit = fminf(__builtin_amdgcn_exp2f(-off[n]), -kLowest);      // (finite where a column has no weight: 0 stays 0)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -1003,7 +1011,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
             float by[NC];
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-                by[n] = tile_unit(high[n] - e, top[n], d_bias[n], o[n]);
+                by[n] = tile_unit(off[n], e, top[n], d_bias[n], o[n]);
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -1022,15 +1030,17 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const float sum = d_bias[n] + __shfl_xor(d_bias[n], 32);
-            // out of their unit 2^(top - 15), which may be below float32's smallest where its sums are not: by the exponent, not by a factor
-            const int unit = (int)fminf(fmaxf(top[n] - kUnit, -1000.0f), 1000.0f);
+            // out of their unit 2^top, which may be below float32's smallest where its sums are not: by the exponent, not by a factor
+            const int unit = (int)fminf(fmaxf(top[n], -1000.0f), 1000.0f);
+            const float tau = f.a.temperature;
             auto out_of_unit = [&](int c, int q) {
-                return f32x4{ldexpf(o[n][c][4 * q], unit), ldexpf(o[n][c][4 * q + 1], unit), ldexpf(o[n][c][4 * q + 2], unit), ldexpf(o[n][c][4 * q + 3], unit)};
+                const f32x4 v = f32x4{o[n][c][4 * q], o[n][c][4 * q + 1], o[n][c][4 * q + 2], o[n][c][4 * q + 3]} * tau;
+                return f32x4{ldexpf(v[0], unit), ldexpf(v[1], unit), ldexpf(v[2], unit), ldexpf(v[3], unit)};
             };
             const int item = (tile + n) * 32 + col;
             if (whole && item < f.a.n_items) {
                 float *out = f.a.d_items + (size_t)item * K;
-                if (half == 0 && f.a.d_bias) f.a.d_bias[item] = ldexpf(sum, unit);
+                if (half == 0 && f.a.d_bias) f.a.d_bias[item] = ldexpf(sum * tau, unit);
 #pragma unroll
                 for (int c = 0; c < Frag<KP>::cols; ++c)
 #pragma unroll
@@ -1041,7 +1051,7 @@ __global__ void __launch_bounds__(Frag<KP>::waves * 64, (kPerSimd<KP, NC>)) item
                     }
             } else if (!whole) {
                 const size_t at = ((size_t)(blockIdx.x + block) * WAVES * NC + wave * NC + n) * 32 + col;
-                if (half == 0) f.part_bias[at] = ldexpf(sum, unit);
+                if (half == 0) f.part_bias[at] = ldexpf(sum * tau, unit);
 #pragma unroll
                 for (int c = 0; c < Frag<KP>::cols; ++c)
 #pragma unroll

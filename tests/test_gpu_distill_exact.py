@@ -269,3 +269,44 @@ def test_a_factor_that_counts_spoils_its_rows_alone(factors, rows, items):
     assert torch.isnan(got.items[:half]).all() and torch.isnan(got.bias[:half]).all()
     for a, b in ((got.loss[1::2], clean.loss[1::2]), (alone[1::2], clean.loss[1::2]), (got.users[1::2], clean.users[1::2]), (got.items[half:], clean.items[half:]), (got.bias[half:], clean.bias[half:])):
         assert torch.isfinite(a).all() and torch.allclose(a, b, rtol=1e-4, atol=1e-5)        # (a tile's scale is that of what is finite in it)
+
+
+@pytest.mark.parametrize("factors", [20, 64, 128, 200])
+@pytest.mark.parametrize("rows,items", [(40, 21_003), (300, 901), (4100, 33_000)])
+@pytest.mark.parametrize("masked", [False, True], ids=["", "masked"])
+def test_next_to_no_temperature(factors, rows, items, masked):
+    """temperatures at which a step of float32 in a score is more than all of the softmax: q is 1 for the best item, which leads by at least 0.001 here (100 times
+    the largest temperature, and a score is off by 2^-21 of the sum of its products' sizes, 10 at most), and the gradients are plain differences of rows"""
+    if rows * items > 30_000_000 and (factors not in (20, 64) or masked):
+        pytest.skip("two column tiles per wavefront: up to 64 factors, without masks")
+    torch.manual_seed(rows + factors)
+    users, table = torch.zeros(rows, factors, device="cuda"), torch.rand(items, factors, device="cuda") / 2
+    best = torch.randint(0, items, (rows,), device="cuda")
+    users[torch.arange(rows), torch.arange(rows) % factors] = torch.rand(rows, device="cuda") * 7 + 1
+    table[best, torch.arange(rows, device="cuda") % factors] = 1.0                # (several of these lead where rows share a factor: the bias decides)
+    bias = torch.rand(items, device="cuda") * 0.3
+    ti = torch.randint(0, items, (rows, 3), device="cuda", dtype=torch.int32)
+    mask = torch.rand(1, items, device="cuda") < 0.7 if masked else None
+    z = users.double() @ table.double().T + bias.double()
+    usable = torch.ones_like(ti, dtype=torch.bool)
+    if masked:
+        z = torch.where(mask, z, -INF)
+        usable = mask.expand(rows, -1).gather(1, ti.long())
+    top2 = z.topk(2, dim=1).values
+    clear = (top2[:, 0] - top2[:, 1] > 1e-3) & usable.any(1)
+    ti[~clear] = -1                                                              # (rows without a clear best have nothing to learn)
+    usable &= clear[:, None]
+    t = torch.zeros(rows, 3, device="cuda")
+    p = usable.double() / usable.sum(1, keepdim=True).clamp(min=1)
+    dz = torch.zeros_like(z).scatter_(1, z.argmax(1, keepdim=True), clear[:, None].double()).scatter_add_(1, ti.long().clamp(min=0), -p)
+    size = dz.abs()
+    for tau in (1e-5, 3e-6, 1e-6, 3e-7, 1e-7, 3e-8, 1e-9, 1e-12, 1e-20):
+        kw = dict(temperature=tau, allowed=None if mask is None else pack_allowed(mask))
+        got, alone = distill_gradients(users, table, bias, ti, t, **kw), distill_loss(users, table, bias, ti, t, **kw)
+        for name, x, want, tol in (("users", got.users, dz @ table.double(), size @ table.double()), ("items", got.items, dz.T @ users.double(), size.T @ users.double()),
+                                   ("bias", got.bias, dz.sum(0), size.sum(0))):
+            off = (x.double() / tau - want).abs() / (1e-4 * tol + 1e-30)
+            assert float(off.max()) <= 1, (name, tau, float(off.max()))
+        want = tau * (top2[:, 0] - (torch.where(usable, z.gather(1, ti.long().clamp(min=0)), 0.0) * p).sum(1)) * clear
+        for loss in (got.loss, alone):
+            assert ((loss.double() - want).abs() <= 1e-4 * tau * 10).all(), tau
