@@ -24,12 +24,12 @@
 //   thin_forward_kernel   the same for one or two tiles of users over a large table, which it takes as it is: no copies of the items.
 //   items_kernel     columns: 32 or 64 items per wavefront, fixed; streams user tiles.  z = users . items^T, dz from the row's lse, O^T += users^T . dz.
 //
-// What bounds them: 8192 rows x 50 k items at k = 64, lists of 32, gradients: 0.70 ms in all, of which forward_kernel 320 us, items_kernel 400, prepare 24, the joins 14 and
-// 12 (under a profiler, which adds a few percent).  2 x 6 x 8192 x 50 k x 64 x 2 operations are 0.63 TFLOP: 393 us at
+// What bounds them: 8192 rows x 50 k items at k = 64, lists of 32, gradients: 0.71 ms in all, of which forward_kernel 323 us, items_kernel 420, prepare 24, the joins 14 and
+// 11 (under a profiler, which adds a few percent).  2 x 6 x 8192 x 50 k x 64 x 2 operations are 0.63 TFLOP: 393 us at
 // the 1.6 PFLOP/s that a loop of nothing but these instructions holds (its power sets its clock).  The matrix cores are busy in 53 % of the
-// cycles of forward_kernel and 41 % of items_kernel; vector instructions issue in 50 % of both.  In copies: no LDS reads of the streamed tiles -18 .. -27 %,
+// cycles of forward_kernel and 39 % of items_kernel; vector instructions issue in 53 % of both.  In copies: no LDS reads of the streamed tiles -18 .. -27 %,
 // no teacher's entries -5 %, no test for a larger maximum -2 .. -4 %, no exponentials or a higher wave priority next to nothing.  The loss alone:
-// 173 us.  2048 rows x 200 k items at k = 128: 1.27 ms, of which 560 + 698; 64 % and 47 %.
+// 165 us.  2048 rows x 200 k items at k = 128: 1.27 ms, of which 549 + 706; 63 % and 46 %.
 #pragma once
 
 namespace rfm {
