@@ -384,7 +384,7 @@ __device__ __forceinline__ float weigh(f32x16 &s, float off) {
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - off);
     return sum16(s);
 }
-// Where nothing but their sum is wanted they are not cut, and the unit is the column's largest so far (50 k items, k = 64, 8192 rows: 179 us; 185 with a unit
+// Where nothing but their sum is wanted they are not cut, and the unit is the column's largest so far (50 k items, k = 64, 8192 rows: 174 us; 185 with a unit
 // per tile)
 __device__ __forceinline__ void add_weights(f32x16 &s, float &top, float &total) {
     const float high = largest16(s);
