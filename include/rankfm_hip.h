@@ -356,7 +356,7 @@ int rfm_top_scores_device(const rfm_score_rules *rules, int32_t dtype, int64_t n
 typedef struct rfm_distill_args {
     int64_t n_rows;
     int32_t n_items, n_factors, n_teacher;
-    float temperature;                /* > 0 */
+    float temperature;                /* 2^-126 at least, finite */
     const float *users;               /* [n_rows, n_factors], rows user_stride apart */
     const float *items;               /* [n_items, n_factors], rows item_stride apart */
     int64_t user_stride, item_stride;

@@ -340,7 +340,7 @@ namespace distill {
 
 static int check(const rfm_distill_args *a) {
     if (!a || a->n_rows < 0 || a->n_items < 1 || a->n_factors < 1 || a->n_teacher < 1) return RFM_ERR_BAD_ARG;
-    if (!(a->temperature > 0.0f && a->temperature < INFINITY)) return RFM_ERR_BAD_ARG;
+    if (!(a->temperature >= 0x1p-126f && a->temperature < INFINITY)) return RFM_ERR_BAD_ARG;      // (below, its inverse is infinite)
     if (a->user_stride < a->n_factors || a->item_stride < a->n_factors) return RFM_ERR_BAD_ARG;
     if (a->allowed && (a->n_allowed < 1 || (!a->allowed_rows && a->n_allowed != 1 && a->n_allowed < a->n_rows))) return RFM_ERR_BAD_ARG;
     if (!a->d_users != !a->d_items || (a->d_bias && !a->d_items)) return RFM_ERR_BAD_ARG;

@@ -62,8 +62,8 @@ def _call(users, items, bias, teacher_items, teacher_scores, temperature, allowe
     if a.n_teacher < 1 or a.n_teacher > 1024:
         raise ValueError("[teacher_items] must have between 1 and 1024 entries per row")
     a.temperature = float(temperature)
-    if not 0.0 < a.temperature < float("inf"):
-        raise ValueError("[temperature] must be a finite number above 0")
+    if not 2.0 ** -126 <= a.temperature < float("inf"):          # (below, its inverse is infinite in float32)
+        raise ValueError("[temperature] must be a finite number above 0, 2^-126 at least")
     allowed_fields(a, allowed, allowed_rows, rows, a.n_items, device)
     if row_weight is not None:
         a.row_weight = check_tensor(row_weight, "row_weight", torch.float32, (rows,), device)

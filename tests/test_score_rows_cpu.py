@@ -1,4 +1,5 @@
 """Where score rows lie, and what a call says of tensors that it cannot take: no GPU."""
+import ctypes as C
 import itertools
 import warnings
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 import rankfm_amd
-from rankfm_amd import ScoreRules, _hip
+from rankfm_amd import ScoreRules, _build, _hip
 from rankfm_amd.scores import _overlap
 
 
@@ -42,3 +43,16 @@ def test_calls_that_cut_the_graph_say_so():
             with warnings.catch_warnings(), torch.set_grad_enabled(quiet is not scores), pytest.raises((_hip.EngineUnavailable, ValueError)):
                 warnings.simplefilter("error")
                 call(quiet)
+
+
+def test_temperatures_without_an_inverse_are_refused():
+    _build.build()
+    lib = _hip.lib()
+
+    def args(t):
+        return _hip.DistillArgs(n_rows=2, n_items=8, n_factors=4, n_teacher=2, temperature=t, users=64, items=64, user_stride=4, item_stride=4, teacher_items=64, teacher_scores=64, loss=64)
+    for t in (0.0, 1e-39, 2.0 ** -127, -1.0, float("nan"), float("inf")):
+        assert lib.rfm_distill_workspace_bytes(C.byref(args(t))) == 0
+        assert lib.rfm_distill_device(C.byref(args(t)), C.c_void_p(64), 1 << 40, None) == _hip.ERR_BAD_ARG, t
+    for t in (2.0 ** -126, 1e-20, 1.0, 3e38):
+        assert lib.rfm_distill_workspace_bytes(C.byref(args(t))) > 0
